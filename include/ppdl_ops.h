@@ -262,6 +262,109 @@ PPDL_OPS_API int ppdl_gemm_tf32x3_split_k(int M, int N, int K, const float * A, 
                                           const float * res, int act, int splits, float * ws,
                                           float * C, void * stream);
 
+/* ---- operators of a transformer block around the attention core -------------
+   No counterpart in the reference (its layer norm is ggml_norm -> mul -> add,
+   src/ppdoclayout.cpp:550-554, and its linears are FP32): layer norm over
+   rows of any width with its backward pass, linear layers in 8-bit integers,
+   and rotary positions with several axes.  FP32, BF16 or FP16 rows; sums,
+   statistics and angles are kept in 32 bits or more and every result is
+   rounded once, to nearest even.  Rows lie ld elements apart (ld >= their
+   width, any alignment of the element type; not used for a single row);
+   elements of a row are contiguous.  Outputs may not overlap inputs unless stated.  Strides and
+   offsets are 64-bit.  Zero rows are allowed everywhere. */
+#define PPDL_F32  0
+#define PPDL_BF16 1
+#define PPDL_F16  2
+
+/* y = (s - mean) * rstd * weight + bias per row, s = x (+ res), mean and
+   variance over the row's D elements, rstd = 1 / sqrt(variance + eps).  With
+   a residual s is rounded to the element type first, and stored in sum when
+   sum is given (what the backward pass takes as its x).  weight and bias
+   [D], of the rows' type or FP32 (w_type), each may be NULL; mean and rstd
+   [rows] may be NULL.  y may be x or res (same pointer and ld) and sum the
+   other of them, or y one and sum NULL.  eps >= 0.
+   Returns PPDL_OK / PPDL_ERR_SHAPE / PPDL_ERR_CUDA. */
+PPDL_OPS_API int ppdl_layernorm(const void * x, long long ldx, const void * res, long long ldres,
+                                const void * weight, const void * bias, int type, int w_type,
+                                long long rows, int D, float eps, void * y, long long ldy,
+                                void * sum, long long ldsum, float * mean, float * rstd,
+                                void * stream);
+
+/* The backward pass of ppdl_layernorm at input x (its sum when it had a
+   residual) with the statistics it returned:
+     xh = (x - mean) * rstd, g = dy * weight,
+     dx = rstd * (g - mean(g) - xh * mean(g * xh)) (+ dsum),
+     dweight = sum over rows of dy * xh, dbias = sum over rows of dy.
+   dsum (may be NULL) is the gradient that reaches the stored sum on its
+   other path; dx is then the gradient of x and of the residual alike.
+   dweight and dbias [D] of w_type may be NULL; when either is given, work
+   holds ppdl_layernorm_backward_workspace(rows, D) floats, 16-byte aligned,
+   for this call alone.  The sums over rows run in an order that depends on
+   the sizes and the GPU's number of SMs alone.
+   Returns PPDL_OK / PPDL_ERR_SHAPE / PPDL_ERR_CUDA. */
+PPDL_OPS_API int ppdl_layernorm_backward(const void * dy, long long lddy, const void * x,
+                                         long long ldx, const void * weight, const float * mean,
+                                         const float * rstd, const void * dsum, long long lddsum,
+                                         int type, int w_type, long long rows, int D, void * dx,
+                                         long long lddx, void * dweight, void * dbias,
+                                         float * work, void * stream);
+PPDL_OPS_API long long ppdl_layernorm_backward_workspace(long long rows, int D);
+
+/* 8-bit rows of x [rows][K]: scale[m] = max |x(m, .)| / 127 (rounded to
+   FP32), q(m, k) = x(m, k) / scale[m] rounded half to even, decided on the
+   exact quotient, in [-127, 127].  A row of zeros has scale 0 and q 0; a row
+   that holds an infinity or a NaN has a scale of that kind and q 0.  q: rows
+   ldq bytes apart, ldq a multiple of 16, q 16-byte aligned; bytes past K are
+   not written. */
+PPDL_OPS_API int ppdl_quantize_rows_i8(const void * x, long long ldx, int type, long long rows,
+                                       int K, int8_t * q, long long ldq, float * scale,
+                                       void * stream);
+
+/* The linear layer on 8-bit rows:
+     y(m, n) = act(sum_k q(m, k) w(n, k) * q_scale[m] * w_scale[n] + bias[n]) + res(m, n)
+   q [M][K] with a scale per token, w [N][K] with a scale per output channel
+   (ppdl_quantize_rows_i8 makes both), any 8-bit values; the integer sums are
+   exact.  ldq and ldw are multiples of 16 bytes, q and w 16-byte aligned;
+   bytes past K are ignored.  bias [N] FP32 and res may be NULL; res and y
+   are of `type`; y may be res (same pointer and ld).  act 0/1/2/3 =
+   none/ReLU/SiLU/GELU.  1 <= K <= 131071 (the sums fit 32 bits).
+   Returns PPDL_OK / PPDL_ERR_SHAPE / PPDL_ERR_CUDA. */
+PPDL_OPS_API int ppdl_linear_i8(const int8_t * q, long long ldq, const float * q_scale,
+                                const int8_t * w, long long ldw, const float * w_scale,
+                                const float * bias, const void * res, long long ldres, int type,
+                                int act, int M, int N, int K, void * y, long long ldy,
+                                void * stream);
+
+/* Heads of ppdl_rotary: value d of head h of token t of sequence b lies at
+   b*batch + t*token + h*head + d (elements). */
+typedef struct {
+    const void * in;
+    void *       out;    /* may be in, with the same strides */
+    int32_t      heads;  /* 0: none */
+    int64_t      in_batch, in_token, in_head;
+    int64_t      out_batch, out_token, out_head;
+} ppdl_rotary_heads;
+
+/* Rotary positions with several axes (time, height, width, ...) on queries
+   and keys in one launch (q or k may be NULL).  Of every head's dim values
+   (at most 1024) the first `rotated` are turned in pairs, the others copied:
+     angle(i) = position[axis(i)] * freq[i]  (64-bit, exact to about 2^-50 turns
+                                              per turn)
+     (a, b) -> (a cos - b sin, b cos + a sin)
+   pair i is (x[i], x[i + rotated/2]), or (x[2i], x[2i + 1]) when interleaved;
+   sections[0 .. axes-1] (host memory) are the numbers of consecutive pairs
+   that each of the 1..4 axes turns, rotated/2 together.  The position of
+   token t of sequence b on axis a is the 32-bit or 64-bit integer
+   positions[a*axis_stride + b*batch_stride + t*token_stride] (a stride may be
+   0); freq [rotated/2] is device memory, in radians per position.  inverse
+   != 0 turns back: the backward pass.
+   Returns PPDL_OK / PPDL_ERR_SHAPE / PPDL_ERR_CUDA. */
+PPDL_OPS_API int ppdl_rotary(const ppdl_rotary_heads * q, const ppdl_rotary_heads * k, int type,
+                             int batch, int length, int dim, int rotated, const void * positions,
+                             int position_bytes, long long axis_stride, long long batch_stride,
+                             long long token_stride, int axes, const int32_t * sections,
+                             const double * freq, int interleaved, int inverse, void * stream);
+
 /* Human-readable text of the last error of ppdl_op_launch on this thread. */
 PPDL_OPS_API const char * ppdl_op_last_error(void);
 

@@ -1,0 +1,60 @@
+// block.cuh — element types and small device helpers of the transformer-block
+// operators (layernorm.cu, linear_i8.cu, rotary.cu).
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+
+namespace ppdl {
+
+// Element types of the block operators (PPDL_F32 / PPDL_BF16 / PPDL_F16).
+enum ElemType : int { T_F32 = 0, T_BF16 = 1, T_F16 = 2 };
+
+inline int elem_size(int type) { return type == T_F32 ? 4 : 2; }
+inline bool elem_type_ok(int type) { return type >= T_F32 && type <= T_F16; }
+
+__device__ __forceinline__ float to_float(float v) { return v; }
+__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
+
+// Round to nearest even, the only rounding of a result to fewer bits.
+template <typename T>
+__device__ __forceinline__ T from_float(float v);
+template <>
+__device__ __forceinline__ float from_float<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) {
+    return __float2bfloat16_rn(v);
+}
+template <>
+__device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
+
+// f(T{}) with the C++ type of an element type
+template <typename F>
+inline Status with_type(int type, F f) {
+    switch (type) {
+        case T_F32: return f(float{});
+        case T_BF16: return f(__nv_bfloat16{});
+        case T_F16: return f(__half{});
+        default: return ERR_SHAPE;
+    }
+}
+
+// Sum of v over the block, known to every thread; sh holds 32 floats.  The
+// order of the additions depends on the block size alone.
+__device__ __forceinline__ float block_sum(float v, float *sh) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    const int warps = blockDim.x >> 5, lane = threadIdx.x & 31;
+    if (lane == 0) sh[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = lane < warps ? sh[lane] : 0.0f;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    __syncthreads();
+    return v;
+}
+
+}  // namespace ppdl

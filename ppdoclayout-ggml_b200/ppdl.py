@@ -8,7 +8,9 @@ Two surfaces, both thin bindings of lib/libppdl_b200.so:
   additive batch and device-output entry points;
 * the operator API of include/ppdl_ops.h (ppdl_op_launch) — the reference's
   tagged ggml custom-op hooks (patches/ggml-ppdl.patch:612-930), driven here
-  with torch CUDA tensors as the device memory.
+  with torch CUDA tensors as the device memory — and the transformer-block
+  operators beside it (layernorm, layernorm_backward, quantize_rows,
+  linear_i8, rotary).
 
 There is no CPU fallback: importing this module never loads anything else,
 and every call fails loudly when the CUDA library is missing.
@@ -81,6 +83,7 @@ def lib() -> C.CDLL:
         L.ppdl_op_supported.argtypes = [C.POINTER(OpDesc)]
         L.ppdl_op_supported.restype = C.c_int
         L.ppdl_op_last_error.restype = C.c_char_p
+        _declare_block_ops(L)
         if hasattr(L, "ppdl_init"):
             L.ppdl_init.argtypes = [C.c_char_p, C.c_int]
             L.ppdl_init.restype = C.c_void_p
@@ -344,3 +347,285 @@ def last_error() -> str:
 def check(status: int) -> None:
     if status != PPDL_OK:
         raise RuntimeError(f"ppdl_op_launch failed ({status}): {last_error()}")
+
+
+# ---- transformer-block operators ---------------------------------------------
+# Functions of torch CUDA tensors.  Each enqueues on torch's current stream of
+# the tensors' device, returns new tensors, and raises ValueError for tensors
+# it does not take and RuntimeError for a call the library refuses.  They
+# record no autograd history: a backward pass is a function of its own.
+
+F32, BF16, F16 = 0, 1, 2
+ACTS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3}
+
+
+class RotaryHeads(C.Structure):
+    """ppdl_rotary_heads."""
+    _fields_ = [("in_", C.c_void_p), ("out", C.c_void_p), ("heads", C.c_int32),
+                ("in_batch", C.c_int64), ("in_token", C.c_int64), ("in_head", C.c_int64),
+                ("out_batch", C.c_int64), ("out_token", C.c_int64), ("out_head", C.c_int64)]
+
+
+def _declare_block_ops(L) -> None:
+    p, i, ll, f = C.c_void_p, C.c_int, C.c_longlong, C.c_float
+    L.ppdl_layernorm.argtypes = [p, ll, p, ll, p, p, i, i, ll, i, f, p, ll, p, ll, p, p, p]
+    L.ppdl_layernorm_backward.argtypes = [p, ll, p, ll, p, p, p, p, ll, i, i, ll, i, p, ll, p, p,
+                                          p, p]
+    L.ppdl_layernorm_backward_workspace.argtypes = [ll, i]
+    L.ppdl_layernorm_backward_workspace.restype = ll
+    L.ppdl_quantize_rows_i8.argtypes = [p, ll, i, ll, i, p, ll, p, p]
+    L.ppdl_linear_i8.argtypes = [p, ll, p, p, ll, p, p, p, ll, i, i, i, i, i, p, ll, p]
+    L.ppdl_rotary.argtypes = [p, p, i, i, i, i, i, p, i, ll, ll, ll, i, p, p, i, i, p]
+
+
+_types = {}
+
+
+def _type(t, name: str) -> int:
+    """The PPDL_* element type of tensor t."""
+    if not _types:
+        import torch
+        _types.update({torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16})
+    code = _types.get(t.dtype)
+    if code is None:
+        raise ValueError(f"{name} must be float32, bfloat16 or float16, not {t.dtype}")
+    return code
+
+
+def _rows(t, name: str, width: int, like=None) -> int:
+    """The distance between the rows of width values that t [..., width]
+    consists of; t may be strided as long as its rows lie evenly apart."""
+    if t.dim() == 0 or t.shape[-1] != width or (like is not None and t.shape != like.shape):
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected "
+                         f"{tuple(like.shape) if like is not None else (..., width)}")
+    if t.is_contiguous():
+        return width
+    ld = span = None
+    if t.stride(-1) == 1 or width == 1:
+        for n, s in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
+            if n == 1:
+                continue
+            if ld is None:
+                ld = s
+            elif s != span:
+                break
+            span = s * n
+        else:
+            return width if ld is None else ld
+    raise ValueError(f"{name} must consist of contiguous rows at one distance, "
+                     f"not strides {tuple(t.stride())} of shape {tuple(t.shape)}")
+
+
+def _vector(t, name: str, n: int, dtype=None):
+    if t.dim() != 1 or t.shape[0] != n or (n > 1 and t.stride(0) != 1) or \
+            (dtype is not None and t.dtype != dtype):
+        raise ValueError(f"{name} must be {n} contiguous values"
+                         + (f" of {dtype}" if dtype is not None else ""))
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _call(fn, tensors, *args) -> None:
+    """fn(*args, stream) on the tensors' device, checked."""
+    import torch
+    dev = tensors[0].device
+    for t in tensors:
+        if t is not None and t.device != dev:
+            raise ValueError(f"tensors on {dev} and {t.device}")
+    if dev.type != "cuda":
+        raise ValueError(f"tensors on {dev}: the operators take CUDA tensors")
+    stream = torch.cuda.current_stream(dev).cuda_stream
+    if dev.index == torch.cuda.current_device():
+        status = fn(*args, stream)
+    else:
+        with torch.cuda.device(dev):
+            status = fn(*args, stream)
+    if status != PPDL_OK:
+        raise RuntimeError(f"{fn.__name__} failed ({status}): {last_error()}")
+
+
+def layernorm(x, weight=None, bias=None, eps: float = 1e-5, *, residual=None,
+              return_sum: bool = False, return_stats: bool = False):
+    """Layer norm of the rows of x [..., D] (ppdl_layernorm), of x + residual
+    when one is given (the sum rounded to x's type).  weight and bias [D] are
+    of x's type or float32.  Returns y, followed by the sum (return_sum) and
+    by the rows' mean and rstd in float32 (return_stats), which the backward
+    pass takes."""
+    import torch
+    D = x.shape[-1] if x.dim() else 0
+    t = _type(x, "x")
+    ldx = _rows(x, "x", D)
+    ldr = 0
+    if residual is not None:
+        ldr = _rows(residual, "residual", D, x)
+        if residual.dtype != x.dtype:
+            raise ValueError("residual must have x's type")
+    elif return_sum:
+        raise ValueError("return_sum needs a residual")
+    wt = t
+    for v, name in ((weight, "weight"), (bias, "bias")):
+        if v is not None:
+            _vector(v, name, D)
+            wt = _type(v, name)
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+        raise ValueError("weight and bias must have one type")
+    rows = x.numel() // D if D else 0
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    s = torch.empty(x.shape, dtype=x.dtype, device=x.device) if return_sum else None
+    mean = rstd = None
+    if return_stats:
+        mean = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+        rstd = torch.empty_like(mean)
+    _call(lib().ppdl_layernorm, (x, residual, weight, bias), x.data_ptr(), ldx, _ptr(residual), ldr,
+          _ptr(weight), _ptr(bias), t, wt, rows, D, eps, y.data_ptr(), D, _ptr(s), D, _ptr(mean),
+          _ptr(rstd))
+    out = (y,) + ((s,) if return_sum else ()) + ((mean, rstd) if return_stats else ())
+    return out if len(out) > 1 else y
+
+
+def layernorm_backward(dy, x, weight, mean, rstd, *, dsum=None, param_grads: bool = True):
+    """The gradients (dx, dweight, dbias) of layernorm at its input x — the
+    returned sum when it had a residual — from the gradient dy of its result
+    and its statistics (ppdl_layernorm_backward).  dsum is the gradient that
+    reaches the sum on its other path; dx is then the gradient of x and of
+    the residual alike.  dweight and dbias have weight's type (x's without a
+    weight) and are None without param_grads."""
+    import torch
+    D = x.shape[-1] if x.dim() else 0
+    t = _type(x, "x")
+    ldx, lddy = _rows(x, "x", D), _rows(dy, "dy", D, x)
+    ldds = _rows(dsum, "dsum", D, x) if dsum is not None else 0
+    if dy.dtype != x.dtype or (dsum is not None and dsum.dtype != x.dtype):
+        raise ValueError("dy and dsum must have x's type")
+    wt = t
+    if weight is not None:
+        _vector(weight, "weight", D)
+        wt = _type(weight, "weight")
+    rows = x.numel() // D if D else 0
+    for v, name in ((mean, "mean"), (rstd, "rstd")):
+        if v.dtype != torch.float32 or v.shape != x.shape[:-1] or not v.is_contiguous():
+            raise ValueError(f"{name} must be contiguous float32 of shape {tuple(x.shape[:-1])}")
+    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    dw = db = work = None
+    L = lib()
+    if param_grads:
+        grads = torch.empty((2, D), dtype=x.dtype if weight is None else weight.dtype,
+                            device=x.device)
+        dw, db = grads[0], grads[1]
+        work = torch.empty(L.ppdl_layernorm_backward_workspace(rows, D), dtype=torch.float32,
+                           device=x.device)
+    _call(L.ppdl_layernorm_backward, (x, dy, weight, mean, rstd, dsum), dy.data_ptr(), lddy,
+          x.data_ptr(), ldx, _ptr(weight), mean.data_ptr(), rstd.data_ptr(), _ptr(dsum), ldds, t,
+          wt, rows, D, dx.data_ptr(), D, _ptr(dw), _ptr(db), _ptr(work))
+    return dx, dw, db
+
+
+def quantize_rows(x):
+    """8-bit rows of x [..., K] (ppdl_quantize_rows_i8): (q, scale) with q
+    int8 [..., K], rows on strides of a multiple of 16 bytes, and scale
+    float32 [...]: q * scale[..., None] stands for x.  It quantises weights
+    [N, K] channel by channel and activations token by token."""
+    import torch
+    K = x.shape[-1] if x.dim() else 0
+    t = _type(x, "x")
+    ldx = _rows(x, "x", K)
+    ldq = (K + 15) // 16 * 16
+    q = torch.empty(x.shape[:-1] + (ldq,), dtype=torch.int8, device=x.device)
+    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    _call(lib().ppdl_quantize_rows_i8, (x,), x.data_ptr(), ldx, t, x.numel() // K if K else 0, K,
+          q.data_ptr(), ldq, scale.data_ptr())
+    return q[..., :K], scale
+
+
+def linear_i8(x, weight, w_scale, *, x_scale=None, bias=None, act: str = "none", residual=None,
+              out_dtype=None):
+    """act(x weight^T + bias) + residual on 8-bit integers (ppdl_linear_i8).
+    weight int8 [N, K] and w_scale float32 [N] as quantize_rows makes them.
+    x [..., K]: float32 / bfloat16 / float16 rows, quantised token by token
+    in the call; or int8 with x_scale float32 [...].  bias float32 [N]; act
+    none, relu, silu or gelu; residual [..., N] of the result's type, which is
+    x's (for int8 x: residual's, else float32) unless out_dtype says
+    otherwise."""
+    import torch
+    if weight.dim() != 2 or weight.dtype != torch.int8:
+        raise ValueError("weight must be int8 [N, K]")
+    N, K = weight.shape
+    if act not in ACTS:
+        raise ValueError(f"act must be one of {', '.join(ACTS)}")
+    ldw = _rows(weight, "weight", K)
+    ldx = _rows(x, "x", K)
+    _vector(w_scale, "w_scale", N, torch.float32)
+    if bias is not None:
+        _vector(bias, "bias", N, torch.float32)
+    lead = x.shape[:-1]
+    M = x.numel() // K if K else 0
+    if x.dtype == torch.int8:
+        if x_scale is None or x_scale.dtype != torch.float32 or x_scale.shape != lead or \
+                not x_scale.is_contiguous():
+            raise ValueError(f"int8 x needs x_scale, contiguous float32 of shape {tuple(lead)}")
+        dtype = out_dtype or (torch.float32 if residual is None else residual.dtype)
+    else:
+        if x_scale is not None:
+            raise ValueError("x_scale goes with int8 x")
+        dtype = out_dtype or x.dtype
+    y = torch.empty(lead + (N,), dtype=dtype, device=x.device)
+    t = _type(y, "the result")
+    ldr = 0
+    if residual is not None:
+        ldr = _rows(residual, "residual", N, y)
+        if residual.dtype != dtype:
+            raise ValueError("residual must have the result's type")
+    L = lib()
+    if x_scale is None:
+        q = torch.empty((M, (K + 15) // 16 * 16), dtype=torch.int8, device=x.device)
+        x_scale = torch.empty(M, dtype=torch.float32, device=x.device)
+        _call(L.ppdl_quantize_rows_i8, (x,), x.data_ptr(), ldx, _type(x, "x"), M, K, q.data_ptr(),
+              q.shape[1], x_scale.data_ptr())
+        x, ldx = q, q.shape[1]
+    _call(L.ppdl_linear_i8, (x, x_scale, weight, w_scale, bias, residual), x.data_ptr(), ldx,
+          x_scale.data_ptr(), weight.data_ptr(), ldw, w_scale.data_ptr(), _ptr(bias),
+          _ptr(residual), ldr, t, ACTS[act], M, N, K, y.data_ptr(), N)
+    return y
+
+
+def _heads(x, out, name: str, dim: int, like):
+    if x.dim() != 4 or x.shape[3] != dim or x.shape[:2] != like.shape[:2] or x.dtype != like.dtype:
+        raise ValueError(f"{name} must be [batch, length, heads, {dim}] of one type")
+    if dim > 1 and x.stride(3) != 1:
+        raise ValueError(f"{name}'s heads must be contiguous")
+    i, o = x.stride(), out.stride()
+    return RotaryHeads(x.data_ptr(), out.data_ptr(), x.shape[2], i[0], i[1], i[2], o[0], o[1], o[2])
+
+
+def rotary(q, k, positions, freq, sections, *, interleaved: bool = False, inverse: bool = False,
+           inplace: bool = False):
+    """Rotary positions with several axes (ppdl_rotary) on q [batch, length,
+    heads, dim] and k (its own number of heads, or None): returns both turned
+    (new tensors, or q and k themselves with inplace).  positions int32 or
+    int64 [axes, batch, length] (may be expanded views); freq float64
+    [rotated / 2] in radians per position turns the first `rotated` values of
+    every head; sections says how many consecutive pairs each axis turns.
+    inverse turns back: the backward pass."""
+    import torch
+    dim = q.shape[-1] if q.dim() else 0
+    t = _type(q, "q")
+    if positions.dtype not in (torch.int32, torch.int64) or positions.dim() != 3 or \
+            positions.shape[0] != len(sections) or positions.shape[1:] != q.shape[:2]:
+        raise ValueError("positions must be int32 or int64 [axes, batch, length], one axis a section")
+    if freq.dtype != torch.float64 or freq.dim() != 1 or not freq.is_contiguous():
+        raise ValueError("freq must be contiguous float64 [rotated / 2]")
+    qo = q if inplace else torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    hq = _heads(q, qo, "q", dim, q)
+    ko = hk = None
+    if k is not None:
+        ko = k if inplace else torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        hk = _heads(k, ko, "k", dim, q)
+    ps = positions.stride()
+    _call(lib().ppdl_rotary, (q, k, positions, freq), C.byref(hq),
+          C.byref(hk) if hk is not None else None, t, q.shape[0], q.shape[1], dim,
+          2 * freq.shape[0], positions.data_ptr(), positions.element_size(), ps[0], ps[1], ps[2],
+          len(sections), (C.c_int32 * len(sections))(*sections), freq.data_ptr(), int(interleaved),
+          int(inverse))
+    return qo, ko
