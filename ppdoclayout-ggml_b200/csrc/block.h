@@ -54,6 +54,8 @@ struct LinearI8Args {
     int M = 0, N = 0, K = 0;
 };
 Status launch_linear_i8(const LinearI8Args &a, cudaStream_t st);
+// its device error flag, as tc_error_fetch_and_clear()
+int linear_error_fetch_and_clear();
 
 struct RotaryHeads {
     const void *in = nullptr;

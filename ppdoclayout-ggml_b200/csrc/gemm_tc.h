@@ -175,6 +175,12 @@ bool tc_gemm_set_bits_output(TcGemm *g, uint32_t *bits, long long words_per_n, l
 
 Status launch_tc_gemm(const TcGemm &g, cudaStream_t st);
 
+// Tensor map of a matrix of bytes (rows of `width` bytes, ld apart) with the
+// 128-byte swizzle, zeros outside.  False when the driver's encoder is
+// missing or base / ld are not multiples of 16.
+bool tma_encode_bytes(CUtensorMap *tm, const void *base, uint64_t width, uint64_t rows,
+                      uint64_t ld, uint32_t box_width, uint32_t box_rows);
+
 // Device error flag of the tensor-core kernels (set when a bounded wait gave
 // up); reads and clears it.
 int tc_error_fetch_and_clear();

@@ -1,116 +1,546 @@
 // linear_i8.cu — linear layers in 8-bit integers with a scale for each token
-// (row of the activations) and each channel (row of the weights):
+// (row of the activations) and each channel (row of the weights), on the
+// 5th-generation tensor cores:
 //
 //   y(m, n) = act(sum_k q(m, k) w(n, k) * q_scale[m] * w_scale[n] + bias[n]) + res(m, n)
 //
-// and the quantiser that makes q and q_scale from FP32 / BF16 / FP16 rows.
-// The integer sums are exact (at most 131071 products of at most 128 x 128: below 2^31).
+// The integer sums are exact: at most 131071 products of at most 128 x 128
+// stay below 2^31, in any order.
+//
+// The product is computed transposed: the MMA's M dimension is 128 output
+// channels (the weights are its A operand), its N dimension BT tokens.  A
+// TMEM lane is then one channel, so that in the epilogue the 32 lanes of a
+// warp hold 32 neighbouring channels of one token: rows of y (and of the
+// residual) are read and written in whole segments straight from registers,
+// with no pass through shared memory, and a lane's channel scale and bias
+// stay in registers for the whole tile.  It also makes a single token cheap:
+// only the N dimension shrinks (to 16).
+//
+// One CTA of 12 warps: warp 0 loads 128-byte wide k-blocks of both operands
+// by TMA (128-byte swizzle) into a ring of stages, warp 1 issues
+// tcgen05.mma kind::i8 (four K = 32 steps a block) into one of two TMEM
+// accumulators, warps 4-11 (two per lane quadrant, each half the tokens) run
+// the epilogue of one tile while the next is accumulated.
+//
+// Two forms.  Whole-K: a persistent grid over the tiles.  Split-K, for few
+// tiles: a cluster shares a tile's k-blocks; every CTA puts its partial
+// sums into its own shared memory, and after a cluster barrier each CTA adds
+// up its share of the tokens over its peers and finishes it.  Integer sums
+// do not depend on the order, so both forms give the same bits.
+//
+// Every mbarrier wait is bounded; on expiry the kernel raises a device error
+// flag, all roles drain out and TMEM is released (ppdl_op_device_error).
+#include <cuda.h>
+
 #include "block.cuh"
 #include "block.h"
+#include "gemm_tc.h"
+#include "tc_ptx.cuh"
 
 namespace ppdl {
 
 namespace {
 
-// x / s rounded half to even, as the real quotient rounds, for a finite
-// |x| <= about 200 s and s in [2^-64, 2^128): the FP32 product with 1 / s
-// may land on the wrong side of a half, so the remainder of the rounded
-// value decides.  r = x - q s is exact: x and q s are whole multiples of
-// half a unit in the last place of s, and |r| is at most about s.
-__device__ __forceinline__ int quantize(float x, float s, float inv) {
-    float q = rintf(x * inv);
-    const float r = __fmaf_rn(-q, s, x), h = 0.5f * s;
-    const bool odd = ((int)q & 1) != 0;
-    if (r > h || (r == h && odd)) q += 1.0f;
-    if (r < -h || (r == -h && odd)) q -= 1.0f;
-    return (int)fminf(fmaxf(q, -127.0f), 127.0f);
+__device__ int g_linear_error = 0;
+
+constexpr int kFeat = 128;  // channels per tile (MMA M)
+constexpr int kBK = 128;    // k per stage: one 128-byte swizzle row
+constexpr int kThreads = 384;
+constexpr int kWarpTma = 0, kWarpMma = 1, kWarpEpi = 4, kEpiWarps = 8;
+constexpr long long kTimeoutCycles = 4000000000LL;
+constexpr int kCtrlBytes = 256;
+constexpr int kSmemMax = 227 * 1024;
+constexpr int kABytes = kFeat * kBK;
+
+constexpr int stage_bytes(int bt) { return kABytes + bt * kBK; }
+// stages in the ring: what fits beside the control block and the alignment
+// slack, at most 8; the split form keeps to 4 so that two CTAs share an SM
+constexpr int stages(int bt, bool split) {
+    const int fit = (kSmemMax - kCtrlBytes - 1024) / stage_bytes(bt);
+    const int most = split ? 4 : 8;
+    return fit < most ? fit : most;
+}
+constexpr int smem_bytes(int bt, bool split) {
+    return kCtrlBytes + 1024 + stages(bt, split) * stage_bytes(bt);
+}
+constexpr uint32_t tmem_cols(int bt, bool split) {
+    const int c = split ? bt : 2 * bt;
+    return c < 32 ? 32 : c;
 }
 
-// One block per row: the largest |x| (as the bits of |x|, whose unsigned
-// order puts infinities and NaNs on top), then the quotients.  Scales below
-// 2^-64 quantise x 2^64 by s 2^64, both exact, so that 1 / s is finite.
-template <typename T>
-__global__ void quantize_rows_kernel(const T *x, long long ldx, int K, int8_t *q, long long ldq,
-                                     float *scale) {
-    pdl_begin();
-    __shared__ unsigned sh[32];
-    const long long row = blockIdx.x;
-    x += row * ldx;
-    q += row * ldq;
-    unsigned m = 0;
-    for (int i = threadIdx.x; i < K; i += blockDim.x)
-        m = max(m, __float_as_uint(fabsf(to_float(x[i]))));
-    m = __reduce_max_sync(0xffffffffu, m);
-    if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = m;
-    __syncthreads();
-    m = 0;
-    for (int i = 0; i < (int)(blockDim.x >> 5); i++) m = max(m, sh[i]);
-    const float s = __fdiv_rn(__uint_as_float(m), 127.0f);
-    if (threadIdx.x == 0) scale[row] = s;
-    const bool usable = s > 0.0f && m < 0x7f800000u;
-    const float up = s < 0x1p-64f ? 0x1p64f : 1.0f;
-    const float su = s * up, inv = usable ? __frcp_rn(su) : 0.0f;
-    for (int i = threadIdx.x; i < K; i += blockDim.x)
-        q[i] = usable ? (int8_t)quantize(to_float(x[i]) * up, su, inv) : (int8_t)0;
-}
+struct Args {
+    int M, N, kblocks;
+    int f_tiles, t_tiles, tiles;
+    int kps;  // split form: k-blocks per CTA of the cluster
+    int act;
+    int pairs;  // 16-bit rows of y and res start on 4 bytes
+    const float *q_scale, *w_scale, *bias;
+    const void *res;
+    void *y;
+    long long ldres, ldy;
+};
 
-// One thread per output, 16 x 16 outputs a block, 64 bytes of k at a time
-// through shared memory, four products an instruction.
-template <typename T>
-__global__ void __launch_bounds__(256) linear_i8_simt_kernel(LinearI8Args a) {
-    pdl_begin();
-    __shared__ int sq[16][17], sw[16][17];
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    const long long m0 = (long long)blockIdx.y * 16;
-    const int n0 = blockIdx.x * 16;
-    auto word = [&](const int8_t *p, int k) {  // bytes k .. k + 3 of a row, zero past K
-        int v = 0;
-        for (int j = 0; j < 4; j++)
-            if (k + j < a.K) v |= (int)(uint8_t)p[k + j] << (8 * j);
-        return v;
-    };
-    int acc = 0;
-    for (int k0 = 0; k0 < a.K; k0 += 64) {
-        const int k = k0 + 4 * tx;
-        sq[ty][tx] = m0 + ty < a.M ? word(a.q + (m0 + ty) * a.ldq, k) : 0;
-        sw[ty][tx] = n0 + ty < a.N ? word(a.w + (long long)(n0 + ty) * a.ldw, k) : 0;
-        __syncthreads();
-#pragma unroll
-        for (int j = 0; j < 16; j++) acc = __dp4a(sq[ty][j], sw[tx][j], acc);
-        __syncthreads();
+// Bounded wait: false when the phase did not complete within the time limit
+// or another role already gave up.
+__device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity, volatile int *abort_flag) {
+    if (mbar_try_wait(bar, parity)) return true;
+    const long long t0 = clock64();
+    for (uint32_t i = 1;; i++) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if ((i & 63) == 0) {
+            if (*abort_flag) return false;
+            if (clock64() - t0 > kTimeoutCycles) {
+                *abort_flag = 1;
+                atomicExch(&g_linear_error, 1);
+                return false;
+            }
+        }
     }
-    const long long m = m0 + ty;
-    const int n = n0 + tx;
-    if (m >= a.M || n >= a.N) return;
-    float v = (float)acc * a.q_scale[m] * a.w_scale[n];
-    if (a.bias) v += a.bias[n];
-    v = act_apply(v, a.act);
-    if (a.res.p) v += to_float(((const T *)a.res.p)[m * a.res.ld + n]);
-    ((T *)a.y.p)[m * a.y.ld + n] = from_float<T>(v);
+}
+
+// D (TMEM) (+)= A (shared) * B (shared), 8-bit signed, K = 32
+__device__ __forceinline__ void umma_i8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                        uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+    return r;
+}
+// the same shared-memory address in the cluster's CTA `rank`
+__device__ __forceinline__ uint32_t peer_addr(uint32_t addr, uint32_t rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ int4 peer_load(uint32_t addr) {
+    int4 v;
+    asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "r"(addr)
+                 : "memory");
+    return v;
+}
+__device__ __forceinline__ int peer_load1(uint32_t addr) {
+    int v;
+    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+    return v;
+}
+
+// tile index -> (channel tile, token tile): token tiles in groups of 8, the
+// group's channel tiles outer, so that the CTAs that run at one time share
+// both operands in L2
+__device__ __forceinline__ void tile_of(const Args &a, int tile, int &ft, int &tt) {
+    constexpr int kGroup = 8;
+    const int per = kGroup * a.f_tiles;
+    const int g = tile / per, r = tile - g * per;
+    const int width = min(kGroup, a.t_tiles - g * kGroup);
+    ft = r / width;
+    tt = g * kGroup + r - ft * width;
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
+    const __nv_bfloat162 p = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&p);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
+    const __half2 p = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&p);
+}
+template <typename T>
+__device__ __forceinline__ float2 unpack2(uint32_t v);
+template <>
+__device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t v) {
+    return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&v));
+}
+template <>
+__device__ __forceinline__ float2 unpack2<__half>(uint32_t v) {
+    return __half22float2(*reinterpret_cast<const __half2 *>(&v));
+}
+
+// What follows the sum.  acc is rounded to FP32 (2^-24 relative), the two
+// scales are multiplied first (they are the same for a whole row or column).
+template <int ACT>
+__device__ __forceinline__ float finish(int acc, float scale, float bias) {
+    return act_apply(__fmaf_rn((float)acc, scale, bias), ACT);
+}
+
+// Epilogue of C tokens t0 .. t0 + C - 1 of channel n (one per lane).
+template <typename T, int C, int ACT>
+__device__ __forceinline__ void epilogue_chunk(const Args &a, const uint32_t (&acc)[C], int t0,
+                                               int n, float sw, float bias, float sx, int lane) {
+    const bool n_ok = n < a.N;
+    const bool full = t0 + C <= a.M;
+    if constexpr (sizeof(T) == 2) {
+        // lane pairs exchange values, so that the even lane holds token j and
+        // the odd lane token j + 1 of two neighbouring channels: one 4-byte
+        // store (and residual load) per lane and pair of tokens
+        if (a.pairs && n - lane + 32 <= a.N) {
+            const int odd = lane & 1;
+            const long long first = t0 + odd, nn = n - odd;
+            uint32_t r[C / 2];
+            if (a.res) {
+                const T *rp = (const T *)a.res + first * a.ldres + nn;
+#pragma unroll
+                for (int j = 0; j < C; j += 2, rp += 2 * a.ldres) {
+                    r[j / 2] = 0;
+                    if (full || first + j < a.M) r[j / 2] = *reinterpret_cast<const uint32_t *>(rp);
+                }
+            }
+            T *yp = (T *)a.y + first * a.ldy + nn;
+#pragma unroll
+            for (int j = 0; j < C; j += 2, yp += 2 * a.ldy) {
+                const float s0 = __shfl_sync(0xffffffffu, sx, j) * sw;
+                const float s1 = __shfl_sync(0xffffffffu, sx, j + 1) * sw;
+                const float v0 = finish<ACT>((int)acc[j], s0, bias);
+                const float v1 = finish<ACT>((int)acc[j + 1], s1, bias);
+                const float other = __shfl_xor_sync(0xffffffffu, odd ? v0 : v1, 1);
+                float lo = odd ? other : v0, hi = odd ? v1 : other;
+                if (a.res) {
+                    const float2 rr = unpack2<T>(r[j / 2]);
+                    lo += rr.x;
+                    hi += rr.y;
+                }
+                if (full || first + j < a.M) *reinterpret_cast<uint32_t *>(yp) = pack2<T>(lo, hi);
+            }
+            return;
+        }
+    }
+    float r[C];
+    if (a.res) {
+        const T *rp = (const T *)a.res + (long long)t0 * a.ldres + n;
+#pragma unroll
+        for (int j = 0; j < C; j++, rp += a.ldres)
+            r[j] = n_ok && (full || t0 + j < a.M) ? to_float(*rp) : 0.0f;
+    }
+    T *yp = (T *)a.y + (long long)t0 * a.ldy + n;
+#pragma unroll
+    for (int j = 0; j < C; j++, yp += a.ldy) {
+        const float s = __shfl_sync(0xffffffffu, sx, j) * sw;
+        float v = finish<ACT>((int)acc[j], s, bias);
+        if (a.res) v += r[j];
+        if (n_ok && (full || t0 + j < a.M)) *yp = from_float<T>(v);
+    }
+}
+
+template <typename T, int C>
+__device__ __forceinline__ void epilogue_any(const Args &a, const uint32_t (&acc)[C], int t0, int n,
+                                             float sw, float bias, float sx, int lane) {
+    switch (a.act) {
+        case ACT_RELU: epilogue_chunk<T, C, ACT_RELU>(a, acc, t0, n, sw, bias, sx, lane); break;
+        case ACT_SILU: epilogue_chunk<T, C, ACT_SILU>(a, acc, t0, n, sw, bias, sx, lane); break;
+        case ACT_GELU: epilogue_chunk<T, C, ACT_GELU>(a, acc, t0, n, sw, bias, sx, lane); break;
+        default: epilogue_chunk<T, C, ACT_NONE>(a, acc, t0, n, sw, bias, sx, lane);
+    }
+}
+
+template <typename T, int BT, bool SPLIT>
+__global__ void __launch_bounds__(kThreads, SPLIT ? 2 : 1)
+linear_i8_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmQ,
+                 const __grid_constant__ Args a) {
+    constexpr int S = stages(BT, SPLIT), kAcc = SPLIT ? 1 : 2;
+    constexpr uint32_t kStage = stage_bytes(BT), kCols = tmem_cols(BT, SPLIT);
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t ctrl = smem_u32(smem_raw);
+    // full[s]: a stage's bytes landed; empty[s]: its MMAs completed;
+    // tfull[i]: accumulator i complete; tempty[i]: read by the epilogue
+    const uint32_t bar_full = ctrl, bar_empty = ctrl + 64, bar_tfull = ctrl + 128,
+                   bar_tempty = ctrl + 144, bar_done = ctrl + 160;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem_raw + 176);
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(smem_raw + 180);
+    const uint32_t stage0 = (ctrl + kCtrlBytes + 1023) & ~1023u;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < S; s++) {
+            mbar_init(bar_full + 8 * s, 1);
+            mbar_init(bar_empty + 8 * s, 1);
+        }
+        for (int i = 0; i < 2; i++) {
+            mbar_init(bar_tfull + 8 * i, 1);
+            mbar_init(bar_tempty + 8 * i, kEpiWarps);
+        }
+        mbar_init(bar_done, 1);
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == kWarpMma) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                         smem_u32(tmem_slot)),
+                     "r"(kCols)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    pdl_begin();
+
+    const uint32_t rank = SPLIT ? cluster_rank() : 0, peers = SPLIT ? cluster_size() : 1;
+    const int first = SPLIT ? (int)(blockIdx.x / peers) : (int)blockIdx.x;
+    const int step = SPLIT ? a.tiles : (int)gridDim.x;  // split form: one tile
+    const int kb0 = SPLIT ? (int)rank * a.kps : 0;
+    const int kbn = SPLIT ? max(0, min(a.kps, a.kblocks - kb0)) : a.kblocks;
+
+    if (warp == kWarpTma) {
+        if (lane == 0) {
+            Ring rs(S);
+            long long it = 0;
+            bool ok = true;
+            for (int tile = first; tile < a.tiles && ok; tile += step) {
+                int ft, tt;
+                tile_of(a, tile, ft, tt);
+                for (int kb = 0; kb < kbn; kb++, it++, rs.next()) {
+                    if (!wait_for(bar_empty + 8 * rs.i, rs.ph ^ 1, abort_flag)) {
+                        ok = false;
+                        break;
+                    }
+                    const uint32_t st = stage0 + rs.i * kStage, fb = bar_full + 8 * rs.i;
+                    mbar_expect_tx(fb, kStage);
+                    tma_load_2d(st, &tmW, fb, (kb0 + kb) * kBK, ft * kFeat);
+                    tma_load_2d(st + kABytes, &tmQ, fb, (kb0 + kb) * kBK, tt * BT);
+                }
+            }
+            // what was issued must land before the CTA may exit
+            for (long long j = it > S ? it - S : 0; j < it; j++) {
+                int dummy = 0;
+                wait_for(bar_full + 8 * (int)(j % S), (uint32_t)((j / S) & 1), (volatile int *)&dummy);
+            }
+        }
+    } else if (warp == kWarpMma) {
+        if (lane == 0) {
+            // S32 accumulators, signed 8-bit A and B, both K-major
+            constexpr uint32_t idesc = (2u << 4) | (1u << 7) | (1u << 10) |
+                                       ((uint32_t)(BT >> 3) << 17) | ((uint32_t)(kFeat >> 4) << 24);
+            Ring rs(S), ra(kAcc);
+            bool ok = true;
+            for (int tile = first; tile < a.tiles && ok; tile += step, ra.next()) {
+                if (!wait_for(bar_tempty + 8 * ra.i, ra.ph ^ 1, abort_flag)) break;
+                tc_fence_after();
+                const uint32_t d = tmem + (uint32_t)(ra.i * BT);
+                for (int kb = 0; kb < kbn; kb++, rs.next()) {
+                    if (!wait_for(bar_full + 8 * rs.i, rs.ph, abort_flag)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint32_t st = stage0 + rs.i * kStage;
+                    // a K = 32 step is 32 bytes into the swizzled row: +2 in the
+                    // descriptors' start address
+                    const uint64_t da = smem_desc(st, 16, 1024, 2);
+                    const uint64_t db = smem_desc(st + kABytes, 16, 1024, 2);
+#pragma unroll
+                    for (int k = 0; k < kBK / 32; k++)
+                        umma_i8(d, da + 2 * k, db + 2 * k, idesc, (kb | k) != 0);
+                    umma_commit(bar_empty + 8 * rs.i);
+                }
+                if (ok) umma_commit(bar_tfull + 8 * ra.i);
+            }
+            // all issued MMAs must finish before TMEM is released
+            umma_commit(bar_done);
+            int dummy = 0;
+            wait_for(bar_done, 0, (volatile int *)&dummy);
+        }
+    } else if (warp >= kWarpEpi) {
+        constexpr int kHalf = BT / 2, C = kHalf < 32 ? kHalf : 32;
+        const int quad = warp & 3, part = (warp - kWarpEpi) >> 2;
+        const uint32_t lane_base = (uint32_t)(quad * 32) << 16;
+        Ring ra(kAcc);
+        for (int tile = first; tile < a.tiles; tile += step, ra.next()) {
+            int ft, tt;
+            tile_of(a, tile, ft, tt);
+            const int n = ft * kFeat + quad * 32 + lane;
+            float sw = 0.0f, bias = 0.0f;
+            if (!SPLIT && n < a.N) {
+                sw = __ldg(a.w_scale + n);
+                if (a.bias) bias = __ldg(a.bias + n);
+            }
+            bool good = true;
+            if (lane == 0) good = wait_for(bar_tfull + 8 * ra.i, ra.ph, abort_flag);
+            if (!__shfl_sync(0xffffffffu, good ? 1 : 0, 0)) break;
+            tc_fence_after();
+            const uint32_t col = tmem + lane_base + (uint32_t)(ra.i * BT + part * kHalf);
+#pragma unroll 1
+            for (int c = 0; c < kHalf; c += C) {
+                const int t0 = tt * BT + part * kHalf + c;
+                uint32_t acc[C];
+                tmem_load(col + c, acc);
+                if (c + C >= kHalf) {
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(bar_tempty + 8 * ra.i);
+                }
+                if constexpr (SPLIT) {
+                    // partial sums, token-major: [BT][128] in the stages, all of
+                    // which the MMAs have read
+                    int *part_sum = reinterpret_cast<int *>(smem_raw + (stage0 - ctrl));
+#pragma unroll
+                    for (int j = 0; j < C; j++)
+                        part_sum[(part * kHalf + c + j) * kFeat + quad * 32 + lane] =
+                            kbn ? (int)acc[j] : 0;
+                } else if (t0 < a.M) {
+                    float sx = 0.0f;
+                    if (lane < C && t0 + lane < a.M) sx = __ldg(a.q_scale + t0 + lane);
+                    epilogue_any<T, C>(a, acc, t0, n, sw, bias, sx, lane);
+                }
+            }
+        }
+    }
+    __syncwarp();
+
+    if constexpr (SPLIT) {
+        cluster_sync();
+        // this CTA's share of the tokens: 4 neighbouring channels a thread,
+        // 12 tokens at a time
+        int ft, tt;
+        tile_of(a, first, ft, tt);
+        const int share = (BT + (int)peers - 1) / (int)peers;
+        const int lo = (int)rank * share, hi = min(min(BT, lo + share), a.M - tt * BT);
+        int bad = 0;
+        for (uint32_t p = 0; p < peers; p++)
+            bad |= peer_load1(peer_addr(ctrl + 180, p));
+        const int n = ft * kFeat + 4 * lane;
+        for (int j = lo + warp; j < hi && !bad; j += kThreads / 32) {
+            int4 s = make_int4(0, 0, 0, 0);
+            for (uint32_t p = 0; p < peers; p++) {
+                const int4 v = peer_load(peer_addr(stage0 + (uint32_t)(j * kFeat + 4 * lane) * 4, p));
+                s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+            }
+            const int t = tt * BT + j;
+            const float sx = __ldg(a.q_scale + t);
+            const int sums[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                if (n + i >= a.N) break;
+                float v = __fmaf_rn((float)sums[i], sx * __ldg(a.w_scale + n + i),
+                                    a.bias ? __ldg(a.bias + n + i) : 0.0f);
+                v = act_apply(v, a.act);
+                if (a.res) v += to_float(((const T *)a.res)[(long long)t * a.ldres + n + i]);
+                ((T *)a.y)[(long long)t * a.ldy + n + i] = from_float<T>(v);
+            }
+        }
+        cluster_sync();  // peers may still be reading this CTA's sums
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == kWarpMma)
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kCols)
+                     : "memory");
+}
+
+int sm_count() {
+    int dev = 0, n = 0;
+    cudaGetDevice(&dev);
+    cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+    return n > 0 ? n : 148;
+}
+
+template <typename T, int BT, bool SPLIT>
+Status launch(const LinearI8Args &p, Args a, int splits, cudaStream_t st) {
+    CUtensorMap tmW, tmQ;
+    if (!tma_encode_bytes(&tmW, p.w, p.K, p.N, p.ldw, kBK, kFeat) ||
+        !tma_encode_bytes(&tmQ, p.q, p.K, p.M, p.ldq, kBK, BT))
+        return ERR_SHAPE;
+    auto kernel = linear_i8_kernel<T, BT, SPLIT>;
+    constexpr int smem = smem_bytes(BT, SPLIT);
+    if (!smem_attr_once((const void *)kernel, smem)) {
+        cudaGetLastError();
+        return ERR_CUDA;
+    }
+    a.f_tiles = cdiv(p.N, kFeat);
+    a.t_tiles = cdiv(p.M, BT);
+    if ((long long)a.f_tiles * a.t_tiles > 0x3fffffff) return ERR_SHAPE;
+    a.tiles = a.f_tiles * a.t_tiles;
+    if (!SPLIT) {
+        const int sms = sm_count();
+        pdl_launch(kernel, a.tiles < sms ? a.tiles : sms, kThreads, smem, st, tmW, tmQ, a);
+        return cuda_status();
+    }
+    a.kps = cdiv(a.kblocks, splits);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(a.tiles * splits));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = (unsigned)splits;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = pdl_enabled() ? 2 : 1;
+    cudaLaunchKernelEx(&cfg, kernel, tmW, tmQ, a);
+    return cuda_status();
 }
 
 }  // namespace
 
-Status launch_quantize_rows(const Rows &x, int type, long long rows, int K, int8_t *q,
-                            long long ldq, float *scale, cudaStream_t st) {
-    if (rows == 0) return OK;
-    if (rows < 0 || rows > 0x7fffffffLL || K <= 0) return ERR_SHAPE;
-    return with_type(type, [&](auto t) {
+Status launch_linear_i8(const LinearI8Args &p, cudaStream_t st) {
+    if (p.M == 0) return OK;
+    if (p.M < 0 || p.N <= 0 || p.K <= 0) return ERR_SHAPE;
+    Args a = {};
+    a.M = p.M; a.N = p.N; a.kblocks = cdiv(p.K, kBK);
+    a.act = p.act;
+    a.q_scale = p.q_scale; a.w_scale = p.w_scale; a.bias = p.bias;
+    a.res = p.res.p; a.ldres = p.res.ld;
+    a.y = (void *)p.y.p; a.ldy = p.y.ld;
+    a.pairs = p.type != T_F32 && ((uintptr_t)a.y & 3) == 0 && (p.M == 1 || a.ldy % 2 == 0) &&
+              (!a.res || (((uintptr_t)a.res & 3) == 0 && (p.M == 1 || a.ldres % 2 == 0)));
+    return with_type(p.type, [&](auto t) {
         using T = decltype(t);
-        pdl_launch(quantize_rows_kernel<T>, (unsigned)rows, K >= 1024 ? 256 : 128, 0, st,
-                   (const T *)x.p, x.ld, K, q, ldq, scale);
-        return cuda_status();
+        const int sms = sm_count();
+        const long long f = cdiv(p.N, kFeat);
+        // few tiles: split K over clusters until two CTAs an SM are busy
+        const int bt = p.M <= 16 ? 16 : p.M <= 32 ? 32 : 64;
+        const long long tiles = f * cdiv(p.M, bt);
+        if (tiles < sms && a.kblocks > 1) {
+            int splits = (int)(2 * sms / tiles);
+            if (splits > 8) splits = 8;
+            if (splits > a.kblocks) splits = a.kblocks;
+            // whole k-blocks, none of the CTAs left without one
+            splits = cdiv(a.kblocks, cdiv(a.kblocks, splits));
+            if (splits > 1) {
+                if (bt == 16) return launch<T, 16, true>(p, a, splits, st);
+                if (bt == 32) return launch<T, 32, true>(p, a, splits, st);
+                return launch<T, 64, true>(p, a, splits, st);
+            }
+        }
+        if (f * cdiv(p.M, 256) >= sms) return launch<T, 256, false>(p, a, 1, st);
+        if (f * cdiv(p.M, 128) >= sms) return launch<T, 128, false>(p, a, 1, st);
+        if (p.M <= 16) return launch<T, 16, false>(p, a, 1, st);
+        return launch<T, 64, false>(p, a, 1, st);
     });
 }
 
-Status launch_linear_i8(const LinearI8Args &a, cudaStream_t st) {
-    if (a.M == 0) return OK;
-    if (a.M < 0 || a.N <= 0 || a.K <= 0 || cdiv(a.M, 16) > 65535) return ERR_SHAPE;
-    return with_type(a.type, [&](auto t) {
-        using T = decltype(t);
-        pdl_launch(linear_i8_simt_kernel<T>, dim3(cdiv(a.N, 16), cdiv(a.M, 16)), 256, 0, st, a);
-        return cuda_status();
-    });
+int linear_error_fetch_and_clear() {
+    int h = 0, zero = 0;
+    cudaMemcpyFromSymbol(&h, g_linear_error, sizeof(int));
+    if (h) cudaMemcpyToSymbol(g_linear_error, &zero, sizeof(int));
+    return h;
 }
 
 }  // namespace ppdl

@@ -12,6 +12,7 @@
 
 #include "../../include/ppdl_ops.h"
 #include "kernels.h"
+#include "block.h"
 #include "conv.h"
 #include "dec.h"
 #include "gemm_tc.h"
@@ -68,7 +69,10 @@ PPDL_OPS_API int ppdl_op_supported(const ppdl_op_desc *d) {
 
 PPDL_OPS_API const char *ppdl_op_last_error(void) { return g_err; }
 
-PPDL_OPS_API int ppdl_op_device_error(void) { return ppdl::tc_error_fetch_and_clear() ? 1 : 0; }
+PPDL_OPS_API int ppdl_op_device_error(void) {
+    const int gemm = ppdl::tc_error_fetch_and_clear(), linear = ppdl::linear_error_fetch_and_clear();
+    return gemm || linear ? 1 : 0;
+}
 
 PPDL_OPS_API int ppdl_gemm_tf32x3_presplit(int M, int N, int K, int batch, const float *A,
                                            int a_m_major, long long lda, long long a_bs,
