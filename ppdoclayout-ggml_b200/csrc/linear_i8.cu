@@ -185,73 +185,98 @@ __device__ __forceinline__ float finish(int acc, float scale, float bias) {
     return act_apply(__fmaf_rn((float)acc, scale, bias), ACT);
 }
 
-// Epilogue of C tokens t0 .. t0 + C - 1 of channel n (one per lane).
-template <typename T, int C, int ACT>
-__device__ __forceinline__ void epilogue_chunk(const Args &a, const uint32_t (&acc)[C], int t0,
-                                               int n, float sw, float bias, float sx, int lane) {
-    const bool n_ok = n < a.N;
-    const bool full = t0 + C <= a.M;
+// Epilogue of C tokens t0 .. t0 + C - 1 of channel n (one per lane), all of
+// them inside y.  No branch depends on a value, so that the C chains of
+// conversion, scale, activation and store overlap: with 2 warps a scheduler
+// there is nothing else to hide their latency.
+template <typename T, int C, int ACT, bool RES>
+__device__ __forceinline__ void epilogue_full(const Args &a, const uint32_t (&acc)[C], int t0, int n,
+                                              float sw, float bias, float sx, int lane) {
+    float v[C];
     if constexpr (sizeof(T) == 2) {
-        // lane pairs exchange values, so that the even lane holds token j and
-        // the odd lane token j + 1 of two neighbouring channels: one 4-byte
-        // store (and residual load) per lane and pair of tokens
-        if (a.pairs && n - lane + 32 <= a.N) {
+        if (a.pairs) {
+            // lane pairs exchange values, so that the even lane holds token j
+            // and the odd lane token j + 1 of two neighbouring channels: one
+            // 4-byte store (and residual load) per lane and pair of tokens
             const int odd = lane & 1;
             const long long first = t0 + odd, nn = n - odd;
-            uint32_t r[C / 2];
-            if (a.res) {
+            uint32_t r[RES ? C / 2 : 1];
+            if constexpr (RES) {
                 const T *rp = (const T *)a.res + first * a.ldres + nn;
 #pragma unroll
-                for (int j = 0; j < C; j += 2, rp += 2 * a.ldres) {
-                    r[j / 2] = 0;
-                    if (full || first + j < a.M) r[j / 2] = *reinterpret_cast<const uint32_t *>(rp);
-                }
+                for (int j = 0; j < C / 2; j++, rp += 2 * a.ldres)
+                    r[j] = *reinterpret_cast<const uint32_t *>(rp);
             }
+#pragma unroll
+            for (int j = 0; j < C; j++)
+                v[j] = finish<ACT>((int)acc[j], __shfl_sync(0xffffffffu, sx, j) * sw, bias);
             T *yp = (T *)a.y + first * a.ldy + nn;
 #pragma unroll
             for (int j = 0; j < C; j += 2, yp += 2 * a.ldy) {
-                const float s0 = __shfl_sync(0xffffffffu, sx, j) * sw;
-                const float s1 = __shfl_sync(0xffffffffu, sx, j + 1) * sw;
-                const float v0 = finish<ACT>((int)acc[j], s0, bias);
-                const float v1 = finish<ACT>((int)acc[j + 1], s1, bias);
-                const float other = __shfl_xor_sync(0xffffffffu, odd ? v0 : v1, 1);
-                float lo = odd ? other : v0, hi = odd ? v1 : other;
-                if (a.res) {
+                const float other = __shfl_xor_sync(0xffffffffu, odd ? v[j] : v[j + 1], 1);
+                float lo = odd ? other : v[j], hi = odd ? v[j + 1] : other;
+                if constexpr (RES) {
                     const float2 rr = unpack2<T>(r[j / 2]);
                     lo += rr.x;
                     hi += rr.y;
                 }
-                if (full || first + j < a.M) *reinterpret_cast<uint32_t *>(yp) = pack2<T>(lo, hi);
+                *reinterpret_cast<uint32_t *>(yp) = pack2<T>(lo, hi);
             }
             return;
         }
     }
-    float r[C];
-    if (a.res) {
+    T r[RES ? C : 1];
+    if constexpr (RES) {
         const T *rp = (const T *)a.res + (long long)t0 * a.ldres + n;
 #pragma unroll
-        for (int j = 0; j < C; j++, rp += a.ldres)
-            r[j] = n_ok && (full || t0 + j < a.M) ? to_float(*rp) : 0.0f;
+        for (int j = 0; j < C; j++, rp += a.ldres) r[j] = *rp;
     }
+#pragma unroll
+    for (int j = 0; j < C; j++)
+        v[j] = finish<ACT>((int)acc[j], __shfl_sync(0xffffffffu, sx, j) * sw, bias);
     T *yp = (T *)a.y + (long long)t0 * a.ldy + n;
 #pragma unroll
-    for (int j = 0; j < C; j++, yp += a.ldy) {
+    for (int j = 0; j < C; j++, yp += a.ldy)
+        *yp = from_float<T>(RES ? v[j] + to_float(r[RES ? j : 0]) : v[j]);
+}
+
+// The same at the edges of y.
+template <typename T, int C>
+__device__ __forceinline__ void epilogue_edge(const Args &a, const uint32_t (&acc)[C], int t0, int n,
+                                              float sw, float bias, float sx) {
+    const T *rp = (const T *)a.res + (long long)t0 * a.ldres + n;
+    T *yp = (T *)a.y + (long long)t0 * a.ldy + n;
+#pragma unroll
+    for (int j = 0; j < C; j++) {
         const float s = __shfl_sync(0xffffffffu, sx, j) * sw;
-        float v = finish<ACT>((int)acc[j], s, bias);
-        if (a.res) v += r[j];
-        if (n_ok && (full || t0 + j < a.M)) *yp = from_float<T>(v);
+        if (n < a.N && t0 + j < a.M) {
+            float v = act_apply(__fmaf_rn((float)(int)acc[j], s, bias), a.act);
+            if (a.res) v += to_float(rp[j * a.ldres]);
+            yp[j * a.ldy] = from_float<T>(v);
+        }
+    }
+}
+
+template <typename T, int C, bool RES>
+__device__ __forceinline__ void epilogue_act(const Args &a, const uint32_t (&acc)[C], int t0, int n,
+                                             float sw, float bias, float sx, int lane) {
+    switch (a.act) {
+        case ACT_RELU: epilogue_full<T, C, ACT_RELU, RES>(a, acc, t0, n, sw, bias, sx, lane); break;
+        case ACT_SILU: epilogue_full<T, C, ACT_SILU, RES>(a, acc, t0, n, sw, bias, sx, lane); break;
+        case ACT_GELU: epilogue_full<T, C, ACT_GELU, RES>(a, acc, t0, n, sw, bias, sx, lane); break;
+        default: epilogue_full<T, C, ACT_NONE, RES>(a, acc, t0, n, sw, bias, sx, lane);
     }
 }
 
 template <typename T, int C>
 __device__ __forceinline__ void epilogue_any(const Args &a, const uint32_t (&acc)[C], int t0, int n,
                                              float sw, float bias, float sx, int lane) {
-    switch (a.act) {
-        case ACT_RELU: epilogue_chunk<T, C, ACT_RELU>(a, acc, t0, n, sw, bias, sx, lane); break;
-        case ACT_SILU: epilogue_chunk<T, C, ACT_SILU>(a, acc, t0, n, sw, bias, sx, lane); break;
-        case ACT_GELU: epilogue_chunk<T, C, ACT_GELU>(a, acc, t0, n, sw, bias, sx, lane); break;
-        default: epilogue_chunk<T, C, ACT_NONE>(a, acc, t0, n, sw, bias, sx, lane);
-    }
+    if (t0 + C > a.M || n - lane + 32 > a.N)
+        epilogue_edge<T, C>(a, acc, t0, n, sw, bias, sx);
+    else if (a.res)
+        epilogue_act<T, C, true>(a, acc, t0, n, sw, bias, sx, lane);
+    else
+        epilogue_act<T, C, false>(a, acc, t0, n, sw, bias, sx, lane);
 }
 
 template <typename T, int BT, bool SPLIT>
