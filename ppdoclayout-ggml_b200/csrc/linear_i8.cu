@@ -45,26 +45,42 @@ __device__ int g_linear_error = 0;
 
 constexpr int kFeat = 128;  // channels per tile (MMA M)
 constexpr int kBK = 128;    // k per stage: one 128-byte swizzle row
-constexpr int kThreads = 384;
-constexpr int kWarpTma = 0, kWarpMma = 1, kWarpEpi = 4, kEpiWarps = 8;
+constexpr int kWarpTma = 0, kWarpMma = 1, kWarpScale = 2, kWarpEpi = 4;
 constexpr long long kTimeoutCycles = 4000000000LL;
-constexpr int kCtrlBytes = 256;
+// barriers, TMEM address and abort flag, then two tiles' scales: 128 channel
+// scales, 128 biases and up to 256 token scales each
+constexpr int kScaleFloats = 512;
+constexpr int kCtrlBytes = 256 + 2 * kScaleFloats * 4;
+constexpr int kAbortAt = 204;
 constexpr int kSmemMax = 227 * 1024;
 constexpr int kABytes = kFeat * kBK;
 
-constexpr int stage_bytes(int bt) { return kABytes + bt * kBK; }
+// The forms of the kernel.
+enum Form : int {
+    WHOLE = 0,  // a CTA per tile, persistent
+    PAIR = 1,   // two CTAs per tile of 256 channels, persistent
+    SPLIT = 2   // a cluster per tile, its k-blocks shared out
+};
+
+// epilogue warps: a multiple of 4, one or more per TMEM lane quadrant, each
+// with its share of the tile's tokens
+constexpr int epi_warps(int bt, int form) { return form != SPLIT && bt >= 128 ? 16 : 8; }
+constexpr int threads(int bt, int form) { return 32 * (kWarpEpi + epi_warps(bt, form)); }
+// token rows of a stage: a CTA of a pair loads half of them
+constexpr int load_tokens(int bt, int form) { return form == PAIR ? bt / 2 : bt; }
+constexpr int stage_bytes(int bt, int form) { return kABytes + load_tokens(bt, form) * kBK; }
 // stages in the ring: what fits beside the control block and the alignment
 // slack, at most 8; the split form keeps to 4 so that two CTAs share an SM
-constexpr int stages(int bt, bool split) {
-    const int fit = (kSmemMax - kCtrlBytes - 1024) / stage_bytes(bt);
-    const int most = split ? 4 : 8;
+constexpr int stages(int bt, int form) {
+    const int fit = (kSmemMax - kCtrlBytes - 1024) / stage_bytes(bt, form);
+    const int most = form == SPLIT ? 4 : 8;
     return fit < most ? fit : most;
 }
-constexpr int smem_bytes(int bt, bool split) {
-    return kCtrlBytes + 1024 + stages(bt, split) * stage_bytes(bt);
+constexpr int smem_bytes(int bt, int form) {
+    return kCtrlBytes + 1024 + stages(bt, form) * stage_bytes(bt, form);
 }
-constexpr uint32_t tmem_cols(int bt, bool split) {
-    const int c = split ? bt : 2 * bt;
+constexpr uint32_t tmem_cols(int bt, int form) {
+    const int c = form == SPLIT ? bt : 2 * bt;
     return c < 32 ? 32 : c;
 }
 
@@ -107,6 +123,45 @@ __device__ __forceinline__ void umma_i8(uint32_t d, uint64_t a, uint64_t b, uint
         "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
         "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
         : "memory");
+}
+
+// The same over a CTA pair: 256 rows of A, each CTA holding 128 of them and
+// half of B's rows, each CTA's TMEM the sums of its own rows.
+__device__ __forceinline__ void umma_i8_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                             uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+// arrives at the barrier of both CTAs of the pair
+__device__ __forceinline__ void umma_commit_pair(uint32_t bar) {
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64"
+        " [%0], %1;" ::"r"(bar),
+        "h"((uint16_t)3)
+        : "memory");
+}
+// a load into this CTA's shared memory that reports to the leader's barrier
+__device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap *tm, uint32_t bar,
+                                                 int x, int y) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4}], [%2];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(tm)), "r"(bar), "r"(x), "r"(y)
+        : "memory");
+}
+// Arrivals that publish nothing in memory: the epilogue has read its TMEM
+// columns (or scales) into registers.  A releasing arrive would wait for the
+// warp's stores to y, hundreds of cycles a tile.
+__device__ __forceinline__ void mbar_arrive_relaxed(uint32_t bar) {
+    asm volatile("mbarrier.arrive.relaxed.cta.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive_relaxed_cluster(uint32_t bar) {
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar)
+                 : "memory");
 }
 
 __device__ __forceinline__ void cluster_sync() {
@@ -185,13 +240,26 @@ __device__ __forceinline__ float finish(int acc, float scale, float bias) {
     return act_apply(__fmaf_rn((float)acc, scale, bias), ACT);
 }
 
+template <int C, int ACT>
+__device__ __forceinline__ void finish_all(float (&v)[C], const uint32_t (&acc)[C], const float *sx,
+                                           float sw, float bias) {
+#pragma unroll
+    for (int j = 0; j < C; j += 4) {
+        const float4 s = *reinterpret_cast<const float4 *>(sx + j);
+        v[j] = finish<ACT>((int)acc[j], s.x * sw, bias);
+        v[j + 1] = finish<ACT>((int)acc[j + 1], s.y * sw, bias);
+        v[j + 2] = finish<ACT>((int)acc[j + 2], s.z * sw, bias);
+        v[j + 3] = finish<ACT>((int)acc[j + 3], s.w * sw, bias);
+    }
+}
+
 // Epilogue of C tokens t0 .. t0 + C - 1 of channel n (one per lane), all of
 // them inside y.  No branch depends on a value, so that the C chains of
 // conversion, scale, activation and store overlap: with 2 warps a scheduler
 // there is nothing else to hide their latency.
 template <typename T, int C, int ACT, bool RES>
 __device__ __forceinline__ void epilogue_full(const Args &a, const uint32_t (&acc)[C], int t0, int n,
-                                              float sw, float bias, float sx, int lane) {
+                                              float sw, float bias, const float *sx, int lane) {
     float v[C];
     if constexpr (sizeof(T) == 2) {
         if (a.pairs) {
@@ -207,9 +275,7 @@ __device__ __forceinline__ void epilogue_full(const Args &a, const uint32_t (&ac
                 for (int j = 0; j < C / 2; j++, rp += 2 * a.ldres)
                     r[j] = *reinterpret_cast<const uint32_t *>(rp);
             }
-#pragma unroll
-            for (int j = 0; j < C; j++)
-                v[j] = finish<ACT>((int)acc[j], __shfl_sync(0xffffffffu, sx, j) * sw, bias);
+            finish_all<C, ACT>(v, acc, sx, sw, bias);
             T *yp = (T *)a.y + first * a.ldy + nn;
 #pragma unroll
             for (int j = 0; j < C; j += 2, yp += 2 * a.ldy) {
@@ -231,9 +297,7 @@ __device__ __forceinline__ void epilogue_full(const Args &a, const uint32_t (&ac
 #pragma unroll
         for (int j = 0; j < C; j++, rp += a.ldres) r[j] = *rp;
     }
-#pragma unroll
-    for (int j = 0; j < C; j++)
-        v[j] = finish<ACT>((int)acc[j], __shfl_sync(0xffffffffu, sx, j) * sw, bias);
+    finish_all<C, ACT>(v, acc, sx, sw, bias);
     T *yp = (T *)a.y + (long long)t0 * a.ldy + n;
 #pragma unroll
     for (int j = 0; j < C; j++, yp += a.ldy)
@@ -243,14 +307,13 @@ __device__ __forceinline__ void epilogue_full(const Args &a, const uint32_t (&ac
 // The same at the edges of y.
 template <typename T, int C>
 __device__ __forceinline__ void epilogue_edge(const Args &a, const uint32_t (&acc)[C], int t0, int n,
-                                              float sw, float bias, float sx) {
+                                              float sw, float bias, const float *sx) {
     const T *rp = (const T *)a.res + (long long)t0 * a.ldres + n;
     T *yp = (T *)a.y + (long long)t0 * a.ldy + n;
 #pragma unroll
     for (int j = 0; j < C; j++) {
-        const float s = __shfl_sync(0xffffffffu, sx, j) * sw;
         if (n < a.N && t0 + j < a.M) {
-            float v = act_apply(__fmaf_rn((float)(int)acc[j], s, bias), a.act);
+            float v = act_apply(__fmaf_rn((float)(int)acc[j], sx[j] * sw, bias), a.act);
             if (a.res) v += to_float(rp[j * a.ldres]);
             yp[j * a.ldy] = from_float<T>(v);
         }
@@ -259,7 +322,7 @@ __device__ __forceinline__ void epilogue_edge(const Args &a, const uint32_t (&ac
 
 template <typename T, int C, bool RES>
 __device__ __forceinline__ void epilogue_act(const Args &a, const uint32_t (&acc)[C], int t0, int n,
-                                             float sw, float bias, float sx, int lane) {
+                                             float sw, float bias, const float *sx, int lane) {
     switch (a.act) {
         case ACT_RELU: epilogue_full<T, C, ACT_RELU, RES>(a, acc, t0, n, sw, bias, sx, lane); break;
         case ACT_SILU: epilogue_full<T, C, ACT_SILU, RES>(a, acc, t0, n, sw, bias, sx, lane); break;
@@ -270,7 +333,7 @@ __device__ __forceinline__ void epilogue_act(const Args &a, const uint32_t (&acc
 
 template <typename T, int C>
 __device__ __forceinline__ void epilogue_any(const Args &a, const uint32_t (&acc)[C], int t0, int n,
-                                             float sw, float bias, float sx, int lane) {
+                                             float sw, float bias, const float *sx, int lane) {
     if (t0 + C > a.M || n - lane + 32 > a.N)
         epilogue_edge<T, C>(a, acc, t0, n, sw, bias, sx);
     else if (a.res)
@@ -279,20 +342,26 @@ __device__ __forceinline__ void epilogue_any(const Args &a, const uint32_t (&acc
         epilogue_act<T, C, false>(a, acc, t0, n, sw, bias, sx, lane);
 }
 
-template <typename T, int BT, bool SPLIT>
-__global__ void __launch_bounds__(kThreads, SPLIT ? 2 : 1)
+template <typename T, int BT, int FORM>
+__global__ void __launch_bounds__(threads(BT, FORM), FORM == SPLIT ? 2 : 1)
 linear_i8_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmQ,
                  const __grid_constant__ Args a) {
-    constexpr int S = stages(BT, SPLIT), kAcc = SPLIT ? 1 : 2;
-    constexpr uint32_t kStage = stage_bytes(BT), kCols = tmem_cols(BT, SPLIT);
+    constexpr int S = stages(BT, FORM), kAcc = FORM == SPLIT ? 1 : 2;
+    constexpr int kEpiWarps = epi_warps(BT, FORM), kLoadT = load_tokens(BT, FORM);
+    constexpr int kTileF = FORM == PAIR ? 2 * kFeat : kFeat;  // channels per tile
+    constexpr uint32_t kStage = stage_bytes(BT, FORM), kCols = tmem_cols(BT, FORM);
     extern __shared__ uint8_t smem_raw[];
     const uint32_t ctrl = smem_u32(smem_raw);
-    // full[s]: a stage's bytes landed; empty[s]: its MMAs completed;
-    // tfull[i]: accumulator i complete; tempty[i]: read by the epilogue
+    // full[s]: a stage's bytes landed (pair: both CTAs', in the leader);
+    // empty[s]: its MMAs completed; tfull[i]: accumulator i complete;
+    // tempty[i]: read by the epilogue (pair: both CTAs', in the leader);
+    // sfull[i] / sempty[i]: a tile's scales written / read
     const uint32_t bar_full = ctrl, bar_empty = ctrl + 64, bar_tfull = ctrl + 128,
-                   bar_tempty = ctrl + 144, bar_done = ctrl + 160;
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem_raw + 176);
-    volatile int *abort_flag = reinterpret_cast<volatile int *>(smem_raw + 180);
+                   bar_tempty = ctrl + 144, bar_done = ctrl + 160, bar_sfull = ctrl + 168,
+                   bar_sempty = ctrl + 184;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem_raw + 200);
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(smem_raw + kAbortAt);
+    float *scales = reinterpret_cast<float *>(smem_raw + 256);
     const uint32_t stage0 = (ctrl + kCtrlBytes + 1023) & ~1023u;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
@@ -303,30 +372,42 @@ linear_i8_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
         }
         for (int i = 0; i < 2; i++) {
             mbar_init(bar_tfull + 8 * i, 1);
-            mbar_init(bar_tempty + 8 * i, kEpiWarps);
+            mbar_init(bar_tempty + 8 * i, FORM == PAIR ? 2 * kEpiWarps : kEpiWarps);
+            mbar_init(bar_sfull + 8 * i, 1);
+            mbar_init(bar_sempty + 8 * i, kEpiWarps);
         }
         mbar_init(bar_done, 1);
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == kWarpMma) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
-                         smem_u32(tmem_slot)),
-                     "r"(kCols)
-                     : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        if constexpr (FORM == PAIR) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                             smem_u32(tmem_slot)),
+                         "r"(kCols)
+                         : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                             smem_u32(tmem_slot)),
+                         "r"(kCols)
+                         : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        }
     }
     tc_fence_before();
     __syncthreads();
+    if constexpr (FORM == PAIR) cluster_sync();  // the peer's barriers are set up
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
     pdl_begin();
 
-    const uint32_t rank = SPLIT ? cluster_rank() : 0, peers = SPLIT ? cluster_size() : 1;
-    const int first = SPLIT ? (int)(blockIdx.x / peers) : (int)blockIdx.x;
-    const int step = SPLIT ? a.tiles : (int)gridDim.x;  // split form: one tile
-    const int kb0 = SPLIT ? (int)rank * a.kps : 0;
-    const int kbn = SPLIT ? max(0, min(a.kps, a.kblocks - kb0)) : a.kblocks;
+    const uint32_t rank = FORM == WHOLE ? 0 : cluster_rank();
+    const uint32_t peers = FORM == WHOLE ? 1 : FORM == PAIR ? 2 : cluster_size();
+    const int first = (int)(blockIdx.x / peers);
+    const int step = FORM == SPLIT ? a.tiles : (int)(gridDim.x / peers);  // split: one tile
+    const int kb0 = FORM == SPLIT ? (int)rank * a.kps : 0;
+    const int kbn = FORM == SPLIT ? max(0, min(a.kps, a.kblocks - kb0)) : a.kblocks;
 
     if (warp == kWarpTma) {
         if (lane == 0) {
@@ -341,23 +422,40 @@ linear_i8_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
                         ok = false;
                         break;
                     }
-                    const uint32_t st = stage0 + rs.i * kStage, fb = bar_full + 8 * rs.i;
-                    mbar_expect_tx(fb, kStage);
-                    tma_load_2d(st, &tmW, fb, (kb0 + kb) * kBK, ft * kFeat);
-                    tma_load_2d(st + kABytes, &tmQ, fb, (kb0 + kb) * kBK, tt * BT);
+                    const uint32_t st = stage0 + rs.i * kStage;
+                    const int k = (kb0 + kb) * kBK;
+                    if constexpr (FORM == PAIR) {
+                        const uint32_t fb = peer_addr(bar_full + 8 * rs.i, 0);
+                        if (rank == 0) mbar_expect_tx(bar_full + 8 * rs.i, 2 * kStage);
+                        tma_load_2d_pair(st, &tmW, fb, k, ft * kTileF + (int)rank * kFeat);
+                        tma_load_2d_pair(st + kABytes, &tmQ, fb, k, tt * BT + (int)rank * kLoadT);
+                    } else {
+                        const uint32_t fb = bar_full + 8 * rs.i;
+                        mbar_expect_tx(fb, kStage);
+                        tma_load_2d(st, &tmW, fb, k, ft * kTileF);
+                        tma_load_2d(st + kABytes, &tmQ, fb, k, tt * BT);
+                    }
                 }
             }
-            // what was issued must land before the CTA may exit
-            for (long long j = it > S ? it - S : 0; j < it; j++) {
-                int dummy = 0;
-                wait_for(bar_full + 8 * (int)(j % S), (uint32_t)((j / S) & 1), (volatile int *)&dummy);
-            }
+            // what was issued must land before the CTA may exit (pair: the
+            // leader waits for both, the peer at the cluster's last barrier)
+            if (FORM != PAIR || rank == 0)
+                for (long long j = it > S ? it - S : 0; j < it; j++) {
+                    int dummy = 0;
+                    wait_for(bar_full + 8 * (int)(j % S), (uint32_t)((j / S) & 1),
+                             (volatile int *)&dummy);
+                }
         }
     } else if (warp == kWarpMma) {
-        if (lane == 0) {
+        if (lane == 0 && (FORM != PAIR || rank == 0)) {
             // S32 accumulators, signed 8-bit A and B, both K-major
             constexpr uint32_t idesc = (2u << 4) | (1u << 7) | (1u << 10) |
-                                       ((uint32_t)(BT >> 3) << 17) | ((uint32_t)(kFeat >> 4) << 24);
+                                       ((uint32_t)(BT >> 3) << 17) |
+                                       ((uint32_t)(kTileF >> 4) << 24);
+            auto commit = [](uint32_t bar) {
+                if constexpr (FORM == PAIR) umma_commit_pair(bar);
+                else umma_commit(bar);
+            };
             Ring rs(S), ra(kAcc);
             bool ok = true;
             for (int tile = first; tile < a.tiles && ok; tile += step, ra.next()) {
@@ -376,77 +474,122 @@ linear_i8_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
                     const uint64_t da = smem_desc(st, 16, 1024, 2);
                     const uint64_t db = smem_desc(st + kABytes, 16, 1024, 2);
 #pragma unroll
-                    for (int k = 0; k < kBK / 32; k++)
-                        umma_i8(d, da + 2 * k, db + 2 * k, idesc, (kb | k) != 0);
-                    umma_commit(bar_empty + 8 * rs.i);
+                    for (int k = 0; k < kBK / 32; k++) {
+                        if constexpr (FORM == PAIR)
+                            umma_i8_pair(d, da + 2 * k, db + 2 * k, idesc, (kb | k) != 0);
+                        else
+                            umma_i8(d, da + 2 * k, db + 2 * k, idesc, (kb | k) != 0);
+                    }
+                    commit(bar_empty + 8 * rs.i);
                 }
-                if (ok) umma_commit(bar_tfull + 8 * ra.i);
+                if (ok) commit(bar_tfull + 8 * ra.i);
             }
             // all issued MMAs must finish before TMEM is released
-            umma_commit(bar_done);
+            commit(bar_done);
             int dummy = 0;
             wait_for(bar_done, 0, (volatile int *)&dummy);
         }
+    } else if (FORM != SPLIT && warp == kWarpScale) {
+        // the scales of each tile, one ahead of the epilogue: loaded by the
+        // epilogue itself they queue behind its stores
+        constexpr int kScaleT = (BT + 31) / 32;
+        Ring ra(kAcc);
+        for (int tile = first; tile < a.tiles; tile += step, ra.next()) {
+            int ft, tt;
+            tile_of(a, tile, ft, tt);
+            const int n0 = ft * kTileF + (FORM == PAIR ? (int)rank * kFeat : 0), m0 = tt * BT;
+            float v[2 * kFeat / 32 + kScaleT];
+#pragma unroll
+            for (int i = 0; i < kFeat / 32; i++) {
+                const int n = n0 + 32 * i + lane;
+                v[2 * i] = n < a.N ? __ldg(a.w_scale + n) : 0.0f;
+                v[2 * i + 1] = a.bias && n < a.N ? __ldg(a.bias + n) : 0.0f;
+            }
+#pragma unroll
+            for (int i = 0; i < kScaleT; i++)
+                v[2 * kFeat / 32 + i] =
+                    m0 + 32 * i + lane < a.M ? __ldg(a.q_scale + m0 + 32 * i + lane) : 0.0f;
+            bool good = true;
+            if (lane == 0) good = wait_for(bar_sempty + 8 * ra.i, ra.ph ^ 1, abort_flag);
+            if (!__shfl_sync(0xffffffffu, good ? 1 : 0, 0)) break;
+            float *sc = scales + ra.i * kScaleFloats;
+#pragma unroll
+            for (int i = 0; i < kFeat / 32; i++) {
+                sc[32 * i + lane] = v[2 * i];
+                sc[kFeat + 32 * i + lane] = v[2 * i + 1];
+            }
+#pragma unroll
+            for (int i = 0; i < kScaleT; i++) sc[2 * kFeat + 32 * i + lane] = v[2 * kFeat / 32 + i];
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar_sfull + 8 * ra.i);
+        }
     } else if (warp >= kWarpEpi) {
-        constexpr int kHalf = BT / 2, C = kHalf < 32 ? kHalf : 32;
+        constexpr int kPart = BT / (kEpiWarps / 4), C = kPart < 32 ? kPart : 32;
         const int quad = warp & 3, part = (warp - kWarpEpi) >> 2;
         const uint32_t lane_base = (uint32_t)(quad * 32) << 16;
         Ring ra(kAcc);
         for (int tile = first; tile < a.tiles; tile += step, ra.next()) {
             int ft, tt;
             tile_of(a, tile, ft, tt);
-            const int n = ft * kFeat + quad * 32 + lane;
-            float sw = 0.0f, bias = 0.0f;
-            if (!SPLIT && n < a.N) {
-                sw = __ldg(a.w_scale + n);
-                if (a.bias) bias = __ldg(a.bias + n);
-            }
+            const int n = ft * kTileF + (FORM == PAIR ? (int)rank * kFeat : 0) + quad * 32 + lane;
             bool good = true;
-            if (lane == 0) good = wait_for(bar_tfull + 8 * ra.i, ra.ph, abort_flag);
+            if (lane == 0)
+                good = (FORM == SPLIT || wait_for(bar_sfull + 8 * ra.i, ra.ph, abort_flag)) &&
+                       wait_for(bar_tfull + 8 * ra.i, ra.ph, abort_flag);
             if (!__shfl_sync(0xffffffffu, good ? 1 : 0, 0)) break;
             tc_fence_after();
-            const uint32_t col = tmem + lane_base + (uint32_t)(ra.i * BT + part * kHalf);
+            const uint32_t col = tmem + lane_base + (uint32_t)(ra.i * BT + part * kPart);
+            const float *sc = scales + ra.i * kScaleFloats;
+            const float sw = FORM == SPLIT ? 0.0f : sc[quad * 32 + lane];
+            const float bias = FORM == SPLIT ? 0.0f : sc[kFeat + quad * 32 + lane];
+            const float *sx = sc + 2 * kFeat + part * kPart;
 #pragma unroll 1
-            for (int c = 0; c < kHalf; c += C) {
-                const int t0 = tt * BT + part * kHalf + c;
+            for (int c = 0; c < kPart; c += C) {
+                const int t0 = tt * BT + part * kPart + c;
                 uint32_t acc[C];
                 tmem_load(col + c, acc);
-                if (c + C >= kHalf) {
+                if (c + C >= kPart) {
                     tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(bar_tempty + 8 * ra.i);
+                    if (lane == 0) {
+                        if constexpr (FORM == PAIR)
+                            mbar_arrive_relaxed_cluster(peer_addr(bar_tempty + 8 * ra.i, 0));
+                        else
+                            mbar_arrive_relaxed(bar_tempty + 8 * ra.i);
+                    }
                 }
-                if constexpr (SPLIT) {
+                if constexpr (FORM == SPLIT) {
                     // partial sums, token-major: [BT][128] in the stages, all of
                     // which the MMAs have read
                     int *part_sum = reinterpret_cast<int *>(smem_raw + (stage0 - ctrl));
 #pragma unroll
                     for (int j = 0; j < C; j++)
-                        part_sum[(part * kHalf + c + j) * kFeat + quad * 32 + lane] =
+                        part_sum[(part * kPart + c + j) * kFeat + quad * 32 + lane] =
                             kbn ? (int)acc[j] : 0;
-                } else if (t0 < a.M) {
-                    float sx = 0.0f;
-                    if (lane < C && t0 + lane < a.M) sx = __ldg(a.q_scale + t0 + lane);
-                    epilogue_any<T, C>(a, acc, t0, n, sw, bias, sx, lane);
+                } else if (t0 < a.M && n - lane < a.N) {
+                    epilogue_any<T, C>(a, acc, t0, n, sw, bias, sx + c, lane);
                 }
+            }
+            if constexpr (FORM != SPLIT) {
+                __syncwarp();
+                if (lane == 0) mbar_arrive_relaxed(bar_sempty + 8 * ra.i);
             }
         }
     }
     __syncwarp();
 
-    if constexpr (SPLIT) {
+    if constexpr (FORM == SPLIT) {
         cluster_sync();
         // this CTA's share of the tokens: 4 neighbouring channels a thread,
-        // 12 tokens at a time
+        // a token per warp at a time
         int ft, tt;
         tile_of(a, first, ft, tt);
         const int share = (BT + (int)peers - 1) / (int)peers;
         const int lo = (int)rank * share, hi = min(min(BT, lo + share), a.M - tt * BT);
         int bad = 0;
-        for (uint32_t p = 0; p < peers; p++)
-            bad |= peer_load1(peer_addr(ctrl + 180, p));
+        for (uint32_t p = 0; p < peers; p++) bad |= peer_load1(peer_addr(ctrl + kAbortAt, p));
         const int n = ft * kFeat + 4 * lane;
-        for (int j = lo + warp; j < hi && !bad; j += kThreads / 32) {
+        for (int j = lo + warp; j < hi && !bad; j += threads(BT, FORM) / 32) {
             int4 s = make_int4(0, 0, 0, 0);
             for (uint32_t p = 0; p < peers; p++) {
                 const int4 v = peer_load(peer_addr(stage0 + (uint32_t)(j * kFeat + 4 * lane) * 4, p));
@@ -465,15 +608,23 @@ linear_i8_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
                 ((T *)a.y)[(long long)t * a.ldy + n + i] = from_float<T>(v);
             }
         }
-        cluster_sync();  // peers may still be reading this CTA's sums
     }
-
+    // split: peers may still be reading this CTA's sums; pair: the leader's
+    // MMAs read the peer's shared memory and write its TMEM
     tc_fence_before();
-    __syncthreads();
+    if constexpr (FORM == WHOLE) __syncthreads();
+    else cluster_sync();
     tc_fence_after();
-    if (warp == kWarpMma)
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kCols)
-                     : "memory");
+    if (warp == kWarpMma) {
+        if constexpr (FORM == PAIR)
+            asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem),
+                         "r"(kCols)
+                         : "memory");
+        else
+            asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem),
+                         "r"(kCols)
+                         : "memory");
+    }
 }
 
 int sm_count() {
@@ -483,36 +634,36 @@ int sm_count() {
     return n > 0 ? n : 148;
 }
 
-template <typename T, int BT, bool SPLIT>
+template <typename T, int BT, int FORM>
 Status launch(const LinearI8Args &p, Args a, int splits, cudaStream_t st) {
     CUtensorMap tmW, tmQ;
     if (!tma_encode_bytes(&tmW, p.w, p.K, p.N, p.ldw, kBK, kFeat) ||
-        !tma_encode_bytes(&tmQ, p.q, p.K, p.M, p.ldq, kBK, BT))
+        !tma_encode_bytes(&tmQ, p.q, p.K, p.M, p.ldq, kBK, load_tokens(BT, FORM)))
         return ERR_SHAPE;
-    auto kernel = linear_i8_kernel<T, BT, SPLIT>;
-    constexpr int smem = smem_bytes(BT, SPLIT);
+    auto kernel = linear_i8_kernel<T, BT, FORM>;
+    constexpr int smem = smem_bytes(BT, FORM);
     if (!smem_attr_once((const void *)kernel, smem)) {
         cudaGetLastError();
         return ERR_CUDA;
     }
-    a.f_tiles = cdiv(p.N, kFeat);
+    a.f_tiles = cdiv(p.N, FORM == PAIR ? 2 * kFeat : kFeat);
     a.t_tiles = cdiv(p.M, BT);
-    if ((long long)a.f_tiles * a.t_tiles > 0x3fffffff) return ERR_SHAPE;
+    if ((long long)a.f_tiles * a.t_tiles > 0x0fffffff) return ERR_SHAPE;
     a.tiles = a.f_tiles * a.t_tiles;
-    if (!SPLIT) {
-        const int sms = sm_count();
-        pdl_launch(kernel, a.tiles < sms ? a.tiles : sms, kThreads, smem, st, tmW, tmQ, a);
-        return cuda_status();
-    }
     a.kps = cdiv(a.kblocks, splits);
+    // CTAs of a cluster, and clusters: one for each tile (split) or as many
+    // as the SMs hold
+    const int cluster = FORM == PAIR ? 2 : FORM == SPLIT ? splits : 1;
+    const int most = FORM == SPLIT ? a.tiles : sm_count() / cluster;
+    const int clusters = a.tiles < most ? a.tiles : most;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(a.tiles * splits));
-    cfg.blockDim = dim3(kThreads);
+    cfg.gridDim = dim3((unsigned)(clusters * cluster));
+    cfg.blockDim = dim3(threads(BT, FORM));
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = (unsigned)splits;
+    at[0].val.clusterDim.x = (unsigned)cluster;
     at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
     at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[1].val.programmaticStreamSerializationAllowed = 1;
@@ -549,15 +700,16 @@ Status launch_linear_i8(const LinearI8Args &p, cudaStream_t st) {
             // whole k-blocks, none of the CTAs left without one
             splits = cdiv(a.kblocks, cdiv(a.kblocks, splits));
             if (splits > 1) {
-                if (bt == 16) return launch<T, 16, true>(p, a, splits, st);
-                if (bt == 32) return launch<T, 32, true>(p, a, splits, st);
-                return launch<T, 64, true>(p, a, splits, st);
+                if (bt == 16) return launch<T, 16, SPLIT>(p, a, splits, st);
+                if (bt == 32) return launch<T, 32, SPLIT>(p, a, splits, st);
+                return launch<T, 64, SPLIT>(p, a, splits, st);
             }
         }
-        if (f * cdiv(p.M, 256) >= sms) return launch<T, 256, false>(p, a, 1, st);
-        if (f * cdiv(p.M, 128) >= sms) return launch<T, 128, false>(p, a, 1, st);
-        if (p.M <= 16) return launch<T, 16, false>(p, a, 1, st);
-        return launch<T, 64, false>(p, a, 1, st);
+        if (getenv("LIN_PAIR") && f * cdiv(p.M, 256) >= sms) return launch<T, 256, PAIR>(p, a, 1, st);
+        if (f * cdiv(p.M, 256) >= sms) return launch<T, 256, WHOLE>(p, a, 1, st);
+        if (f * cdiv(p.M, 128) >= sms) return launch<T, 128, WHOLE>(p, a, 1, st);
+        if (p.M <= 16) return launch<T, 16, WHOLE>(p, a, 1, st);
+        return launch<T, 64, WHOLE>(p, a, 1, st);
     });
 }
 

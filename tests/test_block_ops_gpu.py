@@ -343,7 +343,7 @@ LIN_SHAPES = [(1, 1, 1), (1, 16, 7), (2, 17, 3), (1, 4096, 512), (1, 1000, 333),
               (8, 2048, 256), (16, 512, 1000), (17, 515, 130), (33, 64, 64), (64, 128, 200),
               (100, 256, 300), (128, 128, 128), (129, 130, 257), (300, 256, 1024), (300, 2048, 256),
               (511, 1111, 127), (1000, 96, 2047), (2400, 256, 256), (777, 1111, 513), (5000, 40, 40),
-              (1, 33000, 40), (2049, 513, 1025)]
+              (1, 33000, 40), (2049, 513, 1025), (5003, 200, 2100), (3001, 70, 3333), (19000, 130, 256)]
 
 
 @pytest.mark.parametrize("t", TYPES)
