@@ -84,9 +84,24 @@ constexpr uint32_t tmem_cols(int bt, int form) {
     return c < 32 ? 32 : c;
 }
 
+// n / d for 0 <= n < 2^31 by a multiplication (Granlund and Montgomery,
+// "Division by invariant integers using multiplication", PLDI 1994)
+struct FastDiv {
+    uint32_t d = 1, mul = 1, shift = 0;
+    FastDiv() = default;
+    explicit FastDiv(uint32_t d_) : d(d_) {
+        while ((1ull << shift) < d) shift++;
+        mul = (uint32_t)((((1ull << shift) - d) << 32) / d + 1);
+    }
+    __device__ __forceinline__ int div(int n) const {
+        return (int)((__umulhi((uint32_t)n, mul) + (uint32_t)n) >> shift);
+    }
+};
+
 struct Args {
     int M, N, kblocks;
     int f_tiles, t_tiles, tiles;
+    FastDiv group;  // by the tiles of a whole group
     int kps;  // split form: k-blocks per CTA of the cluster
     int act;
     int pairs;  // 16-bit rows of y and res start on 4 bytes
@@ -201,12 +216,11 @@ __device__ __forceinline__ int peer_load1(uint32_t addr) {
 // tile index -> (channel tile, token tile): token tiles in groups of 8, the
 // group's channel tiles outer, so that the CTAs that run at one time share
 // both operands in L2
+constexpr int kGroup = 8;
 __device__ __forceinline__ void tile_of(const Args &a, int tile, int &ft, int &tt) {
-    constexpr int kGroup = 8;
-    const int per = kGroup * a.f_tiles;
-    const int g = tile / per, r = tile - g * per;
+    const int g = a.group.div(tile), r = tile - g * (kGroup * a.f_tiles);
     const int width = min(kGroup, a.t_tiles - g * kGroup);
-    ft = r / width;
+    ft = width == kGroup ? r / kGroup : r / width;
     tt = g * kGroup + r - ft * width;
 }
 
@@ -233,36 +247,60 @@ __device__ __forceinline__ float2 unpack2<__half>(uint32_t v) {
     return __half22float2(*reinterpret_cast<const __half2 *>(&v));
 }
 
-// What follows the sum.  acc is rounded to FP32 (2^-24 relative), the two
-// scales are multiplied first (they are the same for a whole row or column).
-template <int ACT>
-__device__ __forceinline__ float finish(int acc, float scale, float bias) {
-    return act_apply(__fmaf_rn((float)acc, scale, bias), ACT);
+// Two FP32 values in one register pair: sm_100 multiplies and adds them in
+// one instruction, each rounded as its own.
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 r;
+    asm("{\n\t.reg .b64 x, y, z;\n\t"
+        "mov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
+        "mul.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"
+        : "=f"(r.x), "=f"(r.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 r;
+    asm("{\n\t.reg .b64 x, y, z, w;\n\t"
+        "mov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 w, {%6, %7};\n\t"
+        "fma.rn.f32x2 z, x, y, w;\n\tmov.b64 {%0, %1}, z;\n\t}"
+        : "=f"(r.x), "=f"(r.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return r;
 }
 
+// What follows the sum.  acc is rounded to FP32 (2^-24 relative), the two
+// scales are multiplied first (they are the same for a whole row or column).
 template <int C, int ACT>
 __device__ __forceinline__ void finish_all(float (&v)[C], const uint32_t (&acc)[C], const float *sx,
                                            float sw, float bias) {
+    const float2 sw2 = make_float2(sw, sw), bias2 = make_float2(bias, bias);
 #pragma unroll
     for (int j = 0; j < C; j += 4) {
         const float4 s = *reinterpret_cast<const float4 *>(sx + j);
-        v[j] = finish<ACT>((int)acc[j], s.x * sw, bias);
-        v[j + 1] = finish<ACT>((int)acc[j + 1], s.y * sw, bias);
-        v[j + 2] = finish<ACT>((int)acc[j + 2], s.z * sw, bias);
-        v[j + 3] = finish<ACT>((int)acc[j + 3], s.w * sw, bias);
+        const float2 s01 = mul2(make_float2(s.x, s.y), sw2), s23 = mul2(make_float2(s.z, s.w), sw2);
+        const float2 a01 = make_float2((float)(int)acc[j], (float)(int)acc[j + 1]);
+        const float2 a23 = make_float2((float)(int)acc[j + 2], (float)(int)acc[j + 3]);
+        const float2 v01 = fma2(a01, s01, bias2), v23 = fma2(a23, s23, bias2);
+        v[j] = act_apply(v01.x, ACT);
+        v[j + 1] = act_apply(v01.y, ACT);
+        v[j + 2] = act_apply(v23.x, ACT);
+        v[j + 3] = act_apply(v23.y, ACT);
     }
 }
 
-// Epilogue of C tokens t0 .. t0 + C - 1 of channel n (one per lane), all of
-// them inside y.  No branch depends on a value, so that the C chains of
-// conversion, scale, activation and store overlap: with 2 warps a scheduler
-// there is nothing else to hide their latency.
-template <typename T, int C, int ACT, bool RES>
-__device__ __forceinline__ void epilogue_full(const Args &a, const uint32_t (&acc)[C], int t0, int n,
-                                              float sw, float bias, const float *sx, int lane) {
+// Epilogue of C tokens t0 .. t0 + C - 1 of channel n (one per lane).  No
+// branch depends on a value, so that the C chains of conversion, scale,
+// activation and store overlap: with 2 to 4 warps a scheduler there is
+// little else to hide their latency.  EDGE: some of the tokens or lanes lie
+// past y, their loads and stores are predicated off.
+template <typename T, int C, int ACT, bool RES, bool EDGE>
+__device__ __forceinline__ void epilogue_chunk(const Args &a, const uint32_t (&acc)[C], int t0,
+                                               int n, float sw, float bias, const float *sx,
+                                               int lane) {
     float v[C];
+    const int tokens = EDGE ? a.M - t0 : C;
     if constexpr (sizeof(T) == 2) {
-        if (a.pairs) {
+        if (a.pairs && (!EDGE || n - lane + 32 <= a.N)) {
             // lane pairs exchange values, so that the even lane holds token j
             // and the odd lane token j + 1 of two neighbouring channels: one
             // 4-byte store (and residual load) per lane and pair of tokens
@@ -272,74 +310,74 @@ __device__ __forceinline__ void epilogue_full(const Args &a, const uint32_t (&ac
             if constexpr (RES) {
                 const T *rp = (const T *)a.res + first * a.ldres + nn;
 #pragma unroll
-                for (int j = 0; j < C / 2; j++, rp += 2 * a.ldres)
-                    r[j] = *reinterpret_cast<const uint32_t *>(rp);
+                for (int j = 0; j < C; j += 2, rp += 2 * a.ldres) {
+                    r[j / 2] = 0;
+                    if (!EDGE || j + odd < tokens)
+                        r[j / 2] = *reinterpret_cast<const uint32_t *>(rp);
+                }
             }
             finish_all<C, ACT>(v, acc, sx, sw, bias);
             T *yp = (T *)a.y + first * a.ldy + nn;
 #pragma unroll
             for (int j = 0; j < C; j += 2, yp += 2 * a.ldy) {
-                const float other = __shfl_xor_sync(0xffffffffu, odd ? v[j] : v[j + 1], 1);
-                float lo = odd ? other : v[j], hi = odd ? v[j + 1] : other;
+                uint32_t out;
                 if constexpr (RES) {
+                    const float other = __shfl_xor_sync(0xffffffffu, odd ? v[j] : v[j + 1], 1);
                     const float2 rr = unpack2<T>(r[j / 2]);
-                    lo += rr.x;
-                    hi += rr.y;
+                    out = pack2<T>((odd ? other : v[j]) + rr.x, (odd ? v[j + 1] : other) + rr.y);
+                } else {
+                    // already at its last rounding: exchange the packed pair
+                    // (token j in the low half), then take one half of each
+                    const uint32_t own = pack2<T>(v[j], v[j + 1]);
+                    const uint32_t other = __shfl_xor_sync(0xffffffffu, own, 1);
+                    out = __byte_perm(own, other, odd ? 0x3276 : 0x5410);
                 }
-                *reinterpret_cast<uint32_t *>(yp) = pack2<T>(lo, hi);
+                if (!EDGE || j + odd < tokens) *reinterpret_cast<uint32_t *>(yp) = out;
             }
             return;
         }
     }
+    const int mine = EDGE && n >= a.N ? 0 : tokens;
     T r[RES ? C : 1];
     if constexpr (RES) {
         const T *rp = (const T *)a.res + (long long)t0 * a.ldres + n;
 #pragma unroll
-        for (int j = 0; j < C; j++, rp += a.ldres) r[j] = *rp;
+        for (int j = 0; j < C; j++, rp += a.ldres) {
+            r[j] = from_float<T>(0.0f);
+            if (!EDGE || j < mine) r[j] = *rp;
+        }
     }
     finish_all<C, ACT>(v, acc, sx, sw, bias);
     T *yp = (T *)a.y + (long long)t0 * a.ldy + n;
 #pragma unroll
-    for (int j = 0; j < C; j++, yp += a.ldy)
-        *yp = from_float<T>(RES ? v[j] + to_float(r[RES ? j : 0]) : v[j]);
-}
-
-// The same at the edges of y.
-template <typename T, int C>
-__device__ __forceinline__ void epilogue_edge(const Args &a, const uint32_t (&acc)[C], int t0, int n,
-                                              float sw, float bias, const float *sx) {
-    const T *rp = (const T *)a.res + (long long)t0 * a.ldres + n;
-    T *yp = (T *)a.y + (long long)t0 * a.ldy + n;
-#pragma unroll
-    for (int j = 0; j < C; j++) {
-        if (n < a.N && t0 + j < a.M) {
-            float v = act_apply(__fmaf_rn((float)(int)acc[j], sx[j] * sw, bias), a.act);
-            if (a.res) v += to_float(rp[j * a.ldres]);
-            yp[j * a.ldy] = from_float<T>(v);
-        }
+    for (int j = 0; j < C; j++, yp += a.ldy) {
+        const T out = from_float<T>(RES ? v[j] + to_float(r[RES ? j : 0]) : v[j]);
+        if (!EDGE || j < mine) *yp = out;
     }
 }
 
-template <typename T, int C, bool RES>
+template <typename T, int C, bool RES, bool EDGE>
 __device__ __forceinline__ void epilogue_act(const Args &a, const uint32_t (&acc)[C], int t0, int n,
                                              float sw, float bias, const float *sx, int lane) {
     switch (a.act) {
-        case ACT_RELU: epilogue_full<T, C, ACT_RELU, RES>(a, acc, t0, n, sw, bias, sx, lane); break;
-        case ACT_SILU: epilogue_full<T, C, ACT_SILU, RES>(a, acc, t0, n, sw, bias, sx, lane); break;
-        case ACT_GELU: epilogue_full<T, C, ACT_GELU, RES>(a, acc, t0, n, sw, bias, sx, lane); break;
-        default: epilogue_full<T, C, ACT_NONE, RES>(a, acc, t0, n, sw, bias, sx, lane);
+        case ACT_RELU: epilogue_chunk<T, C, ACT_RELU, RES, EDGE>(a, acc, t0, n, sw, bias, sx, lane); break;
+        case ACT_SILU: epilogue_chunk<T, C, ACT_SILU, RES, EDGE>(a, acc, t0, n, sw, bias, sx, lane); break;
+        case ACT_GELU: epilogue_chunk<T, C, ACT_GELU, RES, EDGE>(a, acc, t0, n, sw, bias, sx, lane); break;
+        default: epilogue_chunk<T, C, ACT_NONE, RES, EDGE>(a, acc, t0, n, sw, bias, sx, lane);
     }
 }
 
 template <typename T, int C>
 __device__ __forceinline__ void epilogue_any(const Args &a, const uint32_t (&acc)[C], int t0, int n,
                                              float sw, float bias, const float *sx, int lane) {
-    if (t0 + C > a.M || n - lane + 32 > a.N)
-        epilogue_edge<T, C>(a, acc, t0, n, sw, bias, sx);
-    else if (a.res)
-        epilogue_act<T, C, true>(a, acc, t0, n, sw, bias, sx, lane);
-    else
-        epilogue_act<T, C, false>(a, acc, t0, n, sw, bias, sx, lane);
+    const bool edge = t0 + C > a.M || n - lane + 32 > a.N;
+    if (a.res) {
+        if (edge) epilogue_act<T, C, true, true>(a, acc, t0, n, sw, bias, sx, lane);
+        else epilogue_act<T, C, true, false>(a, acc, t0, n, sw, bias, sx, lane);
+    } else {
+        if (edge) epilogue_act<T, C, false, true>(a, acc, t0, n, sw, bias, sx, lane);
+        else epilogue_act<T, C, false, false>(a, acc, t0, n, sw, bias, sx, lane);
+    }
 }
 
 template <typename T, int BT, int FORM>
@@ -400,6 +438,10 @@ linear_i8_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
     if constexpr (FORM == PAIR) cluster_sync();  // the peer's barriers are set up
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
+    if (warp == kWarpTma && lane == 0) {
+        prefetch_tensor_map(&tmW);
+        prefetch_tensor_map(&tmQ);
+    }
     pdl_begin();
 
     const uint32_t rank = FORM == WHOLE ? 0 : cluster_rank();
@@ -524,7 +566,7 @@ linear_i8_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
             if (lane == 0) mbar_arrive(bar_sfull + 8 * ra.i);
         }
     } else if (warp >= kWarpEpi) {
-        constexpr int kPart = BT / (kEpiWarps / 4), C = kPart < 32 ? kPart : 32;
+        constexpr int kPart = BT / (kEpiWarps / 4), C = kPart < 16 ? kPart : 16;
         const int quad = warp & 3, part = (warp - kWarpEpi) >> 2;
         const uint32_t lane_base = (uint32_t)(quad * 32) << 16;
         Ring ra(kAcc);
@@ -648,8 +690,9 @@ Status launch(const LinearI8Args &p, Args a, int splits, cudaStream_t st) {
     }
     a.f_tiles = cdiv(p.N, FORM == PAIR ? 2 * kFeat : kFeat);
     a.t_tiles = cdiv(p.M, BT);
-    if ((long long)a.f_tiles * a.t_tiles > 0x0fffffff) return ERR_SHAPE;
+    if ((long long)a.f_tiles * a.t_tiles > 0x0fffffff || a.f_tiles > 0x0fffffff) return ERR_SHAPE;
     a.tiles = a.f_tiles * a.t_tiles;
+    a.group = FastDiv((uint32_t)(kGroup * a.f_tiles));
     a.kps = cdiv(a.kblocks, splits);
     // CTAs of a cluster, and clusters: one for each tile (split) or as many
     // as the SMs hold
@@ -673,6 +716,56 @@ Status launch(const LinearI8Args &p, Args a, int splits, cudaStream_t st) {
     return cuda_status();
 }
 
+// Which form and token tile.  A model of the time in us, from timings of all
+// forms over 26 sizes (M 1..13125, N and K 128..16384, 148 SMs), which it
+// meets to about 10 %: a launch with its set-up and last epilogue takes 2.9;
+// a k-block takes `step`, or what its CTAs' loads take from L2 (9 TB/s
+// together) when that is more; `tail` is what a tile's epilogue adds; a split
+// adds the cluster's exchange.  Some of the sizes, with the best form of each
+// kind (us; K x N = 4096 x 4096 where nothing else is said):
+//   M 1: split 16 by 4 8.0, by 8 8.6, whole 16 12.6;  M 64: split 64 by 4 9.3,
+//   whole 64 13.3;  M 256: whole 64 13.7, split 64 by 2 13.8;  M 1024: whole
+//   256 18.2, 128 26.8;  M 300, 256 x 256: whole 32 3.5, split 16 by 2 4.8;
+//   M 2400, 256 x 1024: whole 64 5.7, 128 6.4, 256 6.7.
+// Pairs against single CTAs at 256 tokens: 16384 x 1024 -> 4096 64.0 / 67.0,
+// 8192 cubed 410 / 422, 52500 x 256 -> 1536 66.6 / 65.8, 1024 x 4096 -> 4096
+// 21.0 / 18.4: pairs halve the token tile's traffic from L2, and pay where
+// the main loop is long and every SM has several tiles.
+struct Choice {
+    int form, bt, splits;
+};
+Choice choose(int M, int N, int kblocks) {
+    constexpr int kTokens[5] = {16, 32, 64, 128, 256};
+    constexpr float kStep[5] = {0.27f, 0.30f, 0.31f, 0.355f, 0.42f};
+    constexpr float kTail[5] = {0.1f, 0.28f, 0.34f, 1.03f, 2.9f};
+    const int sms = sm_count();
+    Choice best = {WHOLE, 256, 1};
+    float least = 1e30f;
+    for (int i = 0; i < 5; i++) {
+        const float tiles = (float)cdiv(N, kFeat) * (float)cdiv(M, kTokens[i]);
+        const float load = (float)stage_bytes(kTokens[i], WHOLE) / 9e6f;
+        for (int splits = 1; splits <= 8; splits *= 2) {
+            if (splits > 1 && (kTokens[i] > 64 || splits > kblocks)) break;
+            const float kb = (float)cdiv(kblocks, splits);
+            const float room = (float)(splits > 1 ? 2 * sms : sms);
+            const float ctas = tiles * (float)splits, at_once = fminf(ctas, room);
+            const float waves = ceilf(ctas / room);
+            const float t = 2.9f + (splits > 1 ? 1.2f + 0.15f * (float)splits : 0.0f) +
+                            waves * (kb * fmaxf(kStep[i], at_once * load) + kTail[i]);
+            if (t < least) {
+                least = t;
+                best = {splits > 1 ? SPLIT : WHOLE, kTokens[i], splits};
+            }
+        }
+    }
+    if (best.form == SPLIT)  // whole k-blocks, none of the CTAs left without one
+        best.splits = cdiv(kblocks, cdiv(kblocks, best.splits));
+    if (best.form == WHOLE && best.bt == 256 && kblocks >= 8 &&
+        (long long)cdiv(N, 2 * kFeat) * cdiv(M, 256) > sms / 2)
+        best.form = PAIR;
+    return best;
+}
+
 }  // namespace
 
 Status launch_linear_i8(const LinearI8Args &p, cudaStream_t st) {
@@ -686,30 +779,20 @@ Status launch_linear_i8(const LinearI8Args &p, cudaStream_t st) {
     a.y = (void *)p.y.p; a.ldy = p.y.ld;
     a.pairs = p.type != T_F32 && ((uintptr_t)a.y & 3) == 0 && (p.M == 1 || a.ldy % 2 == 0) &&
               (!a.res || (((uintptr_t)a.res & 3) == 0 && (p.M == 1 || a.ldres % 2 == 0)));
+    const Choice c = choose(p.M, p.N, a.kblocks);
     return with_type(p.type, [&](auto t) {
         using T = decltype(t);
-        const int sms = sm_count();
-        const long long f = cdiv(p.N, kFeat);
-        // few tiles: split K over clusters until two CTAs an SM are busy
-        const int bt = p.M <= 16 ? 16 : p.M <= 32 ? 32 : 64;
-        const long long tiles = f * cdiv(p.M, bt);
-        if (tiles < sms && a.kblocks > 1) {
-            int splits = (int)(2 * sms / tiles);
-            if (splits > 8) splits = 8;
-            if (splits > a.kblocks) splits = a.kblocks;
-            // whole k-blocks, none of the CTAs left without one
-            splits = cdiv(a.kblocks, cdiv(a.kblocks, splits));
-            if (splits > 1) {
-                if (bt == 16) return launch<T, 16, SPLIT>(p, a, splits, st);
-                if (bt == 32) return launch<T, 32, SPLIT>(p, a, splits, st);
-                return launch<T, 64, SPLIT>(p, a, splits, st);
-            }
+        switch (c.form * 1024 + c.bt) {
+            case PAIR * 1024 + 256: return launch<T, 256, PAIR>(p, a, 1, st);
+            case SPLIT * 1024 + 16: return launch<T, 16, SPLIT>(p, a, c.splits, st);
+            case SPLIT * 1024 + 32: return launch<T, 32, SPLIT>(p, a, c.splits, st);
+            case SPLIT * 1024 + 64: return launch<T, 64, SPLIT>(p, a, c.splits, st);
+            case WHOLE * 1024 + 16: return launch<T, 16, WHOLE>(p, a, 1, st);
+            case WHOLE * 1024 + 32: return launch<T, 32, WHOLE>(p, a, 1, st);
+            case WHOLE * 1024 + 64: return launch<T, 64, WHOLE>(p, a, 1, st);
+            case WHOLE * 1024 + 128: return launch<T, 128, WHOLE>(p, a, 1, st);
+            default: return launch<T, 256, WHOLE>(p, a, 1, st);
         }
-        if (getenv("LIN_PAIR") && f * cdiv(p.M, 256) >= sms) return launch<T, 256, PAIR>(p, a, 1, st);
-        if (f * cdiv(p.M, 256) >= sms) return launch<T, 256, WHOLE>(p, a, 1, st);
-        if (f * cdiv(p.M, 128) >= sms) return launch<T, 128, WHOLE>(p, a, 1, st);
-        if (p.M <= 16) return launch<T, 16, WHOLE>(p, a, 1, st);
-        return launch<T, 64, WHOLE>(p, a, 1, st);
     });
 }
 

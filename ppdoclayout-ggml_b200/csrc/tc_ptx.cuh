@@ -55,6 +55,10 @@ __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap *tm,
         "l"(reinterpret_cast<uint64_t>(tm)), "r"(bar), "r"(x), "r"(y)
         : "memory");
 }
+// a kernel parameter's tensor map into the descriptor cache
+__device__ __forceinline__ void prefetch_tensor_map(const CUtensorMap *tm) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(tm)) : "memory");
+}
 __device__ __forceinline__ uint64_t smem_desc(uint32_t saddr, uint32_t lbo, uint32_t sbo,
                                               uint32_t layout) {
     uint64_t d = (uint64_t)((saddr >> 4) & 0x3FFFu);
