@@ -300,7 +300,7 @@ PPDL_OPS_API int ppdl_layernorm(const void * x, long long ldx, const void * res,
    dweight and dbias [D] of w_type may be NULL; when either is given, work
    holds ppdl_layernorm_backward_workspace(rows, D) floats, 16-byte aligned,
    for this call alone.  The sums over rows run in an order that depends on
-   the sizes and the GPU's number of SMs alone.
+   the sizes and alignments alone: the same call gives the same bits.
    Returns PPDL_OK / PPDL_ERR_SHAPE / PPDL_ERR_CUDA. */
 PPDL_OPS_API int ppdl_layernorm_backward(const void * dy, long long lddy, const void * x,
                                          long long ldx, const void * weight, const float * mean,

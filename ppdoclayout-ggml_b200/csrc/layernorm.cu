@@ -14,6 +14,7 @@
 // mean, not a difference of moments, so a large common offset costs nothing.
 #include "block.cuh"
 #include "block.h"
+#include "rows.cuh"
 
 namespace ppdl {
 
@@ -24,8 +25,8 @@ __device__ __forceinline__ float weight_at(const WT *w, long long i, float none)
     return w ? to_float(w[i]) : none;
 }
 
-// One block per row, any width: the row is read once for the mean, once for
-// the variance and once for the output.
+// One block per row, any width (rows too wide for registers): read once for the
+// mean, and again, from L2, for the variance and for the output.
 template <typename T, typename WT>
 __global__ void layernorm_row_kernel(const T *x, long long ldx, const T *res, long long ldres, T *y,
                                      long long ldy, T *sum, long long ldsum, const WT *w,
@@ -57,6 +58,64 @@ __global__ void layernorm_row_kernel(const T *x, long long ldx, const T *res, lo
         y[i] = from_float<T>((v - mean) * rstd * weight_at(w, i, 1.0f) + weight_at(b, i, 0.0f));
     }
     if (threadIdx.x == 0) {
+        if (mean_out) mean_out[row] = mean;
+        if (rstd_out) rstd_out[row] = rstd;
+    }
+}
+
+// Rows in registers: TPR threads hold a row of at most TPR * NE values, a
+// block has as many rows as fit 128 threads (one, when TPR is more).  One pass
+// over memory.
+template <typename T, typename WT, int TPR, int NE, bool VEC>
+__global__ void __launch_bounds__(TPR < 128 ? 128 : TPR)
+layernorm_tile_kernel(const T *x, long long ldx, const T *res, long long ldres, T *y,
+                      long long ldy, T *sum, long long ldsum, const WT *w, const WT *b,
+                      float *mean_out, float *rstd_out, long long rows, int D, float eps) {
+    using Tile = RowTile<T, TPR, NE, VEC>;
+    pdl_begin();
+    __shared__ float sh[2][32];
+    constexpr int kRows = TPR < 128 ? 128 / TPR : 1;
+    const int lane = threadIdx.x % TPR;
+    long long row = (long long)blockIdx.x * kRows + threadIdx.x / TPR;
+    // rows past the end repeat the last one (its threads take part in the
+    // shuffles) and store nothing
+    const bool real = row < rows;
+    if (!real) row = rows - 1;
+    typename Tile::Raw r;
+    Tile::load(r, x + row * ldx, D, lane);
+    if (res) {
+        typename Tile::Raw q;
+        Tile::load(q, res + row * ldres, D, lane);
+#pragma unroll
+        for (int j = 0; j < NE; j++) r.v[j] = from_float<T>(to_float(r.v[j]) + to_float(q.v[j]));
+    }
+    float v[NE], s[1] = {0.0f};
+#pragma unroll
+    for (int j = 0; j < NE; j++) {
+        v[j] = to_float(r.v[j]);
+        s[0] += v[j];
+    }
+    row_sums<TPR>(s, sh[0]);
+    const float mean = s[0] / (float)D;
+    s[0] = 0.0f;
+#pragma unroll
+    for (int j = 0; j < NE; j++) {
+        v[j] -= mean;
+        if (Tile::inside(j, D, lane)) s[0] += v[j] * v[j];
+    }
+    row_sums<TPR>(s, sh[1]);
+    const float rstd = 1.0f / sqrtf(s[0] / (float)D + eps);
+    if (!real) return;
+    if (sum) Tile::store(sum + row * ldsum, r, D, lane);
+    float p[NE];
+    Tile::load_params(p, w, 1.0f, D, lane);
+#pragma unroll
+    for (int j = 0; j < NE; j++) v[j] = v[j] * rstd * p[j];
+    Tile::load_params(p, b, 0.0f, D, lane);
+#pragma unroll
+    for (int j = 0; j < NE; j++) r.v[j] = from_float<T>(v[j] + p[j]);
+    Tile::store(y + row * ldy, r, D, lane);
+    if (lane == 0) {
         if (mean_out) mean_out[row] = mean;
         if (rstd_out) rstd_out[row] = rstd;
     }
@@ -112,20 +171,137 @@ __global__ void layernorm_dw_column_kernel(const T *dy, long long lddy, const T 
     part[((long long)blockIdx.y * 2 + 1) * D + c] = sb;
 }
 
-// dw, db = the parts' sums, in part order
-template <typename WT>
-__global__ void layernorm_dw_sum_kernel(const float *part, int parts, int D, WT *dw, WT *db) {
+// The whole backward pass in one reading of dy and x: TPR threads hold a row
+// of at most TPR * NE values, a block of kThreads goes through rows
+// blockIdx.x * kRows, + gridDim.x * kRows, ... and keeps its share of the
+// weights' gradients in registers, column by column.  The next rows are
+// loaded while the present ones are summed.  part[block][2][D] takes the
+// block's sums (null: no weights' gradients).
+constexpr int bwd_threads(int tpr) { return tpr < 256 ? 256 : tpr; }
+template <typename T, typename WT, int TPR, int NE, bool VEC>
+__global__ void __launch_bounds__(bwd_threads(TPR), TPR > 512 ? 1 : TPR > 256 ? 2 : 3)
+layernorm_bwd_tile_kernel(const T *dy, long long lddy, const T *x, long long ldx, const T *dsum,
+                          long long lddsum, T *dx, long long lddx, const WT *w,
+                          const float *mean_in, const float *rstd_in, long long rows, int D,
+                          float *part) {
+    using Tile = RowTile<T, TPR, NE, VEC>;
+    constexpr int kThreads = bwd_threads(TPR), kRows = kThreads / TPR;
+    __shared__ float sh[2][kThreads / 32 * 2];
+    __shared__ float red[kRows > 1 ? kThreads * NE : 1];
     pdl_begin();
-    const int c = blockIdx.x * blockDim.x + threadIdx.x;
-    if (c >= D) return;
-    WT *out = blockIdx.y ? db : dw;
-    if (!out) return;
-    float s = 0.0f;
-    for (int p = 0; p < parts; p++) s += part[((long long)p * 2 + blockIdx.y) * D + c];
-    out[c] = from_float<WT>(s);
+    const int lane = threadIdx.x % TPR, group = threadIdx.x / TPR;
+    float p[NE], dw[NE], db[NE];
+    Tile::load_params(p, w, 1.0f, D, lane);
+#pragma unroll
+    for (int j = 0; j < NE; j++) dw[j] = db[j] = 0.0f;
+
+    typename Tile::Raw rx, rdy;
+    float mean = 0.0f, rstd = 0.0f;
+    // rows past the end repeat the last one with a zero gradient
+    auto load = [&](long long row) {
+        const long long at = min(row, rows - 1);
+        Tile::load(rx, x + at * ldx, D, lane);
+        Tile::load(rdy, dy + at * lddy, D, lane);
+        mean = mean_in[at];
+        rstd = rstd_in[at];
+    };
+    const long long step = (long long)gridDim.x * kRows;
+    long long row = (long long)blockIdx.x * kRows + group;
+    int parity = 0;
+    load(row);
+    for (long long base = (long long)blockIdx.x * kRows; base < rows;
+         base += step, row += step, parity ^= 1) {
+        const bool real = row < rows;
+        const float m = mean, r = rstd;
+        float xh[NE], g[NE];
+#pragma unroll
+        for (int j = 0; j < NE; j++) {
+            xh[j] = (to_float(rx.v[j]) - m) * r;
+            g[j] = real ? to_float(rdy.v[j]) : 0.0f;
+        }
+        if (base + step < rows) load(row + step);
+        float s[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int j = 0; j < NE; j++) {
+            // past D every g is zero (loaded as zero), and xh counts only with it
+            dw[j] += g[j] * xh[j];
+            db[j] += g[j];
+            g[j] *= p[j];
+            s[0] += g[j];
+            s[1] += g[j] * xh[j];
+        }
+        typename Tile::Raw out;
+        if (dsum && real) Tile::load(out, dsum + row * lddsum, D, lane);
+        row_sums<TPR>(s, sh[parity]);
+        const float m1 = s[0] / (float)D, m2 = s[1] / (float)D;
+        if (real) {
+#pragma unroll
+            for (int j = 0; j < NE; j++) {
+                float v = (g[j] - m1 - xh[j] * m2) * r;
+                if (dsum) v += to_float(out.v[j]);
+                out.v[j] = from_float<T>(v);
+            }
+            Tile::store(dx + row * lddx, out, D, lane);
+        }
+    }
+    if (!part) return;
+    part += (long long)blockIdx.x * 2 * D;
+    if constexpr (kRows == 1) {
+#pragma unroll
+        for (int j = 0; j < NE; j++) {
+            const int c = Tile::column(j / Tile::kVec, lane) + j % Tile::kVec;
+            if (c < D) {
+                part[c] = dw[j];
+                part[D + c] = db[j];
+            }
+        }
+    } else {
+        // the block's row groups, in order
+        for (int which = 0; which < 2; which++) {
+#pragma unroll
+            for (int j = 0; j < NE; j++)
+                red[(group * NE + j) * TPR + lane] = which ? db[j] : dw[j];
+            __syncthreads();
+            for (int t = threadIdx.x; t < TPR * NE; t += kThreads) {
+                const int j = t / TPR, l = t % TPR;
+                const int c = Tile::column(j / Tile::kVec, l) + j % Tile::kVec;
+                if (c < D) {
+                    float sum = 0.0f;
+                    for (int q = 0; q < kRows; q++) sum += red[q * NE * TPR + t];
+                    part[which * D + c] = sum;
+                }
+            }
+            __syncthreads();
+        }
+    }
 }
 
-constexpr int kMaxParts = 296;
+// dw (blockIdx.y 0) and db (1): the parts' sums, 32 columns a block, 8
+// threads a column, each every eighth part, then the 8 in order.
+template <typename WT>
+__global__ void __launch_bounds__(256) layernorm_dw_sum_kernel(const float *part, int parts, int D,
+                                                               WT *dw, WT *db) {
+    pdl_begin();
+    __shared__ float sh[8][32];
+    WT *out = blockIdx.y ? db : dw;
+    if (!out) return;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
+    float s = 0.0f;
+    if (c < D) {
+        const float *p = part + (long long)blockIdx.y * D + c;
+#pragma unroll 8
+        for (int q = warp; q < parts; q += 8) s += p[(long long)q * 2 * D];
+    }
+    sh[warp][lane] = s;
+    __syncthreads();
+    if (warp == 0 && c < D) {
+        for (int q = 1; q < 8; q++) s += sh[q][lane];
+        out[c] = from_float<WT>(s);
+    }
+}
+
+// blocks that keep column sums, at most: three on each of 148 SMs
+constexpr int kMaxParts = 444;
 int row_parts(long long rows) { return (int)(rows < kMaxParts ? rows : kMaxParts); }
 
 // f(T{}, WT{}) for the element types of rows and weights
@@ -148,8 +324,33 @@ Status launch_layernorm(const LayerNormArgs &a, cudaStream_t st) {
     return with_types(a.type, a.w_type, [&](auto t, auto wt) {
         using T = decltype(t);
         using WT = decltype(wt);
-        const int threads = a.D >= 1024 ? 256 : 128;
-        pdl_launch(layernorm_row_kernel<T, WT>, (unsigned)a.rows, threads, 0, st,
+        const int size = (int)sizeof(T);
+        const bool vec = vector_rows(a.x.p, a.x.ld, a.rows, a.D, size) &&
+                         vector_rows(a.res.p, a.res.ld, a.rows, a.D, size) &&
+                         vector_rows(a.y.p, a.y.ld, a.rows, a.D, size) &&
+                         vector_rows(a.sum.p, a.sum.ld, a.rows, a.D, size);
+        auto tile = [&](auto tpr, auto ne) {
+            constexpr int TPR = decltype(tpr)::value, NE = decltype(ne)::value;
+            constexpr int kThreads = TPR < 128 ? 128 : TPR;
+            auto kernel = vec ? layernorm_tile_kernel<T, WT, TPR, NE, true>
+                              : layernorm_tile_kernel<T, WT, TPR, NE, false>;
+            pdl_launch(kernel, (unsigned)cdiv(a.rows, kThreads / TPR), kThreads, 0, st,
+                       (const T *)a.x.p, a.x.ld, (const T *)a.res.p, a.res.ld, ptr<T>(a.y), a.y.ld,
+                       ptr<T>(a.sum), a.sum.ld, (const WT *)a.weight, (const WT *)a.bias, a.mean,
+                       a.rstd, a.rows, a.D, a.eps);
+            return cuda_status();
+        };
+        // the smallest tile that holds the row; 16-bit threads take one to
+        // four vectors of 8, FP32 ones of 4
+        if (a.D <= 64) return tile(Int<8>{}, Int<8>{});
+        if (a.D <= 256) return tile(Int<32>{}, Int<8>{});
+        if (a.D <= 512) return tile(Int<32>{}, Int<16>{});
+        if (a.D <= 1024) return tile(Int<32>{}, Int<32>{});
+        if (a.D <= 2048) return tile(Int<128>{}, Int<16>{});
+        if (a.D <= 4096) return tile(Int<256>{}, Int<16>{});
+        if (a.D <= 8192) return tile(Int<512>{}, Int<16>{});
+        if (a.D <= 16384) return tile(Int<1024>{}, Int<16>{});
+        pdl_launch(layernorm_row_kernel<T, WT>, (unsigned)a.rows, 512, 0, st,
                    (const T *)a.x.p, a.x.ld, (const T *)a.res.p, a.res.ld, ptr<T>(a.y), a.y.ld,
                    ptr<T>(a.sum), a.sum.ld, (const WT *)a.weight, (const WT *)a.bias, a.mean,
                    a.rstd, a.D, a.eps);
@@ -168,21 +369,56 @@ Status launch_layernorm_backward(const LayerNormBackwardArgs &a, cudaStream_t st
     return with_types(a.type, a.w_type, [&](auto t, auto wt) {
         using T = decltype(t);
         using WT = decltype(wt);
+        const int size = (int)sizeof(T);
+        const bool vec = vector_rows(a.dy.p, a.dy.ld, a.rows, a.D, size) &&
+                         vector_rows(a.x.p, a.x.ld, a.rows, a.D, size) &&
+                         vector_rows(a.dx.p, a.dx.ld, a.rows, a.D, size) &&
+                         vector_rows(a.dsum.p, a.dsum.ld, a.rows, a.D, size);
+        const bool grads = a.dweight || a.dbias;
         int parts = 0;
-        if (a.rows > 0) {
-            pdl_launch(layernorm_dx_row_kernel<T, WT>, (unsigned)a.rows, a.D >= 1024 ? 256 : 128, 0,
-                       st, (const T *)a.dy.p, a.dy.ld, (const T *)a.x.p, a.x.ld,
+        auto tile = [&](auto tpr, auto ne) {
+            constexpr int TPR = decltype(tpr)::value, NE = decltype(ne)::value;
+            constexpr int kThreads = bwd_threads(TPR), kRows = kThreads / TPR;
+            auto kernel = vec ? layernorm_bwd_tile_kernel<T, WT, TPR, NE, true>
+                              : layernorm_bwd_tile_kernel<T, WT, TPR, NE, false>;
+            const int most = TPR > 512 ? 148 : TPR > 256 ? 296 : kMaxParts;
+            const long long blocks = (a.rows + kRows - 1) / kRows;
+            parts = (int)(blocks < most ? blocks : most);
+            pdl_launch(kernel, (unsigned)parts, kThreads, 0, st, (const T *)a.dy.p, a.dy.ld,
+                       (const T *)a.x.p, a.x.ld, (const T *)a.dsum.p, a.dsum.ld, ptr<T>(a.dx),
+                       a.dx.ld, (const WT *)a.weight, a.mean, a.rstd, a.rows, a.D,
+                       grads ? a.work : nullptr);
+        };
+        if (a.rows == 0) {
+        } else if (a.D <= 64) {
+            tile(Int<8>{}, Int<8>{});
+        } else if (a.D <= 256) {
+            tile(Int<32>{}, Int<8>{});
+        } else if (a.D <= 512) {
+            tile(Int<64>{}, Int<8>{});
+        } else if (a.D <= 1024) {
+            tile(Int<128>{}, Int<8>{});
+        } else if (a.D <= 2048) {
+            tile(Int<256>{}, Int<8>{});
+        } else if (a.D <= 4096) {
+            tile(Int<512>{}, Int<8>{});
+        } else if (a.D <= 8192) {
+            tile(Int<1024>{}, Int<8>{});
+        } else {
+            pdl_launch(layernorm_dx_row_kernel<T, WT>, (unsigned)a.rows, 512, 0, st,
+                       (const T *)a.dy.p, a.dy.ld, (const T *)a.x.p, a.x.ld,
                        (const T *)a.dsum.p, a.dsum.ld, ptr<T>(a.dx), a.dx.ld, (const WT *)a.weight,
                        a.mean, a.rstd, a.D);
-            if (!a.dweight && !a.dbias) return cuda_status();
-            const long long chunk = (a.rows + row_parts(a.rows) - 1) / row_parts(a.rows);
-            parts = (int)((a.rows + chunk - 1) / chunk);
-            pdl_launch(layernorm_dw_column_kernel<T>, dim3(cdiv(a.D, 128), parts), 128, 0, st,
-                       (const T *)a.dy.p, a.dy.ld, (const T *)a.x.p, a.x.ld, a.mean, a.rstd, a.rows,
-                       a.D, chunk, a.work);
+            if (grads) {
+                const long long chunk = (a.rows + row_parts(a.rows) - 1) / row_parts(a.rows);
+                parts = (int)((a.rows + chunk - 1) / chunk);
+                pdl_launch(layernorm_dw_column_kernel<T>, dim3(cdiv(a.D, 128), parts), 128, 0, st,
+                           (const T *)a.dy.p, a.dy.ld, (const T *)a.x.p, a.x.ld, a.mean, a.rstd,
+                           a.rows, a.D, chunk, a.work);
+            }
         }
-        if (a.dweight || a.dbias)
-            pdl_launch(layernorm_dw_sum_kernel<WT>, dim3(cdiv(a.D, 128), 2), 128, 0, st, a.work,
+        if (grads)
+            pdl_launch(layernorm_dw_sum_kernel<WT>, dim3(cdiv(a.D, 32), 2), 256, 0, st, a.work,
                        parts, a.D, (WT *)a.dweight, (WT *)a.dbias);
         return cuda_status();
     });

@@ -2,6 +2,7 @@
 // q = x / scale rounded half to even on the exact quotient.
 #include "block.cuh"
 #include "block.h"
+#include "rows.cuh"
 
 namespace ppdl {
 
@@ -21,12 +22,90 @@ __device__ __forceinline__ int quantize(float x, float s, float inv) {
     return (int)fminf(fmaxf(q, -127.0f), 127.0f);
 }
 
-// One block per row: the largest |x| (as the bits of |x|, whose unsigned
-// order puts infinities and NaNs on top), then the quotients.  Scales below
+// What a row is divided by: its scale from the largest |x| (as the bits of
+// |x|, whose unsigned order puts infinities and NaNs on top).  Scales below
 // 2^-64 quantise x 2^64 by s 2^64, both exact, so that 1 / s is finite.
+struct Divisor {
+    float s, su, up, inv;
+    bool usable;
+    __device__ explicit Divisor(unsigned amax) {
+        s = __fdiv_rn(__uint_as_float(amax), 127.0f);
+        usable = s > 0.0f && amax < 0x7f800000u;
+        up = s < 0x1p-64f ? 0x1p64f : 1.0f;
+        su = s * up;
+        inv = usable ? __frcp_rn(su) : 0.0f;
+    }
+    __device__ __forceinline__ int operator()(float x) const {
+        return usable ? quantize(x * up, su, inv) : 0;
+    }
+};
+
+template <int TPR>
+__device__ __forceinline__ unsigned row_max(unsigned m, unsigned *sh) {
+    constexpr int kWidth = TPR < 32 ? TPR : 32;
+#pragma unroll
+    for (int o = kWidth / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if constexpr (TPR > 32) {
+        if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = m;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < TPR / 32; w++) m = max(m, sh[w]);
+    }
+    return m;
+}
+
+// Rows in registers, as layernorm_tile_kernel; a thread's neighbouring
+// values leave as one store of 4 or 8 bytes.
+template <typename T, int TPR, int NE, bool VEC>
+__global__ void __launch_bounds__(TPR < 128 ? 128 : TPR)
+quantize_tile_kernel(const T *x, long long ldx, long long rows, int K, int8_t *q, long long ldq,
+                     float *scale) {
+    using Tile = RowTile<T, TPR, NE, VEC, 4>;
+    pdl_begin();
+    __shared__ unsigned sh[32];
+    constexpr int kRows = TPR < 128 ? 128 / TPR : 1;
+    const int lane = threadIdx.x % TPR;
+    long long row = (long long)blockIdx.x * kRows + threadIdx.x / TPR;
+    const bool real = row < rows;
+    if (!real) row = rows - 1;
+    typename Tile::Raw r;
+    Tile::load(r, x + row * ldx, K, lane);
+    unsigned m = 0;
+#pragma unroll
+    for (int j = 0; j < NE; j++) m = max(m, __float_as_uint(fabsf(to_float(r.v[j]))));
+    const Divisor d(row_max<TPR>(m, sh));
+    if (!real) return;
+    if (lane == 0) scale[row] = d.s;
+    q += row * ldq;
+#pragma unroll
+    for (int i = 0; i < Tile::kVecs; i++) {
+        const int c = Tile::column(i, lane);
+        unsigned w[Tile::kVec / 4];
+#pragma unroll
+        for (int h = 0; h < Tile::kVec / 4; h++) {
+            w[h] = 0;
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                w[h] |= (unsigned)(d(to_float(r.v[i * Tile::kVec + 4 * h + e])) & 255) << (8 * e);
+        }
+        if (c + Tile::kVec <= K) {
+            if constexpr (Tile::kVec == 8)
+                *reinterpret_cast<uint2 *>(q + c) = make_uint2(w[0], w[1]);
+            else
+                *reinterpret_cast<unsigned *>(q + c) = w[0];
+        } else {
+#pragma unroll
+            for (int e = 0; e < Tile::kVec; e++)
+                if (c + e < K) q[c + e] = (int8_t)(w[e / 4] >> (8 * (e % 4)));
+        }
+    }
+}
+
+// One block per row, any width (rows too wide for registers): read once for
+// the scale and again, from L2, for the quotients.
 template <typename T>
-__global__ void quantize_rows_kernel(const T *x, long long ldx, int K, int8_t *q, long long ldq,
-                                     float *scale) {
+__global__ void quantize_row_kernel(const T *x, long long ldx, int K, int8_t *q, long long ldq,
+                                    float *scale) {
     pdl_begin();
     __shared__ unsigned sh[32];
     const long long row = blockIdx.x;
@@ -35,18 +114,9 @@ __global__ void quantize_rows_kernel(const T *x, long long ldx, int K, int8_t *q
     unsigned m = 0;
     for (int i = threadIdx.x; i < K; i += blockDim.x)
         m = max(m, __float_as_uint(fabsf(to_float(x[i]))));
-    m = __reduce_max_sync(0xffffffffu, m);
-    if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = m;
-    __syncthreads();
-    m = 0;
-    for (int i = 0; i < (int)(blockDim.x >> 5); i++) m = max(m, sh[i]);
-    const float s = __fdiv_rn(__uint_as_float(m), 127.0f);
-    if (threadIdx.x == 0) scale[row] = s;
-    const bool usable = s > 0.0f && m < 0x7f800000u;
-    const float up = s < 0x1p-64f ? 0x1p64f : 1.0f;
-    const float su = s * up, inv = usable ? __frcp_rn(su) : 0.0f;
-    for (int i = threadIdx.x; i < K; i += blockDim.x)
-        q[i] = usable ? (int8_t)quantize(to_float(x[i]) * up, su, inv) : (int8_t)0;
+    const Divisor d(row_max<512>(m, sh));
+    if (threadIdx.x == 0) scale[row] = d.s;
+    for (int i = threadIdx.x; i < K; i += blockDim.x) q[i] = (int8_t)d(to_float(x[i]));
 }
 
 }  // namespace
@@ -57,8 +127,26 @@ Status launch_quantize_rows(const Rows &x, int type, long long rows, int K, int8
     if (rows < 0 || rows > 0x7fffffffLL || K <= 0) return ERR_SHAPE;
     return with_type(type, [&](auto t) {
         using T = decltype(t);
-        pdl_launch(quantize_rows_kernel<T>, (unsigned)rows, K >= 1024 ? 256 : 128, 0, st,
-                   (const T *)x.p, x.ld, K, q, ldq, scale);
+        const bool vec = vector_rows(x.p, x.ld, rows, K, (int)sizeof(T));
+        auto tile = [&](auto tpr, auto ne) {
+            constexpr int TPR = decltype(tpr)::value, NE = decltype(ne)::value;
+            constexpr int kThreads = TPR < 128 ? 128 : TPR;
+            auto kernel = vec ? quantize_tile_kernel<T, TPR, NE, true>
+                              : quantize_tile_kernel<T, TPR, NE, false>;
+            pdl_launch(kernel, (unsigned)cdiv(rows, kThreads / TPR), kThreads, 0, st,
+                       (const T *)x.p, x.ld, rows, K, q, ldq, scale);
+            return cuda_status();
+        };
+        if (K <= 64) return tile(Int<8>{}, Int<8>{});
+        if (K <= 256) return tile(Int<32>{}, Int<8>{});
+        if (K <= 512) return tile(Int<32>{}, Int<16>{});
+        if (K <= 1024) return tile(Int<32>{}, Int<32>{});
+        if (K <= 2048) return tile(Int<128>{}, Int<16>{});
+        if (K <= 4096) return tile(Int<256>{}, Int<16>{});
+        if (K <= 8192) return tile(Int<512>{}, Int<16>{});
+        if (K <= 16384) return tile(Int<1024>{}, Int<16>{});
+        pdl_launch(quantize_row_kernel<T>, (unsigned)rows, 512, 0, st, (const T *)x.p, x.ld, K, q,
+                   ldq, scale);
         return cuda_status();
     });
 }
