@@ -40,6 +40,8 @@ struct LayerNormBackwardArgs {
 };
 Status launch_layernorm_backward(const LayerNormBackwardArgs &a, cudaStream_t st);
 long long layernorm_backward_work(long long rows, int D);
+// the backward pass' device error flag, as tc_error_fetch_and_clear()
+int row_error_fetch_and_clear();
 
 // q[m][k] = x[m][k] / scale[m] rounded half to even, scale[m] = amax / 127
 Status launch_quantize_rows(const Rows &x, int type, long long rows, int K, int8_t *q,

@@ -15,6 +15,7 @@
 #include "block.cuh"
 #include "block.h"
 #include "rows.cuh"
+#include "tc_ptx.cuh"
 
 namespace ppdl {
 
@@ -73,6 +74,7 @@ layernorm_tile_kernel(const T *x, long long ldx, const T *res, long long ldres, 
                       float *mean_out, float *rstd_out, long long rows, int D, float eps) {
     using Tile = RowTile<T, TPR, NE, VEC>;
     pdl_begin();
+    pdl_trigger();
     __shared__ float sh[2][32];
     constexpr int kRows = TPR < 128 ? 128 / TPR : 1;
     const int lane = threadIdx.x % TPR;
@@ -118,6 +120,82 @@ layernorm_tile_kernel(const T *x, long long ldx, const T *res, long long ldres, 
     if (lane == 0) {
         if (mean_out) mean_out[row] = mean;
         if (rstd_out) rstd_out[row] = rstd;
+    }
+}
+
+__device__ int g_row_error = 0;
+
+// Persistent blocks with the rows coming through a ring in shared memory
+// (RowRing), weights and biases in registers: for many rows of whole 16-byte
+// vectors.
+constexpr int ring_threads(int tpr) { return tpr < 256 ? 256 : tpr; }
+constexpr int ring_blocks(int tpr) { return tpr > 256 ? 1 : 2; }
+template <typename T, typename WT, int TPR, int NE>
+__global__ void __launch_bounds__(ring_threads(TPR), ring_blocks(TPR))
+layernorm_ring_kernel(const T *x, long long ldx, const T *res, long long ldres, T *y,
+                      long long ldy, T *sum, long long ldsum, const WT *w, const WT *b,
+                      float *mean_out, float *rstd_out, long long rows, int D, float eps,
+                      int stages) {
+    using Tile = RowTile<T, TPR, NE, true>;
+    constexpr int kThreads = ring_threads(TPR);
+    using Rows = RowRing<T, TPR, kThreads, 2>;
+    extern __shared__ __align__(16) uint8_t ring_smem[];
+    __shared__ uint64_t bars[Rows::kTeams * kRingStages];
+    __shared__ float sh[2][kThreads / 32];
+    __shared__ int abort_word;
+    const int lane = threadIdx.x % TPR, team = threadIdx.x / Rows::kTeam;
+    const int sub = threadIdx.x % Rows::kTeam / TPR;
+    Rows ring;
+    ring.src[0] = x; ring.src[1] = res;
+    ring.ld[0] = ldx; ring.ld[1] = ldres;
+    ring.setup(ring_smem, bars, &abort_word, &g_row_error, rows, D, stages);
+    pdl_begin();
+    pdl_trigger();
+    ring.start();
+    float pw[NE], pb[NE];
+    Tile::load_params(pw, w, 1.0f, D, lane);
+    Tile::load_params(pb, b, 0.0f, D, lane);
+    const float inv_d = 1.0f / (float)D;
+    for (long long r0 = ring.first; r0 < rows; r0 += ring.step, ring.at.next()) {
+        const long long row = r0 + sub;
+        ring.wait();
+        typename Tile::Raw r;
+        Tile::load(r, ring.row(0), D, lane);
+        if (res) {
+            typename Tile::Raw q;
+            Tile::load(q, ring.row(1), D, lane);
+#pragma unroll
+            for (int j = 0; j < NE; j++) r.v[j] = from_float<T>(to_float(r.v[j]) + to_float(q.v[j]));
+        }
+        float v[NE], s[1] = {0.0f};
+#pragma unroll
+        for (int j = 0; j < NE; j++) {
+            v[j] = to_float(r.v[j]);
+            s[0] += v[j];
+        }
+        team_sums<TPR>(s, sh[0], team);
+        if constexpr (TPR <= 32) __syncwarp();
+        ring.refill(r0);
+        const float mean = s[0] * inv_d;
+        s[0] = 0.0f;
+#pragma unroll
+        for (int j = 0; j < NE; j++) {
+            v[j] -= mean;
+            if (Tile::inside(j, D, lane)) s[0] += v[j] * v[j];
+        }
+        team_sums<TPR>(s, sh[1], team);
+        const float rstd = 1.0f / sqrtf(s[0] * inv_d + eps);
+        if (row < rows && ring.good) {
+            if (sum) Tile::store(sum + row * ldsum, r, D, lane);
+#pragma unroll
+            for (int j = 0; j < NE; j++)
+                r.v[j] = from_float<T>(__fmaf_rn(v[j] * rstd, pw[j], pb[j]));
+            Tile::store(y + row * ldy, r, D, lane);
+            if (lane == 0) {
+                if (mean_out) mean_out[row] = mean;
+                if (rstd_out) rstd_out[row] = rstd;
+            }
+        }
     }
 }
 
@@ -179,7 +257,7 @@ __global__ void layernorm_dw_column_kernel(const T *dy, long long lddy, const T 
 // block's sums (null: no weights' gradients).
 constexpr int bwd_threads(int tpr) { return tpr < 256 ? 256 : tpr; }
 template <typename T, typename WT, int TPR, int NE, bool VEC>
-__global__ void __launch_bounds__(bwd_threads(TPR), TPR > 512 ? 1 : TPR > 256 ? 2 : 3)
+__global__ void __launch_bounds__(bwd_threads(TPR), TPR > 256 ? 1 : 2)
 layernorm_bwd_tile_kernel(const T *dy, long long lddy, const T *x, long long ldx, const T *dsum,
                           long long lddsum, T *dx, long long lddx, const WT *w,
                           const float *mean_in, const float *rstd_in, long long rows, int D,
@@ -189,6 +267,7 @@ layernorm_bwd_tile_kernel(const T *dy, long long lddy, const T *x, long long ldx
     __shared__ float sh[2][kThreads / 32 * 2];
     __shared__ float red[kRows > 1 ? kThreads * NE : 1];
     pdl_begin();
+    pdl_trigger();
     const int lane = threadIdx.x % TPR, group = threadIdx.x / TPR;
     float p[NE], dw[NE], db[NE];
     Tile::load_params(p, w, 1.0f, D, lane);
@@ -276,12 +355,127 @@ layernorm_bwd_tile_kernel(const T *dy, long long lddy, const T *x, long long ldx
     }
 }
 
+// The same with the rows coming through a ring in shared memory (RowRing).
+template <typename T, typename WT, int TPR, int NE>
+__global__ void __launch_bounds__(ring_threads(TPR), ring_blocks(TPR))
+layernorm_bwd_ring_kernel(const T *dy, long long lddy, const T *x, long long ldx, const T *dsum,
+                          long long lddsum, T *dx, long long lddx, const WT *w,
+                          const float *mean_in, const float *rstd_in, long long rows, int D,
+                          float *part, int stages) {
+    using Tile = RowTile<T, TPR, NE, true>;
+    constexpr int kThreads = ring_threads(TPR);
+    using Rows = RowRing<T, TPR, kThreads, 3>;
+    constexpr int kRows = Rows::kRows;
+    extern __shared__ __align__(16) uint8_t ring_smem[];
+    __shared__ uint64_t bars[Rows::kTeams * kRingStages];
+    __shared__ float sh[2][kThreads / 32 * 2];
+    __shared__ int abort_word;
+    const int lane = threadIdx.x % TPR, team = threadIdx.x / Rows::kTeam;
+    const int sub = threadIdx.x % Rows::kTeam / TPR;
+    Rows ring;
+    ring.src[0] = x; ring.src[1] = dy; ring.src[2] = dsum;
+    ring.ld[0] = ldx; ring.ld[1] = lddy; ring.ld[2] = lddsum;
+    ring.setup(ring_smem, bars, &abort_word, &g_row_error, rows, D, stages);
+    pdl_begin();
+    pdl_trigger();
+    ring.start();
+
+    float p[NE], dw[NE], db[NE];
+    Tile::load_params(p, w, 1.0f, D, lane);
+#pragma unroll
+    for (int j = 0; j < NE; j++) dw[j] = db[j] = 0.0f;
+    float mean = 0.0f, rstd = 0.0f;
+    if (ring.first + sub < rows) {
+        mean = mean_in[ring.first + sub];
+        rstd = rstd_in[ring.first + sub];
+    }
+    const float inv_d = 1.0f / (float)D;
+    int parity = 0;
+    for (long long r0 = ring.first; r0 < rows; r0 += ring.step, ring.at.next(), parity ^= 1) {
+        const long long row = r0 + sub;
+        const bool real = row < rows;
+        ring.wait();
+        typename Tile::Raw rx, rdy, out;
+        Tile::load(rx, ring.row(0), D, lane);
+        Tile::load(rdy, ring.row(1), D, lane);
+        if (dsum) Tile::load(out, ring.row(2), D, lane);
+        const float r = rstd, mr = -mean * rstd;
+        if (row + ring.step < rows) {
+            mean = mean_in[row + ring.step];
+            rstd = rstd_in[row + ring.step];
+        }
+        float xh[NE], g[NE], s[2] = {0.0f, 0.0f};
+        if (!real) {
+            // past the end: whatever the buffer held, and no gradient
+#pragma unroll
+            for (int j = 0; j < NE; j++) rx.v[j] = rdy.v[j] = from_float<T>(0.0f);
+        }
+#pragma unroll
+        for (int j = 0; j < NE; j++) {
+            // x r - mean r: off by the rounding of mean r, u |mean| r
+            xh[j] = __fmaf_rn(to_float(rx.v[j]), r, mr);
+            g[j] = to_float(rdy.v[j]);
+            dw[j] += g[j] * xh[j];
+            db[j] += g[j];
+            g[j] *= p[j];
+            s[0] += g[j];
+            s[1] += g[j] * xh[j];
+        }
+        team_sums<TPR>(s, sh[parity], team);
+        if constexpr (TPR <= 32) __syncwarp();
+        ring.refill(r0);
+        const float m1 = s[0] * inv_d * r, m2 = s[1] * inv_d * r;
+        if (real && ring.good) {
+#pragma unroll
+            for (int j = 0; j < NE; j++) {
+                float v = __fmaf_rn(g[j], r, -__fmaf_rn(xh[j], m2, m1));
+                if (dsum) v += to_float(out.v[j]);
+                out.v[j] = from_float<T>(v);
+            }
+            Tile::store(dx + row * lddx, out, D, lane);
+        }
+    }
+    if (!part) return;
+    part += (long long)blockIdx.x * 2 * D;
+    if constexpr (kRows == 1) {
+#pragma unroll
+        for (int j = 0; j < NE; j++) {
+            const int c = Tile::column(j / Tile::kVec, lane) + j % Tile::kVec;
+            if (c < D) {
+                part[c] = dw[j];
+                part[D + c] = db[j];
+            }
+        }
+    } else {
+        // the block's rows' sums in order, through the ring (all copies landed)
+        float *red = reinterpret_cast<float *>(ring_smem);
+        const int group = threadIdx.x / TPR;
+        for (int which = 0; which < 2; which++) {
+            __syncthreads();
+#pragma unroll
+            for (int j = 0; j < NE; j++)
+                red[(group * NE + j) * TPR + lane] = which ? db[j] : dw[j];
+            __syncthreads();
+            for (int t = threadIdx.x; t < TPR * NE; t += kThreads) {
+                const int j = t / TPR, l = t % TPR;
+                const int c = Tile::column(j / Tile::kVec, l) + j % Tile::kVec;
+                if (c < D) {
+                    float sum = 0.0f;
+                    for (int q = 0; q < kRows; q++) sum += red[q * NE * TPR + t];
+                    part[which * D + c] = sum;
+                }
+            }
+        }
+    }
+}
+
 // dw (blockIdx.y 0) and db (1): the parts' sums, 32 columns a block, 8
 // threads a column, each every eighth part, then the 8 in order.
 template <typename WT>
 __global__ void __launch_bounds__(256) layernorm_dw_sum_kernel(const float *part, int parts, int D,
                                                                WT *dw, WT *db) {
     pdl_begin();
+    pdl_trigger();
     __shared__ float sh[8][32];
     WT *out = blockIdx.y ? db : dw;
     if (!out) return;
@@ -300,8 +494,8 @@ __global__ void __launch_bounds__(256) layernorm_dw_sum_kernel(const float *part
     }
 }
 
-// blocks that keep column sums, at most: three on each of 148 SMs
-constexpr int kMaxParts = 444;
+// blocks that keep column sums, at most: two on each of 148 SMs
+constexpr int kMaxParts = 296;
 int row_parts(long long rows) { return (int)(rows < kMaxParts ? rows : kMaxParts); }
 
 // f(T{}, WT{}) for the element types of rows and weights
@@ -313,10 +507,20 @@ Status with_types(int type, int w_type, F f) {
     });
 }
 
+// shared memory of a block's ring: its share of an SM's
+constexpr int ring_bytes(int tpr) { return 216 * 1024 / ring_blocks(tpr) - 4096; }
+
 template <typename T>
 T *ptr(const Rows &r) { return (T *)r.p; }
 
 }  // namespace
+
+int row_error_fetch_and_clear() {
+    int h = 0, zero = 0;
+    cudaMemcpyFromSymbol(&h, g_row_error, sizeof(int));
+    if (h) cudaMemcpyToSymbol(g_row_error, &zero, sizeof(int));
+    return h;
+}
 
 Status launch_layernorm(const LayerNormArgs &a, cudaStream_t st) {
     if (a.rows == 0) return OK;
@@ -340,16 +544,46 @@ Status launch_layernorm(const LayerNormArgs &a, cudaStream_t st) {
                        a.rstd, a.rows, a.D, a.eps);
             return cuda_status();
         };
-        // the smallest tile that holds the row; 16-bit threads take one to
-        // four vectors of 8, FP32 ones of 4
-        if (a.D <= 64) return tile(Int<8>{}, Int<8>{});
-        if (a.D <= 256) return tile(Int<32>{}, Int<8>{});
-        if (a.D <= 512) return tile(Int<32>{}, Int<16>{});
-        if (a.D <= 1024) return tile(Int<32>{}, Int<32>{});
-        if (a.D <= 2048) return tile(Int<128>{}, Int<16>{});
-        if (a.D <= 4096) return tile(Int<256>{}, Int<16>{});
-        if (a.D <= 8192) return tile(Int<512>{}, Int<16>{});
-        if (a.D <= 16384) return tile(Int<1024>{}, Int<16>{});
+        auto ring = [&](auto tpr, auto ne) {
+            constexpr int TPR = decltype(tpr)::value, NE = decltype(ne)::value;
+            constexpr int kThreads = ring_threads(TPR), kRows = kThreads / TPR;
+            constexpr int kMost = 148 * ring_blocks(TPR);
+            auto kernel = layernorm_ring_kernel<T, WT, TPR, NE>;
+            const int stages = ring_stages(ring_bytes(TPR), a.res.p ? 2 : 1, kRows, a.D, size);
+            const long long blocks = (a.rows + kRows - 1) / kRows;
+            if (blocks < 3 * kMost || stages < 2 ||
+                !smem_attr_once((const void *)kernel, ring_bytes(TPR)))
+                return false;
+            pdl_launch(kernel, (unsigned)kMost, kThreads,
+                       (size_t)(stages * (a.res.p ? 2 : 1) * kRows * a.D * size), st,
+                       (const T *)a.x.p, a.x.ld, (const T *)a.res.p, a.res.ld, ptr<T>(a.y), a.y.ld,
+                       ptr<T>(a.sum), a.sum.ld, (const WT *)a.weight, (const WT *)a.bias, a.mean,
+                       a.rstd, a.rows, a.D, a.eps, stages);
+            return true;
+        };
+        if (vec) {
+            bool done = false;
+            if (a.D <= 64) done = ring(Int<4>{}, Int<16>{});
+            else if (a.D <= 128) done = ring(Int<8>{}, Int<16>{});
+            else if (a.D <= 256) done = ring(Int<16>{}, Int<16>{});
+            else if (a.D <= 512) done = ring(Int<32>{}, Int<16>{});
+            else if (a.D <= 1024) done = ring(Int<64>{}, Int<16>{});
+            else if (a.D <= 2048) done = ring(Int<128>{}, Int<16>{});
+            else if (a.D <= 4096) done = ring(Int<256>{}, Int<16>{});
+            else if (a.D <= 8192) done = ring(Int<512>{}, Int<16>{});
+            else if (a.D <= 16384) done = ring(Int<1024>{}, Int<16>{});
+            if (done) return cuda_status();
+        }
+        // the smallest tile that holds the row, 64 bytes a thread
+        constexpr int NE = sizeof(T) == 2 ? 32 : 16, F = sizeof(T) == 2 ? 1 : 2;
+        if (a.D <= 64) return tile(Int<4>{}, Int<16>{});
+        if (a.D <= 256) return tile(Int<16>{}, Int<16>{});
+        if (a.D <= 512) return tile(Int<16 * F>{}, Int<NE>{});
+        if (a.D <= 1024) return tile(Int<32 * F>{}, Int<NE>{});
+        if (a.D <= 2048) return tile(Int<64 * F>{}, Int<NE>{});
+        if (a.D <= 4096) return tile(Int<128 * F>{}, Int<NE>{});
+        if (a.D <= 8192) return tile(Int<256 * F>{}, Int<NE>{});
+        if (a.D <= 16384) return tile(Int<512 * F>{}, Int<NE>{});
         pdl_launch(layernorm_row_kernel<T, WT>, (unsigned)a.rows, 512, 0, st,
                    (const T *)a.x.p, a.x.ld, (const T *)a.res.p, a.res.ld, ptr<T>(a.y), a.y.ld,
                    ptr<T>(a.sum), a.sum.ld, (const WT *)a.weight, (const WT *)a.bias, a.mean,
@@ -379,9 +613,8 @@ Status launch_layernorm_backward(const LayerNormBackwardArgs &a, cudaStream_t st
         auto tile = [&](auto tpr, auto ne) {
             constexpr int TPR = decltype(tpr)::value, NE = decltype(ne)::value;
             constexpr int kThreads = bwd_threads(TPR), kRows = kThreads / TPR;
-            auto kernel = vec ? layernorm_bwd_tile_kernel<T, WT, TPR, NE, true>
-                              : layernorm_bwd_tile_kernel<T, WT, TPR, NE, false>;
-            const int most = TPR > 512 ? 148 : TPR > 256 ? 296 : kMaxParts;
+            auto kernel = layernorm_bwd_tile_kernel<T, WT, TPR, NE, false>;
+            const int most = TPR > 256 ? kMaxParts / 2 : kMaxParts;
             const long long blocks = (a.rows + kRows - 1) / kRows;
             parts = (int)(blocks < most ? blocks : most);
             pdl_launch(kernel, (unsigned)parts, kThreads, 0, st, (const T *)a.dy.p, a.dy.ld,
@@ -389,7 +622,37 @@ Status launch_layernorm_backward(const LayerNormBackwardArgs &a, cudaStream_t st
                        a.dx.ld, (const WT *)a.weight, a.mean, a.rstd, a.rows, a.D,
                        grads ? a.work : nullptr);
         };
-        if (a.rows == 0) {
+        auto ring = [&](auto tpr, auto ne) {
+            constexpr int TPR = decltype(tpr)::value, NE = decltype(ne)::value;
+            constexpr int kThreads = ring_threads(TPR), kRows = kThreads / TPR;
+            auto kernel = layernorm_bwd_ring_kernel<T, WT, TPR, NE>;
+            const int stages = ring_stages(ring_bytes(TPR), a.dsum.p ? 3 : 2, kRows, a.D, size);
+            if (stages < 2 || !smem_attr_once((const void *)kernel, ring_bytes(TPR))) return false;
+            const int reduce = kRows > 1 ? kThreads * NE * 4 : 0;
+            const int filled = stages * (a.dsum.p ? 3 : 2) * kRows * a.D * size;
+            const int smem = filled > reduce ? filled : reduce;
+            const long long blocks = (a.rows + kRows - 1) / kRows;
+            constexpr int kMost = 148 * ring_blocks(TPR);
+            parts = (int)(blocks < kMost ? blocks : kMost);
+            pdl_launch(kernel, (unsigned)parts, kThreads, (size_t)smem, st, (const T *)a.dy.p,
+                       a.dy.ld, (const T *)a.x.p, a.x.ld, (const T *)a.dsum.p, a.dsum.ld,
+                       ptr<T>(a.dx), a.dx.ld, (const WT *)a.weight, a.mean, a.rstd, a.rows, a.D,
+                       grads ? a.work : nullptr, stages);
+            return true;
+        };
+        // whole 16-byte vectors: the ring, 16 values a thread
+        bool done = a.rows == 0;
+        if (vec && !done) {
+            if (a.D <= 64) done = ring(Int<4>{}, Int<16>{});
+            else if (a.D <= 128) done = ring(Int<8>{}, Int<16>{});
+            else if (a.D <= 256) done = ring(Int<16>{}, Int<16>{});
+            else if (a.D <= 512) done = ring(Int<32>{}, Int<16>{});
+            else if (a.D <= 1024) done = ring(Int<64>{}, Int<16>{});
+            else if (a.D <= 2048) done = ring(Int<128>{}, Int<16>{});
+            else if (a.D <= 4096) done = ring(Int<256>{}, Int<16>{});
+            else if (a.D <= 8192) done = ring(Int<512>{}, Int<16>{});
+        }
+        if (done) {
         } else if (a.D <= 64) {
             tile(Int<8>{}, Int<8>{});
         } else if (a.D <= 256) {

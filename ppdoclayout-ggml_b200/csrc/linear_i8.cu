@@ -46,7 +46,6 @@ __device__ int g_linear_error = 0;
 constexpr int kFeat = 128;  // channels per tile (MMA M)
 constexpr int kBK = 128;    // k per stage: one 128-byte swizzle row
 constexpr int kWarpTma = 0, kWarpMma = 1, kWarpScale = 2, kWarpEpi = 4;
-constexpr long long kTimeoutCycles = 4000000000LL;
 // barriers, TMEM address and abort flag, then two tiles' scales: 128 channel
 // scales, 128 biases and up to 256 token scales each
 constexpr int kScaleFloats = 512;
@@ -111,22 +110,8 @@ struct Args {
     long long ldres, ldy;
 };
 
-// Bounded wait: false when the phase did not complete within the time limit
-// or another role already gave up.
 __device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity, volatile int *abort_flag) {
-    if (mbar_try_wait(bar, parity)) return true;
-    const long long t0 = clock64();
-    for (uint32_t i = 1;; i++) {
-        if (mbar_try_wait(bar, parity)) return true;
-        if ((i & 63) == 0) {
-            if (*abort_flag) return false;
-            if (clock64() - t0 > kTimeoutCycles) {
-                *abort_flag = 1;
-                atomicExch(&g_linear_error, 1);
-                return false;
-            }
-        }
-    }
+    return mbar_wait_bounded(bar, parity, abort_flag, &g_linear_error);
 }
 
 // D (TMEM) (+)= A (shared) * B (shared), 8-bit signed, K = 32
@@ -443,6 +428,7 @@ linear_i8_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
         prefetch_tensor_map(&tmQ);
     }
     pdl_begin();
+    pdl_trigger();
 
     const uint32_t rank = FORM == WHOLE ? 0 : cluster_rank();
     const uint32_t peers = FORM == WHOLE ? 1 : FORM == PAIR ? 2 : cluster_size();

@@ -70,8 +70,9 @@ PPDL_OPS_API int ppdl_op_supported(const ppdl_op_desc *d) {
 PPDL_OPS_API const char *ppdl_op_last_error(void) { return g_err; }
 
 PPDL_OPS_API int ppdl_op_device_error(void) {
-    const int gemm = ppdl::tc_error_fetch_and_clear(), linear = ppdl::linear_error_fetch_and_clear();
-    return gemm || linear ? 1 : 0;
+    const int gemm = ppdl::tc_error_fetch_and_clear(), linear = ppdl::linear_error_fetch_and_clear(),
+              rows = ppdl::row_error_fetch_and_clear();
+    return gemm || linear || rows ? 1 : 0;
 }
 
 PPDL_OPS_API int ppdl_gemm_tf32x3_presplit(int M, int N, int K, int batch, const float *A,

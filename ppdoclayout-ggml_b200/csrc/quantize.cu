@@ -62,6 +62,7 @@ quantize_tile_kernel(const T *x, long long ldx, long long rows, int K, int8_t *q
                      float *scale) {
     using Tile = RowTile<T, TPR, NE, VEC, 4>;
     pdl_begin();
+    pdl_trigger();
     __shared__ unsigned sh[32];
     constexpr int kRows = TPR < 128 ? 128 / TPR : 1;
     const int lane = threadIdx.x % TPR;
@@ -107,6 +108,7 @@ template <typename T>
 __global__ void quantize_row_kernel(const T *x, long long ldx, int K, int8_t *q, long long ldq,
                                     float *scale) {
     pdl_begin();
+    pdl_trigger();
     __shared__ unsigned sh[32];
     const long long row = blockIdx.x;
     x += row * ldx;

@@ -36,6 +36,7 @@ __device__ __forceinline__ float2 turn_of(const RotaryArgs &a, long long at, int
 template <typename T>
 __global__ void rotary_token_kernel(RotaryArgs a) {
     pdl_begin();
+    pdl_trigger();
     extern __shared__ float2 turn[];
     const int pairs = a.rotated / 2;
     const int b = blockIdx.x / a.length, t = blockIdx.x % a.length;

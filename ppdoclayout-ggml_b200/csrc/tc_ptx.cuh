@@ -33,6 +33,35 @@ __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
         : "memory");
     return ok != 0;
 }
+// Bounded wait (about 2 s): false when the phase did not complete in time —
+// then *error is raised on the device — or another thread of the block gave
+// up before (*abort_flag, in shared memory).
+__device__ __forceinline__ bool mbar_wait_bounded(uint32_t bar, uint32_t parity,
+                                                  volatile int *abort_flag, int *error) {
+    if (mbar_try_wait(bar, parity)) return true;
+    const long long t0 = clock64();
+    for (uint32_t i = 1;; i++) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if ((i & 63) == 0) {
+            if (*abort_flag) return false;
+            if (clock64() - t0 > 4000000000LL) {
+                *abort_flag = 1;
+                atomicExch(error, 1);
+                return false;
+            }
+        }
+    }
+}
+// `bytes` (a multiple of 16) from global to shared memory, both 16-byte
+// aligned, reported to the barrier
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes,
+                                          uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+            dst),
+        "l"(src), "r"(bytes), "r"(bar)
+        : "memory");
+}
 // Position in a ring of n stages or slots: index and mbarrier phase parity,
 // advanced by one step at a time (no division on the issue paths).
 struct Ring {
