@@ -52,7 +52,7 @@ __global__ void layernorm_row_kernel(const T *x, long long ldx, const T *res, lo
         const float d = value(i) - mean;
         s += d * d;
     }
-    const float rstd = 1.0f / sqrtf(block_sum(s, sh) / (float)D + eps);
+    const float rstd = rsqrtf(block_sum(s, sh) / (float)D + eps);
     for (int i = threadIdx.x; i < D; i += blockDim.x) {
         const float v = value(i);
         if (sum) sum[i] = from_float<T>(v);
@@ -106,7 +106,7 @@ layernorm_tile_kernel(const T *x, long long ldx, const T *res, long long ldres, 
         if (Tile::inside(j, D, lane)) s[0] += v[j] * v[j];
     }
     row_sums<TPR>(s, sh[1]);
-    const float rstd = 1.0f / sqrtf(s[0] / (float)D + eps);
+    const float rstd = rsqrtf(s[0] / (float)D + eps);
     if (!real) return;
     if (sum) Tile::store(sum + row * ldsum, r, D, lane);
     float p[NE];
@@ -125,9 +125,10 @@ layernorm_tile_kernel(const T *x, long long ldx, const T *res, long long ldres, 
 
 __device__ int g_row_error = 0;
 
-// Persistent blocks with the rows coming through a ring in shared memory
+// Persistent blocks with their rows coming through rings in shared memory
 // (RowRing), weights and biases in registers: for many rows of whole 16-byte
-// vectors.
+// vectors.  What bounds a 16-bit row is instructions, so a thread has 64 bytes
+// of it: sums, barrier and ring cost a warp about 100 instructions a row.
 constexpr int ring_threads(int tpr) { return tpr < 256 ? 256 : tpr; }
 constexpr int ring_blocks(int tpr) { return tpr > 256 ? 1 : 2; }
 template <typename T, typename WT, int TPR, int NE>
@@ -136,66 +137,79 @@ layernorm_ring_kernel(const T *x, long long ldx, const T *res, long long ldres, 
                       long long ldy, T *sum, long long ldsum, const WT *w, const WT *b,
                       float *mean_out, float *rstd_out, long long rows, int D, float eps,
                       int stages) {
-    using Tile = RowTile<T, TPR, NE, true>;
-    constexpr int kThreads = ring_threads(TPR);
-    using Rows = RowRing<T, TPR, kThreads, 2>;
+    using Tile = PairTile<T, TPR, NE>;
+    constexpr int kThreads = ring_threads(TPR), kHalf = Tile::kVec / 2;
+    using Rows = RowRing<T, TPR, NE, kThreads, 2>;
     extern __shared__ __align__(16) uint8_t ring_smem[];
-    __shared__ uint64_t bars[Rows::kTeams * kRingStages];
-    __shared__ float sh[2][kThreads / 32];
-    __shared__ int abort_word;
-    const int lane = threadIdx.x % TPR, team = threadIdx.x / Rows::kTeam;
-    const int sub = threadIdx.x % Rows::kTeam / TPR;
+    __shared__ typename Rows::Shared shared;
+    __shared__ __align__(16) float sh[2][kThreads / 32];
+    const int lane = threadIdx.x % TPR, team = threadIdx.x / TPR;
     Rows ring;
-    ring.src[0] = x; ring.src[1] = res;
-    ring.ld[0] = ldx; ring.ld[1] = ldres;
-    ring.setup(ring_smem, bars, &abort_word, &g_row_error, rows, D, stages);
+    ring.setup({x, res}, {ldx, ldres}, ring_smem, &shared, &g_row_error, rows, D, stages);
     pdl_begin();
     pdl_trigger();
     ring.start();
-    float pw[NE], pb[NE];
+    float2 pw[NE / 2], pb[NE / 2];
     Tile::load_params(pw, w, 1.0f, D, lane);
     Tile::load_params(pb, b, 0.0f, D, lane);
     const float inv_d = 1.0f / (float)D;
-    for (long long r0 = ring.first; r0 < rows; r0 += ring.step, ring.at.next()) {
-        const long long row = r0 + sub;
+    y += ring.first * ldy;
+    if (sum) sum += ring.first * ldsum;
+    if (mean_out) mean_out += ring.first;
+    if (rstd_out) rstd_out += ring.first;
+    const long long ystep = ring.step * ldy, sumstep = ring.step * ldsum;
+    for (int it = 0; it < ring.iters; it++, ring.at.next()) {
         ring.wait();
         typename Tile::Raw r;
-        Tile::load(r, ring.row(0), D, lane);
+        Tile::load(r, ring.slice(0), D, lane);
         if (res) {
             typename Tile::Raw q;
-            Tile::load(q, ring.row(1), D, lane);
+            Tile::load(q, ring.slice(1), D, lane);
 #pragma unroll
-            for (int j = 0; j < NE; j++) r.v[j] = from_float<T>(to_float(r.v[j]) + to_float(q.v[j]));
+            for (int j = 0; j < NE / 2; j++)
+                Tile::set_pair(r, j, add2(Tile::pair(r, j), Tile::pair(q, j)));
         }
-        float v[NE], s[1] = {0.0f};
+        ring.refill();
+        float2 v[NE / 2], t = both(0.0f);
 #pragma unroll
-        for (int j = 0; j < NE; j++) {
-            v[j] = to_float(r.v[j]);
-            s[0] += v[j];
+        for (int j = 0; j < NE / 2; j++) {
+            v[j] = Tile::pair(r, j);
+            t = add2(t, v[j]);
         }
+        const bool real = it < ring.mine && ring.good;
+        if (sum && real) Tile::store(sum, r, D, lane);
+        float s[1] = {t.x + t.y};
         team_sums<TPR>(s, sh[0], team);
-        if constexpr (TPR <= 32) __syncwarp();
-        ring.refill(r0);
         const float mean = s[0] * inv_d;
-        s[0] = 0.0f;
+        t = both(0.0f);
 #pragma unroll
-        for (int j = 0; j < NE; j++) {
-            v[j] -= mean;
-            if (Tile::inside(j, D, lane)) s[0] += v[j] * v[j];
-        }
-        team_sums<TPR>(s, sh[1], team);
-        const float rstd = 1.0f / sqrtf(s[0] * inv_d + eps);
-        if (row < rows && ring.good) {
-            if (sum) Tile::store(sum + row * ldsum, r, D, lane);
+        for (int i = 0; i < Tile::kVecs; i++) {
+            // a vector past D holds zeros and takes no part
+            if (Tile::column(i, lane) < D) {
 #pragma unroll
-            for (int j = 0; j < NE; j++)
-                r.v[j] = from_float<T>(__fmaf_rn(v[j] * rstd, pw[j], pb[j]));
-            Tile::store(y + row * ldy, r, D, lane);
-            if (lane == 0) {
-                if (mean_out) mean_out[row] = mean;
-                if (rstd_out) rstd_out[row] = rstd;
+                for (int j = i * kHalf; j < (i + 1) * kHalf; j++) {
+                    v[j] = add2(v[j], both(-mean));
+                    t = fma2(v[j], v[j], t);
+                }
             }
         }
+        s[0] = t.x + t.y;
+        team_sums<TPR>(s, sh[1], team);
+        const float rstd = rsqrtf(s[0] * inv_d + eps);
+        if (real) {
+#pragma unroll
+            for (int j = 0; j < NE / 2; j++)
+                Tile::set_pair(r, j, fma2(mul2(v[j], both(rstd)), pw[j], pb[j]));
+            Tile::store(y, r, D, lane);
+            if (lane == 0) {
+                if (mean_out) *mean_out = mean;
+                if (rstd_out) *rstd_out = rstd;
+            }
+        }
+        y += ystep;
+        if (sum) sum += sumstep;
+        if (mean_out) mean_out += ring.step;
+        if (rstd_out) rstd_out += ring.step;
     }
 }
 
@@ -291,12 +305,12 @@ layernorm_bwd_tile_kernel(const T *dy, long long lddy, const T *x, long long ldx
     for (long long base = (long long)blockIdx.x * kRows; base < rows;
          base += step, row += step, parity ^= 1) {
         const bool real = row < rows;
-        const float m = mean, r = rstd;
+        const float m = mean, r = rstd, gate = real ? 1.0f : 0.0f;
         float xh[NE], g[NE];
 #pragma unroll
         for (int j = 0; j < NE; j++) {
             xh[j] = (to_float(rx.v[j]) - m) * r;
-            g[j] = real ? to_float(rdy.v[j]) : 0.0f;
+            g[j] = to_float(rdy.v[j]) * gate;
         }
         if (base + step < rows) load(row + step);
         float s[2] = {0.0f, 0.0f};
@@ -355,114 +369,126 @@ layernorm_bwd_tile_kernel(const T *dy, long long lddy, const T *x, long long ldx
     }
 }
 
-// The same with the rows coming through a ring in shared memory (RowRing).
+// The same with the rows coming through rings in shared memory, as in
+// layernorm_ring_kernel.
 template <typename T, typename WT, int TPR, int NE>
 __global__ void __launch_bounds__(ring_threads(TPR), ring_blocks(TPR))
 layernorm_bwd_ring_kernel(const T *dy, long long lddy, const T *x, long long ldx, const T *dsum,
                           long long lddsum, T *dx, long long lddx, const WT *w,
                           const float *mean_in, const float *rstd_in, long long rows, int D,
                           float *part, int stages) {
-    using Tile = RowTile<T, TPR, NE, true>;
+    using Tile = PairTile<T, TPR, NE>;
     constexpr int kThreads = ring_threads(TPR);
-    using Rows = RowRing<T, TPR, kThreads, 3>;
+    using Rows = RowRing<T, TPR, NE, kThreads, 3>;
     constexpr int kRows = Rows::kRows;
     extern __shared__ __align__(16) uint8_t ring_smem[];
-    __shared__ uint64_t bars[Rows::kTeams * kRingStages];
-    __shared__ float sh[2][kThreads / 32 * 2];
-    __shared__ int abort_word;
-    const int lane = threadIdx.x % TPR, team = threadIdx.x / Rows::kTeam;
-    const int sub = threadIdx.x % Rows::kTeam / TPR;
+    __shared__ typename Rows::Shared shared;
+    __shared__ __align__(16) float sh[2][kThreads / 32 * 2];
+    const int lane = threadIdx.x % TPR, team = threadIdx.x / TPR;
     Rows ring;
-    ring.src[0] = x; ring.src[1] = dy; ring.src[2] = dsum;
-    ring.ld[0] = ldx; ring.ld[1] = lddy; ring.ld[2] = lddsum;
-    ring.setup(ring_smem, bars, &abort_word, &g_row_error, rows, D, stages);
+    ring.setup({x, dy, dsum}, {ldx, lddy, lddsum}, ring_smem, &shared, &g_row_error, rows, D,
+               stages);
     pdl_begin();
     pdl_trigger();
     ring.start();
-
-    float p[NE], dw[NE], db[NE];
+    float2 p[NE / 2], dw[NE / 2], db[NE / 2];
     Tile::load_params(p, w, 1.0f, D, lane);
 #pragma unroll
-    for (int j = 0; j < NE; j++) dw[j] = db[j] = 0.0f;
-    float mean = 0.0f, rstd = 0.0f;
-    if (ring.first + sub < rows) {
-        mean = mean_in[ring.first + sub];
-        rstd = rstd_in[ring.first + sub];
-    }
+    for (int j = 0; j < NE / 2; j++) dw[j] = db[j] = both(0.0f);
     const float inv_d = 1.0f / (float)D;
-    int parity = 0;
-    for (long long r0 = ring.first; r0 < rows; r0 += ring.step, ring.at.next(), parity ^= 1) {
-        const long long row = r0 + sub;
-        const bool real = row < rows;
+    // the rows' statistics, two iterations ahead: a load queues behind the
+    // stores before it
+    float mean[2] = {}, rstd[2] = {};
+    mean_in += ring.first;
+    rstd_in += ring.first;
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+        if (k < ring.mine) {
+            mean[k] = *mean_in;
+            rstd[k] = *rstd_in;
+        }
+        mean_in += ring.step;
+        rstd_in += ring.step;
+    }
+    dx += ring.first * lddx;
+    const long long dxstep = ring.step * lddx;
+    for (int it = 0; it < ring.iters; it++, ring.at.next(), dx += dxstep) {
         ring.wait();
+        const float r = rstd[0];
+        // x r - mean r: off by the rounding of mean r, u |mean| r
+        const float mr = -mean[0] * r;
+        mean[0] = mean[1];
+        rstd[0] = rstd[1];
+        if (it + 2 < ring.mine) {
+            mean[1] = *mean_in;
+            rstd[1] = *rstd_in;
+        }
+        mean_in += ring.step;
+        rstd_in += ring.step;
+        const bool real = it < ring.mine;
         typename Tile::Raw rx, rdy, out;
-        Tile::load(rx, ring.row(0), D, lane);
-        Tile::load(rdy, ring.row(1), D, lane);
-        if (dsum) Tile::load(out, ring.row(2), D, lane);
-        const float r = rstd, mr = -mean * rstd;
-        if (row + ring.step < rows) {
-            mean = mean_in[row + ring.step];
-            rstd = rstd_in[row + ring.step];
-        }
-        float xh[NE], g[NE], s[2] = {0.0f, 0.0f};
-        if (!real) {
-            // past the end: whatever the buffer held, and no gradient
+        float2 g[NE / 2], t0 = both(0.0f), t1 = both(0.0f);
+        if (real) {
+            Tile::load(rx, ring.slice(0), D, lane);
+            Tile::load(rdy, ring.slice(1), D, lane);
+            if (dsum) Tile::load(out, ring.slice(2), D, lane);
 #pragma unroll
-            for (int j = 0; j < NE; j++) rx.v[j] = rdy.v[j] = from_float<T>(0.0f);
+            for (int j = 0; j < NE / 2; j++) {
+                const float2 xh = fma2(Tile::pair(rx, j), both(r), both(mr));
+                const float2 d = Tile::pair(rdy, j);
+                dw[j] = fma2(d, xh, dw[j]);
+                db[j] = add2(db[j], d);
+                g[j] = mul2(d, p[j]);
+                t0 = add2(t0, g[j]);
+                t1 = fma2(g[j], xh, t1);
+            }
         }
-#pragma unroll
-        for (int j = 0; j < NE; j++) {
-            // x r - mean r: off by the rounding of mean r, u |mean| r
-            xh[j] = __fmaf_rn(to_float(rx.v[j]), r, mr);
-            g[j] = to_float(rdy.v[j]);
-            dw[j] += g[j] * xh[j];
-            db[j] += g[j];
-            g[j] *= p[j];
-            s[0] += g[j];
-            s[1] += g[j] * xh[j];
-        }
-        team_sums<TPR>(s, sh[parity], team);
-        if constexpr (TPR <= 32) __syncwarp();
-        ring.refill(r0);
-        const float m1 = s[0] * inv_d * r, m2 = s[1] * inv_d * r;
+        ring.refill();
+        float s[2] = {t0.x + t0.y, t1.x + t1.y};
+        team_sums<TPR>(s, sh[it & 1], team);
+        const float2 m1 = both(-s[0] * inv_d * r), m2 = both(-s[1] * inv_d * r);
         if (real && ring.good) {
 #pragma unroll
-            for (int j = 0; j < NE; j++) {
-                float v = __fmaf_rn(g[j], r, -__fmaf_rn(xh[j], m2, m1));
-                if (dsum) v += to_float(out.v[j]);
-                out.v[j] = from_float<T>(v);
+            for (int j = 0; j < NE / 2; j++) {
+                // xh again: kept, it would be spilled, and a load from local
+                // memory queues behind the stores
+                const float2 xh = fma2(Tile::pair(rx, j), both(r), both(mr));
+                float2 v = fma2(g[j], both(r), fma2(xh, m2, m1));
+                if (dsum) v = add2(v, Tile::pair(out, j));
+                Tile::set_pair(out, j, v);
             }
-            Tile::store(dx + row * lddx, out, D, lane);
+            Tile::store(dx, out, D, lane);
         }
     }
     if (!part) return;
     part += (long long)blockIdx.x * 2 * D;
     if constexpr (kRows == 1) {
 #pragma unroll
-        for (int j = 0; j < NE; j++) {
-            const int c = Tile::column(j / Tile::kVec, lane) + j % Tile::kVec;
+        for (int j = 0; j < NE / 2; j++) {
+            const int c = Tile::pair_column(j, lane);
             if (c < D) {
-                part[c] = dw[j];
-                part[D + c] = db[j];
+                part[c] = dw[j].x;
+                part[c + 1] = dw[j].y;
+                part[D + c] = db[j].x;
+                part[D + c + 1] = db[j].y;
             }
         }
     } else {
         // the block's rows' sums in order, through the ring (all copies landed)
-        float *red = reinterpret_cast<float *>(ring_smem);
-        const int group = threadIdx.x / TPR;
+        float2 *red = reinterpret_cast<float2 *>(ring_smem);
         for (int which = 0; which < 2; which++) {
             __syncthreads();
 #pragma unroll
-            for (int j = 0; j < NE; j++)
-                red[(group * NE + j) * TPR + lane] = which ? db[j] : dw[j];
+            for (int j = 0; j < NE / 2; j++)
+                red[(team * (NE / 2) + j) * TPR + lane] = which ? db[j] : dw[j];
             __syncthreads();
-            for (int t = threadIdx.x; t < TPR * NE; t += kThreads) {
-                const int j = t / TPR, l = t % TPR;
-                const int c = Tile::column(j / Tile::kVec, l) + j % Tile::kVec;
+            for (int t = threadIdx.x; t < TPR * NE / 2; t += kThreads) {
+                const int c = Tile::pair_column(t / TPR, t % TPR);
                 if (c < D) {
-                    float sum = 0.0f;
-                    for (int q = 0; q < kRows; q++) sum += red[q * NE * TPR + t];
-                    part[which * D + c] = sum;
+                    float2 sum = both(0.0f);
+                    for (int q = 0; q < kRows; q++) sum = add2(sum, red[q * (NE / 2) * TPR + t]);
+                    part[which * D + c] = sum.x;
+                    part[which * D + c + 1] = sum.y;
                 }
             }
         }
@@ -507,8 +533,22 @@ Status with_types(int type, int w_type, F f) {
     });
 }
 
-// shared memory of a block's ring: its share of an SM's
+// the ring kernels: SMs, shared memory of a block's ring, and the threads of
+// a row of D values, NE each
+constexpr int kSms = 148;
 constexpr int ring_bytes(int tpr) { return 216 * 1024 / ring_blocks(tpr) - 4096; }
+template <int NE, typename F>
+bool ring_dispatch(int D, F f) {
+    if (D <= 4 * NE) return f(Int<4>{});
+    if (D <= 8 * NE) return f(Int<8>{});
+    if (D <= 16 * NE) return f(Int<16>{});
+    if (D <= 32 * NE) return f(Int<32>{});
+    if (D <= 64 * NE) return f(Int<64>{});
+    if (D <= 128 * NE) return f(Int<128>{});
+    if (D <= 256 * NE) return f(Int<256>{});
+    if (D <= 512 * NE) return f(Int<512>{});
+    return false;
+}
 
 template <typename T>
 T *ptr(const Rows &r) { return (T *)r.p; }
@@ -544,36 +584,30 @@ Status launch_layernorm(const LayerNormArgs &a, cudaStream_t st) {
                        a.rstd, a.rows, a.D, a.eps);
             return cuda_status();
         };
-        auto ring = [&](auto tpr, auto ne) {
-            constexpr int TPR = decltype(tpr)::value, NE = decltype(ne)::value;
-            constexpr int kThreads = ring_threads(TPR), kRows = kThreads / TPR;
-            constexpr int kMost = 148 * ring_blocks(TPR);
-            auto kernel = layernorm_ring_kernel<T, WT, TPR, NE>;
-            const int stages = ring_stages(ring_bytes(TPR), a.res.p ? 2 : 1, kRows, a.D, size);
-            const long long blocks = (a.rows + kRows - 1) / kRows;
-            if (blocks < 3 * kMost || stages < 2 ||
+        constexpr int kRingNE = 16;
+        auto ring = [&](auto tpr) {
+            constexpr int TPR = decltype(tpr)::value, kThreads = ring_threads(TPR);
+            using Rows = RowRing<T, TPR, kRingNE, kThreads, 2>;
+            auto kernel = layernorm_ring_kernel<T, WT, TPR, kRingNE>;
+            const long long stage = Rows::block_stage(a.res.p ? 2 : 1, a.D);
+            const int stages = ring_stages(ring_bytes(TPR), stage);
+            constexpr int kBlocks = kSms * ring_blocks(TPR);
+            // at least 4 rows for each place in a block, or the tile's blocks
+            // are done before the rings are set up
+            if (a.rows < 4LL * kBlocks * Rows::kRows || stages < 2 ||
                 !smem_attr_once((const void *)kernel, ring_bytes(TPR)))
                 return false;
-            pdl_launch(kernel, (unsigned)kMost, kThreads,
-                       (size_t)(stages * (a.res.p ? 2 : 1) * kRows * a.D * size), st,
+            pdl_launch(kernel, (unsigned)kBlocks, kThreads, (size_t)(stages * stage), st,
                        (const T *)a.x.p, a.x.ld, (const T *)a.res.p, a.res.ld, ptr<T>(a.y), a.y.ld,
                        ptr<T>(a.sum), a.sum.ld, (const WT *)a.weight, (const WT *)a.bias, a.mean,
                        a.rstd, a.rows, a.D, a.eps, stages);
             return true;
         };
-        if (vec) {
-            bool done = false;
-            if (a.D <= 64) done = ring(Int<4>{}, Int<16>{});
-            else if (a.D <= 128) done = ring(Int<8>{}, Int<16>{});
-            else if (a.D <= 256) done = ring(Int<16>{}, Int<16>{});
-            else if (a.D <= 512) done = ring(Int<32>{}, Int<16>{});
-            else if (a.D <= 1024) done = ring(Int<64>{}, Int<16>{});
-            else if (a.D <= 2048) done = ring(Int<128>{}, Int<16>{});
-            else if (a.D <= 4096) done = ring(Int<256>{}, Int<16>{});
-            else if (a.D <= 8192) done = ring(Int<512>{}, Int<16>{});
-            else if (a.D <= 16384) done = ring(Int<1024>{}, Int<16>{});
-            if (done) return cuda_status();
-        }
+        // FP32 rows fill the bandwidth from the tile kernel's blocks (52500 x
+        // 256 with a residual 33.7 us, by the ring 36.9) unless they are short
+        // (100000 x 96: 22.5 / 13.2); 16-bit ones gain (8192 x 4096 34 / 30)
+        if (vec && (sizeof(T) == 2 || a.D <= 128) && ring_dispatch<kRingNE>(a.D, ring))
+            return cuda_status();
         // the smallest tile that holds the row, 64 bytes a thread
         constexpr int NE = sizeof(T) == 2 ? 32 : 16, F = sizeof(T) == 2 ? 1 : 2;
         if (a.D <= 64) return tile(Int<4>{}, Int<16>{});
@@ -623,35 +657,30 @@ Status launch_layernorm_backward(const LayerNormBackwardArgs &a, cudaStream_t st
                        grads ? a.work : nullptr);
         };
         auto ring = [&](auto tpr, auto ne) {
-            constexpr int TPR = decltype(tpr)::value, NE = decltype(ne)::value;
-            constexpr int kThreads = ring_threads(TPR), kRows = kThreads / TPR;
+            constexpr int TPR = decltype(tpr)::value, NE = decltype(ne)::value, kThreads = ring_threads(TPR);
+            using Rows = RowRing<T, TPR, NE, kThreads, 3>;
             auto kernel = layernorm_bwd_ring_kernel<T, WT, TPR, NE>;
-            const int stages = ring_stages(ring_bytes(TPR), a.dsum.p ? 3 : 2, kRows, a.D, size);
+            const long long stage = Rows::block_stage(a.dsum.p ? 3 : 2, a.D);
+            const int stages = ring_stages(ring_bytes(TPR), stage);
             if (stages < 2 || !smem_attr_once((const void *)kernel, ring_bytes(TPR))) return false;
-            const int reduce = kRows > 1 ? kThreads * NE * 4 : 0;
-            const int filled = stages * (a.dsum.p ? 3 : 2) * kRows * a.D * size;
-            const int smem = filled > reduce ? filled : reduce;
-            const long long blocks = (a.rows + kRows - 1) / kRows;
-            constexpr int kMost = 148 * ring_blocks(TPR);
-            parts = (int)(blocks < kMost ? blocks : kMost);
+            const long long reduce = Rows::kRows > 1 ? kThreads * NE * 4 : 0;
+            const long long smem = stages * stage > reduce ? stages * stage : reduce;
+            const long long blocks = (a.rows + Rows::kRows - 1) / Rows::kRows;
+            constexpr int kBlocks = kSms * ring_blocks(TPR);
+            parts = (int)(blocks < kBlocks ? blocks : kBlocks);
             pdl_launch(kernel, (unsigned)parts, kThreads, (size_t)smem, st, (const T *)a.dy.p,
                        a.dy.ld, (const T *)a.x.p, a.x.ld, (const T *)a.dsum.p, a.dsum.ld,
                        ptr<T>(a.dx), a.dx.ld, (const WT *)a.weight, a.mean, a.rstd, a.rows, a.D,
                        grads ? a.work : nullptr, stages);
             return true;
         };
-        // whole 16-byte vectors: the ring, 16 values a thread
-        bool done = a.rows == 0;
-        if (vec && !done) {
-            if (a.D <= 64) done = ring(Int<4>{}, Int<16>{});
-            else if (a.D <= 128) done = ring(Int<8>{}, Int<16>{});
-            else if (a.D <= 256) done = ring(Int<16>{}, Int<16>{});
-            else if (a.D <= 512) done = ring(Int<32>{}, Int<16>{});
-            else if (a.D <= 1024) done = ring(Int<64>{}, Int<16>{});
-            else if (a.D <= 2048) done = ring(Int<128>{}, Int<16>{});
-            else if (a.D <= 4096) done = ring(Int<256>{}, Int<16>{});
-            else if (a.D <= 8192) done = ring(Int<512>{}, Int<16>{});
-        }
+        // two vectors a thread: 16 values of 16 bits or 8 of 32 (with 16, FP32
+        // rows spill; wider than 4096 they have to)
+        constexpr int kNE = 32 / (int)sizeof(T);
+        const bool done =
+            a.rows == 0 ||
+            (vec && (ring_dispatch<kNE>(a.D, [&](auto tpr) { return ring(tpr, Int<kNE>{}); }) ||
+                     (sizeof(T) == 4 && a.D > 4096 && a.D <= 8192 && ring(Int<512>{}, Int<16>{}))));
         if (done) {
         } else if (a.D <= 64) {
             tile(Int<8>{}, Int<8>{});

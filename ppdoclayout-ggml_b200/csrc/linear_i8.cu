@@ -153,12 +153,7 @@ __device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap
         "l"(reinterpret_cast<uint64_t>(tm)), "r"(bar), "r"(x), "r"(y)
         : "memory");
 }
-// Arrivals that publish nothing in memory: the epilogue has read its TMEM
-// columns (or scales) into registers.  A releasing arrive would wait for the
-// warp's stores to y, hundreds of cycles a tile.
-__device__ __forceinline__ void mbar_arrive_relaxed(uint32_t bar) {
-    asm volatile("mbarrier.arrive.relaxed.cta.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
-}
+// mbar_arrive_relaxed at another CTA's barrier
 __device__ __forceinline__ void mbar_arrive_relaxed_cluster(uint32_t bar) {
     asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar)
                  : "memory");
@@ -207,50 +202,6 @@ __device__ __forceinline__ void tile_of(const Args &a, int tile, int &ft, int &t
     const int width = min(kGroup, a.t_tiles - g * kGroup);
     ft = width == kGroup ? r / kGroup : r / width;
     tt = g * kGroup + r - ft * width;
-}
-
-template <typename T>
-__device__ __forceinline__ uint32_t pack2(float lo, float hi);
-template <>
-__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
-    const __nv_bfloat162 p = __floats2bfloat162_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t *>(&p);
-}
-template <>
-__device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
-    const __half2 p = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t *>(&p);
-}
-template <typename T>
-__device__ __forceinline__ float2 unpack2(uint32_t v);
-template <>
-__device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t v) {
-    return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&v));
-}
-template <>
-__device__ __forceinline__ float2 unpack2<__half>(uint32_t v) {
-    return __half22float2(*reinterpret_cast<const __half2 *>(&v));
-}
-
-// Two FP32 values in one register pair: sm_100 multiplies and adds them in
-// one instruction, each rounded as its own.
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-    float2 r;
-    asm("{\n\t.reg .b64 x, y, z;\n\t"
-        "mov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
-        "mul.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"
-        : "=f"(r.x), "=f"(r.y)
-        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-    return r;
-}
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-    float2 r;
-    asm("{\n\t.reg .b64 x, y, z, w;\n\t"
-        "mov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 w, {%6, %7};\n\t"
-        "fma.rn.f32x2 z, x, y, w;\n\tmov.b64 {%0, %1}, z;\n\t}"
-        : "=f"(r.x), "=f"(r.y)
-        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-    return r;
 }
 
 // What follows the sum.  acc is rounded to FP32 (2^-24 relative), the two

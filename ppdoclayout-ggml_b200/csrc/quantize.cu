@@ -48,19 +48,104 @@ __device__ __forceinline__ unsigned row_max(unsigned m, unsigned *sh) {
     if constexpr (TPR > 32) {
         if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = m;
         __syncthreads();
+        sh += threadIdx.x / TPR * (TPR / 32);  // the row's warps
 #pragma unroll
         for (int w = 0; w < TPR / 32; w++) m = max(m, sh[w]);
     }
     return m;
 }
 
-// Rows in registers, as layernorm_tile_kernel; a thread's neighbouring
-// values leave as one store of 4 or 8 bytes.
-template <typename T, int TPR, int NE, bool VEC>
+// The bits of the largest |v| of a word of values (two 16-bit ones, or one).
+template <typename T>
+struct AbsMax {
+    uint32_t m = 0;
+    __device__ __forceinline__ void add(uint32_t w) { m = max(m, w & 0x7fffffffu); }
+    __device__ __forceinline__ unsigned bits() const { return m; }
+};
+template <>
+struct AbsMax<__nv_bfloat16> {
+    uint32_t m = 0;
+    __device__ __forceinline__ void add(uint32_t w) { m = __vmaxu2(m, w & 0x7fff7fffu); }
+    __device__ __forceinline__ unsigned bits() const { return max(m & 0xffffu, m >> 16) << 16; }
+};
+template <>
+struct AbsMax<__half> {
+    uint32_t m = 0;
+    __device__ __forceinline__ void add(uint32_t w) { m = __vmaxu2(m, w & 0x7fff7fffu); }
+    __device__ __forceinline__ unsigned bits() const {
+        return __float_as_uint(__half2float(__ushort_as_half((unsigned short)max(m & 0xffffu, m >> 16))));
+    }
+};
+
+// Rows of whole 16-byte vectors in registers.  The quotient is first taken
+// as x (1 / s), off by at most 127 x 2^-23 = 1.6e-5, and rounded by adding
+// 1.5 x 2^23, which leaves the whole number in the low byte; only a thread
+// with a value that close to a half decides on the remainders (about one in
+// a thousand).
+template <typename T, int TPR, int NE>
+__global__ void __launch_bounds__(TPR < 128 ? 128 : TPR)
+quantize_vector_kernel(const T *x, long long ldx, long long rows, int K, int8_t *q, long long ldq,
+                       float *scale) {
+    using Tile = PairTile<T, TPR, NE>;
+    pdl_begin();
+    pdl_trigger();
+    __shared__ unsigned sh[32];
+    constexpr int kRows = TPR < 128 ? 128 / TPR : 1, kWords = Tile::kVecs * 4;
+    const int lane = threadIdx.x % TPR;
+    long long row = (long long)blockIdx.x * kRows + threadIdx.x / TPR;
+    const bool real = row < rows;
+    if (!real) row = rows - 1;
+    typename Tile::Raw r;
+    Tile::load_row(r, x + row * ldx, K, lane);
+    AbsMax<T> most;
+#pragma unroll
+    for (int k = 0; k < kWords; k++) most.add(Tile::word(r, k));
+    const Divisor d(row_max<TPR>(most.bits(), sh));
+    if (!real) return;
+    if (lane == 0) scale[row] = d.s;
+    q += row * ldq;
+    const float2 inv = both(d.usable ? d.inv : 0.0f), magic = both(12582912.0f);
+    float far = 0.0f;
+    uint32_t out[NE / 4];
+#pragma unroll
+    for (int j = 0; j < NE / 2; j += 2) {
+        const float2 t0 = mul2(Tile::pair(r, j), inv), t1 = mul2(Tile::pair(r, j + 1), inv);
+        const float2 m0 = add2(t0, magic), m1 = add2(t1, magic);
+        // how far each is from its whole number: at most 1/2
+        const float2 d0 = add2(t0, sub2(magic, m0)), d1 = add2(t1, sub2(magic, m1));
+        far = fmaxf(fmaxf(far, fmaxf(fabsf(d0.x), fabsf(d0.y))), fmaxf(fabsf(d1.x), fabsf(d1.y)));
+        const uint32_t lo = __byte_perm(__float_as_uint(m0.x), __float_as_uint(m0.y), 0x0040);
+        const uint32_t hi = __byte_perm(__float_as_uint(m1.x), __float_as_uint(m1.y), 0x0040);
+        out[j / 2] = __byte_perm(lo, hi, 0x5410);
+    }
+    // (a row that is not usable has inv 0 and q 0; its NaNs and infinities
+    // give NaN here and are zeroed by the exact form)
+    if (!(far < 0.49998f) || d.up != 1.0f || !d.usable) {
+#pragma unroll
+        for (int j = 0; j < NE / 2; j += 2) {
+            const float2 a = Tile::pair(r, j), b = Tile::pair(r, j + 1);
+            out[j / 2] = (uint32_t)(d(a.x) & 255) | (uint32_t)(d(a.y) & 255) << 8 |
+                         (uint32_t)(d(b.x) & 255) << 16 | (uint32_t)(d(b.y) & 255) << 24;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < Tile::kVecs; i++) {
+        const int c = Tile::column(i, lane);
+        if (c >= K) continue;
+        if constexpr (Tile::kVec == 8)
+            *reinterpret_cast<uint2 *>(q + c) = make_uint2(out[2 * i], out[2 * i + 1]);
+        else
+            *reinterpret_cast<uint32_t *>(q + c) = out[i];
+    }
+}
+
+// Rows in registers, any alignment; a thread's neighbouring values leave as
+// one store of 4 bytes.
+template <typename T, int TPR, int NE>
 __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR)
 quantize_tile_kernel(const T *x, long long ldx, long long rows, int K, int8_t *q, long long ldq,
                      float *scale) {
-    using Tile = RowTile<T, TPR, NE, VEC, 4>;
+    using Tile = RowTile<T, TPR, NE, false, 4>;
     pdl_begin();
     pdl_trigger();
     __shared__ unsigned sh[32];
@@ -90,10 +175,7 @@ quantize_tile_kernel(const T *x, long long ldx, long long rows, int K, int8_t *q
                 w[h] |= (unsigned)(d(to_float(r.v[i * Tile::kVec + 4 * h + e])) & 255) << (8 * e);
         }
         if (c + Tile::kVec <= K) {
-            if constexpr (Tile::kVec == 8)
-                *reinterpret_cast<uint2 *>(q + c) = make_uint2(w[0], w[1]);
-            else
-                *reinterpret_cast<unsigned *>(q + c) = w[0];
+            *reinterpret_cast<unsigned *>(q + c) = w[0];
         } else {
 #pragma unroll
             for (int e = 0; e < Tile::kVec; e++)
@@ -133,12 +215,28 @@ Status launch_quantize_rows(const Rows &x, int type, long long rows, int K, int8
         auto tile = [&](auto tpr, auto ne) {
             constexpr int TPR = decltype(tpr)::value, NE = decltype(ne)::value;
             constexpr int kThreads = TPR < 128 ? 128 : TPR;
-            auto kernel = vec ? quantize_tile_kernel<T, TPR, NE, true>
-                              : quantize_tile_kernel<T, TPR, NE, false>;
-            pdl_launch(kernel, (unsigned)cdiv(rows, kThreads / TPR), kThreads, 0, st,
+            pdl_launch(quantize_tile_kernel<T, TPR, NE>, (unsigned)cdiv(rows, kThreads / TPR), kThreads, 0, st,
                        (const T *)x.p, x.ld, rows, K, q, ldq, scale);
             return cuda_status();
         };
+        auto vectors = [&](auto tpr) {
+            constexpr int TPR = decltype(tpr)::value, NE = 64 / (int)sizeof(T);
+            constexpr int kThreads = TPR < 128 ? 128 : TPR;
+            pdl_launch(quantize_vector_kernel<T, TPR, NE>, (unsigned)cdiv(rows, kThreads / TPR),
+                       kThreads, 0, st, (const T *)x.p, x.ld, rows, K, q, ldq, scale);
+            return cuda_status();
+        };
+        if (vec) {
+            constexpr int NE = 64 / (int)sizeof(T);
+            if (K <= 4 * NE) return vectors(Int<4>{});
+            if (K <= 8 * NE) return vectors(Int<8>{});
+            if (K <= 16 * NE) return vectors(Int<16>{});
+            if (K <= 32 * NE) return vectors(Int<32>{});
+            if (K <= 64 * NE) return vectors(Int<64>{});
+            if (K <= 128 * NE) return vectors(Int<128>{});
+            if (K <= 256 * NE) return vectors(Int<256>{});
+            if (K <= 512 * NE) return vectors(Int<512>{});
+        }
         if (K <= 64) return tile(Int<8>{}, Int<8>{});
         if (K <= 256) return tile(Int<32>{}, Int<8>{});
         if (K <= 512) return tile(Int<32>{}, Int<16>{});

@@ -135,108 +135,232 @@ __device__ __forceinline__ void team_sums(float (&v)[N], float *sh, int team) {
         for (int i = 0; i < N; i++) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
     if constexpr (TPR > 32) {
         constexpr int kWarps = TPR / 32;
+        static_assert(kWarps * N % 2 == 0, "whole pairs");
         sh += team * (kWarps * N);
         if ((threadIdx.x & 31) == 0)
 #pragma unroll
             for (int i = 0; i < N; i++) sh[threadIdx.x % TPR / 32 * N + i] = v[i];
         asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "n"(TPR) : "memory");
+        // read as vectors; added in the warps' order
+        constexpr int kV = kWarps * N % 4 == 0 ? 4 : 2;
+        float all[kWarps * N];
 #pragma unroll
-        for (int i = 0; i < N; i++) v[i] = sh[i];
+        for (int i = 0; i < kWarps * N; i += kV) {
+            if constexpr (kV == 4) {
+                const float4 f = *reinterpret_cast<const float4 *>(sh + i);
+                all[i] = f.x; all[i + 1] = f.y; all[i + 2] = f.z; all[i + 3] = f.w;
+            } else {
+                const float2 f = *reinterpret_cast<const float2 *>(sh + i);
+                all[i] = f.x; all[i + 1] = f.y;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < N; i++) v[i] = all[i];
 #pragma unroll
         for (int w = 1; w < kWarps; w++)
 #pragma unroll
-            for (int i = 0; i < N; i++) v[i] += sh[w * N + i];
+            for (int i = 0; i < N; i++) v[i] += all[w * N + i];
     }
 }
 
-// Row buffers in shared memory, filled by bulk copies several rows ahead, for
-// persistent blocks over rows that are whole 16-byte vectors.  With one row
-// ahead in registers an iteration takes a memory latency, and the rows that
-// two or three blocks have in flight are not enough to hide it.
-//
-// A team (the TPR threads of a row, or a warp with its 32 / TPR rows) has a
-// ring of its own: stage = N matrices x kPer rows.  Every wait is bounded; a
-// team that gave up goes on through its rows (its barriers stay matched)
-// and stores nothing.
-constexpr int kRingStages = 8;  // at most
+// Sixteen-byte vectors of a row held by TPR threads as pairs of FP32 values,
+// NE values a thread.  A warp's vectors are one contiguous slice of the row
+// (the whole row, when TPR < 32), vector after vector across its lanes.
+template <typename T, int TPR, int NE>
+struct PairTile {
+    static constexpr int kVec = 16 / (int)sizeof(T), kVecs = NE / kVec, kPairs = NE / 2;
+    static_assert(NE % kVec == 0, "whole vectors");
 
-template <typename T, int TPR, int THREADS, int N>
-struct RowRing {
-    static constexpr int kTeam = TPR < 32 ? 32 : TPR;
-    static constexpr int kTeams = THREADS / kTeam, kPer = kTeam / TPR;
-    static constexpr int kRows = kTeams * kPer;  // rows a block has at a time
-
-    const T *src[N];  // null: no such matrix (the last one only)
-    long long ld[N];
-    long long rows, first, step;  // the team's first row, and from one of its stages to the next
-    uint32_t row_bytes, stage_bytes, ring, bar0;
-    const uint8_t *ptr;
-    int n, stages, in_team;
-    Ring at{1};
-    volatile int *abort_flag;
-    int *error;
-    bool good = true;
-
-    // bars: [kTeams][kRingStages]; smem: kTeams * stages * stage bytes,
-    // 16-byte aligned.  Ends in a barrier of the block.
-    __device__ __forceinline__ void setup(uint8_t *smem, uint64_t *bars, int *abort_word, int *err,
-                                          long long rows_, int D, int stages_) {
-        const int team = threadIdx.x / kTeam;
-        in_team = threadIdx.x % kTeam;
-        n = src[N - 1] ? N : N - 1;
-        rows = rows_;
-        stages = stages_;
-        row_bytes = (uint32_t)D * sizeof(T);
-        stage_bytes = (uint32_t)(n * kPer) * row_bytes;
-        ring = smem_u32(smem) + (uint32_t)(team * stages) * stage_bytes;
-        ptr = smem + (size_t)(team * stages) * stage_bytes;
-        bar0 = smem_u32(bars + team * kRingStages);
-        first = (long long)blockIdx.x * kRows + team * kPer;
-        step = (long long)gridDim.x * kRows;
-        at = Ring(stages);
-        abort_flag = abort_word;
-        error = err;
-        if (threadIdx.x == 0) *abort_word = 0;
-        if (in_team == 0) {
-            for (int s = 0; s < stages; s++) mbar_init(bar0 + 8 * s, 1);
-            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        }
-        __syncthreads();
+    struct Raw {
+        uint4 u[kVecs];
+    };
+    static constexpr int kWide = TPR < 32 ? TPR : 32;    // threads of a slice
+    static constexpr int kSlice = kWide * NE;            // its values
+    static __device__ __forceinline__ int column(int i, int lane) {
+        return lane / kWide * kSlice + (i * kWide + lane % kWide) * kVec;
     }
-    // stage s takes rows r .. r + kPer - 1, as far as there are any
-    __device__ __forceinline__ void fill(int s, long long r) {
-        if (in_team >= 32 || r >= rows) return;
-        const int count = (int)min((long long)kPer, rows - r);
-        const uint32_t bar = bar0 + 8 * s, dst = ring + (uint32_t)s * stage_bytes;
-        if (in_team == 0) mbar_expect_tx(bar, (uint32_t)(n * count) * row_bytes);
-        __syncwarp();
-        if (in_team < count) {
+    // column of pair j's first value
+    static __device__ __forceinline__ int pair_column(int j, int lane) {
+        return column(j / (kVec / 2), lane) + j % (kVec / 2) * 2;
+    }
+    // from the slice in shared memory; what lies past D is zero
+    static __device__ __forceinline__ void load(Raw &r, const T *slice, int D, int lane) {
 #pragma unroll
-            for (int i = 0; i < N; i++)
-                if (i < n)
-                    bulk_load(dst + (uint32_t)(i * kPer + in_team) * row_bytes,
-                              src[i] + (r + in_team) * ld[i], row_bytes, bar);
+        for (int i = 0; i < kVecs; i++) {
+            r.u[i] = make_uint4(0, 0, 0, 0);
+            if (column(i, lane) < D)
+                r.u[i] = *reinterpret_cast<const uint4 *>(slice + (i * kWide + lane % kWide) * kVec);
         }
     }
-    __device__ __forceinline__ void start() {
-        for (int s = 0; s < stages; s++) fill(s, first + s * step);
+    // from the row in global memory
+    static __device__ __forceinline__ void load_row(Raw &r, const T *row, int D, int lane) {
+#pragma unroll
+        for (int i = 0; i < kVecs; i++) {
+            r.u[i] = make_uint4(0, 0, 0, 0);
+            if (column(i, lane) < D) r.u[i] = *reinterpret_cast<const uint4 *>(row + column(i, lane));
+        }
     }
-    __device__ __forceinline__ void wait() {
-        good &= mbar_wait_bounded(bar0 + 8 * at.i, at.ph, abort_flag, error);
+    static __device__ __forceinline__ void store(T *row, const Raw &r, int D, int lane) {
+#pragma unroll
+        for (int i = 0; i < kVecs; i++)
+            if (column(i, lane) < D) *reinterpret_cast<uint4 *>(row + column(i, lane)) = r.u[i];
     }
-    // the calling thread's row of matrix i in the present stage
-    __device__ __forceinline__ const T *row(int i) const {
-        return reinterpret_cast<const T *>(ptr + (size_t)at.i * stage_bytes +
-                                           (size_t)(i * kPer + in_team / TPR) * row_bytes);
+    static __device__ __forceinline__ uint32_t word(const Raw &r, int k) {
+        const uint4 u = r.u[k / 4];
+        return k % 4 == 0 ? u.x : k % 4 == 1 ? u.y : k % 4 == 2 ? u.z : u.w;
     }
-    // after a barrier of the team behind its last read of the stage at rows
-    // r0: filled again
-    __device__ __forceinline__ void refill(long long r0) { fill(at.i, r0 + stages * step); }
+    static __device__ __forceinline__ void set_word(Raw &r, int k, uint32_t v) {
+        uint4 &u = r.u[k / 4];
+        if (k % 4 == 0) u.x = v;
+        else if (k % 4 == 1) u.y = v;
+        else if (k % 4 == 2) u.z = v;
+        else u.w = v;
+    }
+    static __device__ __forceinline__ float2 pair(const Raw &r, int j) {
+        if constexpr (sizeof(T) == 2)
+            return unpack2<T>(word(r, j));
+        else
+            return make_float2(__uint_as_float(word(r, 2 * j)), __uint_as_float(word(r, 2 * j + 1)));
+    }
+    static __device__ __forceinline__ void set_pair(Raw &r, int j, float2 v) {
+        if constexpr (sizeof(T) == 2) {
+            set_word(r, j, pack2<T>(v.x, v.y));
+        } else {
+            set_word(r, 2 * j, __float_as_uint(v.x));
+            set_word(r, 2 * j + 1, __float_as_uint(v.y));
+        }
+    }
+    // parameters (weights) at the tile's columns, `none` where w is null
+    template <typename WT>
+    static __device__ __forceinline__ void load_params(float2 (&p)[kPairs], const WT *w, float none,
+                                                       int D, int lane) {
+#pragma unroll
+        for (int j = 0; j < kPairs; j++) {
+            const int c = pair_column(j, lane);
+            p[j] = make_float2(none, none);
+            if (w && c < D) p[j] = make_float2(to_float(w[c]), to_float(w[c + 1]));
+        }
+    }
 };
 
-// stages of a block's ring in `bytes` of shared memory
-inline int ring_stages(int bytes, int matrices, int rows, int D, int size) {
-    const long long stage = (long long)matrices * rows * D * size;
+// Rows (of whole 16-byte vectors) through rings of buffers in shared memory,
+// several rows ahead, by bulk copies.  With one row ahead in registers an
+// iteration takes a memory latency, and the rows that two or three blocks
+// have in flight are not enough to hide it.
+//
+// Every warp has a ring of its own for its slice of each row (Tile::kSlice
+// values; when TPR < 32 for 32 / TPR whole rows) and refills a stage as soon
+// as its lanes have read it: the copies' issue is spread evenly, and no
+// barrier between warps is needed.  A stage holds N matrices.  Every wait is
+// bounded; a thread that gave up goes on through its rows (barriers stay
+// matched) and stores nothing.
+constexpr int kRingStages = 8;  // at most
+
+template <typename T, int TPR, int NE, int THREADS, int N>
+struct RowRing {
+    using Tile = PairTile<T, TPR, NE>;
+    static constexpr int kPer = TPR < 32 ? 32 / TPR : 1;  // rows a warp has at a time
+    static constexpr int kRows = THREADS / TPR;           // rows a block has at a time
+    struct Shared {
+        uint64_t full[THREADS / 32][kRingStages];
+        int abort_word;
+    };
+    // Pointers and counts advance by additions: an instruction here is one for
+    // 32 * NE values only.
+    const T *next[N];           // what the lane copies next (lanes < kPer)
+    long long advance[N], step;  // from one stage to the next: in elements, in rows
+    long long first;            // the calling thread's first row
+    uint32_t bytes, slot, stage_bytes, full, ring;
+    const uint8_t *ptr;
+    int n, stages, lane, iters, fills, last_count, mine;
+    Ring at{1};
+    int *abort_flag, *error;
+    bool good = true;
+
+    // bytes of a stage of a block
+    static constexpr long long block_stage(int matrices, int D) {
+        return (long long)(THREADS / 32) * matrices * kPer *
+               (TPR < 32 ? D : Tile::kSlice) * (int)sizeof(T);
+    }
+
+    // src[i] null: no such matrix (the last one only).  smem: stages *
+    // block_stage() bytes, 16-byte aligned.  Ends in a barrier of the block.
+    __device__ __forceinline__ void setup(const T *const (&src)[N], const long long (&ld)[N],
+                                          uint8_t *smem, Shared *shared, int *err, long long rows,
+                                          int D, int stages_) {
+        const int warp = threadIdx.x / 32;
+        lane = threadIdx.x % 32;
+        n = src[N - 1] ? N : N - 1;
+        stages = stages_;
+        const int start_column = TPR < 32 ? 0 : threadIdx.x % TPR / 32 * Tile::kSlice;
+        const int values = TPR < 32 ? D : max(0, min(Tile::kSlice, D - start_column));
+        bytes = (uint32_t)values * sizeof(T);
+        slot = (uint32_t)(TPR < 32 ? D : Tile::kSlice) * sizeof(T);
+        stage_bytes = (uint32_t)(n * kPer) * slot;
+        const uint32_t at_byte = (uint32_t)(warp * stages) * stage_bytes;
+        ptr = smem + at_byte;
+        ring = smem_u32(smem) + at_byte;
+        full = smem_u32(shared->full[warp]);
+        abort_flag = &shared->abort_word;
+        error = err;
+        step = (long long)gridDim.x * kRows;
+        const long long warp_first =
+            (long long)blockIdx.x * kRows + (TPR < 32 ? warp * kPer : threadIdx.x / TPR);
+        // rows of the warp, and of the calling thread among them
+        iters = warp_first < rows ? (int)((rows - 1 - warp_first) / step) + 1 : 0;
+        last_count = (int)min((long long)kPer, rows - warp_first - (iters - 1) * step);
+        first = warp_first + (TPR < 32 ? lane / TPR : 0);
+        mine = first < rows ? (int)((rows - 1 - first) / step) + 1 : 0;
+        fills = 0;
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            next[i] = src[i] + (warp_first + (lane < kPer ? lane : 0)) * ld[i] + start_column;
+            advance[i] = step * ld[i];
+        }
+        at = Ring(stages);
+        if (lane == 0) {
+            for (int s = 0; s < stages; s++) mbar_init(full + 8 * s, 1);
+            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        }
+        if (threadIdx.x == 0) shared->abort_word = 0;
+        __syncthreads();
+    }
+    // stage s takes the slices of the warp's next rows, as far as there are any
+    __device__ __forceinline__ void fill(int s) {
+        if (fills >= iters || bytes == 0) return;
+        const uint32_t bar = full + 8 * s, dst = ring + (uint32_t)s * stage_bytes;
+        const int count = kPer == 1 ? 1 : fills == iters - 1 ? last_count : kPer;
+        if (lane == 0) mbar_expect_tx(bar, (uint32_t)(n * count) * bytes);
+        if (kPer > 1) __syncwarp();
+        if (lane < count) {
+#pragma unroll
+            for (int i = 0; i < N; i++)
+                if (i < n) bulk_load(dst + (uint32_t)(i * kPer + lane) * slot, next[i], bytes, bar);
+        }
+#pragma unroll
+        for (int i = 0; i < N; i++) next[i] += advance[i];
+        fills++;
+    }
+    __device__ __forceinline__ void start() {
+        for (int s = 0; s < stages; s++) fill(s);
+    }
+    __device__ __forceinline__ void wait() {
+        if (bytes) good &= mbar_wait_bounded(full + 8 * at.i, at.ph, abort_flag, error);
+    }
+    // the calling thread's slice of matrix i in the present stage
+    __device__ __forceinline__ const T *slice(int i) const {
+        return reinterpret_cast<const T *>(ptr + (uint32_t)at.i * stage_bytes +
+                                           (uint32_t)(i * kPer + lane / Tile::kWide) * slot);
+    }
+    // the warp has read the present stage into registers
+    __device__ __forceinline__ void refill() {
+        __syncwarp();
+        fill(at.i);
+    }
+};
+
+// stages of a block's rings in `bytes` of shared memory
+inline int ring_stages(long long bytes, long long stage) {
     const long long n = bytes / stage;
     return n > kRingStages ? kRingStages : (int)n;
 }
