@@ -90,6 +90,20 @@ __device__ __forceinline__ float2 sub2(float2 a, float2 b) {
 }
 __device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 
+// n / d for 0 <= n < 2^31 by a multiplication (Granlund and Montgomery,
+// "Division by invariant integers using multiplication", PLDI 1994)
+struct FastDiv {
+    uint32_t d = 1, mul = 1, shift = 0;
+    FastDiv() = default;
+    explicit FastDiv(uint32_t d_) : d(d_) {
+        while ((1ull << shift) < d) shift++;
+        mul = (uint32_t)((((1ull << shift) - d) << 32) / d + 1);
+    }
+    __device__ __forceinline__ int div(int n) const {
+        return (int)((__umulhi((uint32_t)n, mul) + (uint32_t)n) >> shift);
+    }
+};
+
 // f(T{}) with the C++ type of an element type
 template <typename F>
 inline Status with_type(int type, F f) {

@@ -83,20 +83,6 @@ constexpr uint32_t tmem_cols(int bt, int form) {
     return c < 32 ? 32 : c;
 }
 
-// n / d for 0 <= n < 2^31 by a multiplication (Granlund and Montgomery,
-// "Division by invariant integers using multiplication", PLDI 1994)
-struct FastDiv {
-    uint32_t d = 1, mul = 1, shift = 0;
-    FastDiv() = default;
-    explicit FastDiv(uint32_t d_) : d(d_) {
-        while ((1ull << shift) < d) shift++;
-        mul = (uint32_t)((((1ull << shift) - d) << 32) / d + 1);
-    }
-    __device__ __forceinline__ int div(int n) const {
-        return (int)((__umulhi((uint32_t)n, mul) + (uint32_t)n) >> shift);
-    }
-};
-
 struct Args {
     int M, N, kblocks;
     int f_tiles, t_tiles, tiles;

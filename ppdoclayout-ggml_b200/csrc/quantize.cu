@@ -79,9 +79,10 @@ struct AbsMax<__half> {
 
 // Rows of whole 16-byte vectors in registers.  The quotient is first taken
 // as x (1 / s), off by at most 127 x 2^-23 = 1.6e-5, and rounded by adding
-// 1.5 x 2^23, which leaves the whole number in the low byte; only a thread
-// with a value that close to a half decides on the remainders (about one in
-// a thousand).
+// 1.5 x 2^23, which leaves the whole number in the low byte.  Values that
+// close to a half decide on their remainders, pair by pair: in 16-bit rows
+// half the largest value (63.5 steps) alone makes them common, one in some
+// hundreds, so that most warps have one and few pairs do.
 template <typename T, int TPR, int NE>
 __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR)
 quantize_vector_kernel(const T *x, long long ldx, long long rows, int K, int8_t *q, long long ldq,
@@ -104,28 +105,40 @@ quantize_vector_kernel(const T *x, long long ldx, long long rows, int K, int8_t 
     if (!real) return;
     if (lane == 0) scale[row] = d.s;
     q += row * ldq;
-    const float2 inv = both(d.usable ? d.inv : 0.0f), magic = both(12582912.0f);
+    constexpr float kNear = 0.49998f;
+    const float2 inv = both(d.inv), magic = both(12582912.0f);
+    // the rounded pair's bits, and how far its quotients are from whole numbers
+    auto round_pair = [&](int j, float2 &m) {
+        const float2 t = mul2(Tile::pair(r, j), inv);
+        m = add2(t, magic);
+        const float2 off = add2(t, sub2(magic, m));
+        return fmaxf(fabsf(off.x), fabsf(off.y));
+    };
     float far = 0.0f;
     uint32_t out[NE / 4];
 #pragma unroll
     for (int j = 0; j < NE / 2; j += 2) {
-        const float2 t0 = mul2(Tile::pair(r, j), inv), t1 = mul2(Tile::pair(r, j + 1), inv);
-        const float2 m0 = add2(t0, magic), m1 = add2(t1, magic);
-        // how far each is from its whole number: at most 1/2
-        const float2 d0 = add2(t0, sub2(magic, m0)), d1 = add2(t1, sub2(magic, m1));
-        far = fmaxf(fmaxf(far, fmaxf(fabsf(d0.x), fabsf(d0.y))), fmaxf(fabsf(d1.x), fabsf(d1.y)));
+        float2 m0, m1;
+        far = fmaxf(far, round_pair(j, m0));
+        far = fmaxf(far, round_pair(j + 1, m1));
         const uint32_t lo = __byte_perm(__float_as_uint(m0.x), __float_as_uint(m0.y), 0x0040);
         const uint32_t hi = __byte_perm(__float_as_uint(m1.x), __float_as_uint(m1.y), 0x0040);
         out[j / 2] = __byte_perm(lo, hi, 0x5410);
     }
-    // (a row that is not usable has inv 0 and q 0; its NaNs and infinities
-    // give NaN here and are zeroed by the exact form)
-    if (!(far < 0.49998f) || d.up != 1.0f || !d.usable) {
+    auto exact_pair = [&](int j) {
+        const float2 v = Tile::pair(r, j);
+        const uint32_t b = (uint32_t)(d(v.x) & 255) | (uint32_t)(d(v.y) & 255) << 8;
+        out[j / 2] = __byte_perm(out[j / 2], b, j & 1 ? 0x5410 : 0x3254);
+    };
+    if (!d.usable || d.up != 1.0f) {
+        // zeros, infinities and NaNs, or a scale below 2^-64
 #pragma unroll
-        for (int j = 0; j < NE / 2; j += 2) {
-            const float2 a = Tile::pair(r, j), b = Tile::pair(r, j + 1);
-            out[j / 2] = (uint32_t)(d(a.x) & 255) | (uint32_t)(d(a.y) & 255) << 8 |
-                         (uint32_t)(d(b.x) & 255) << 16 | (uint32_t)(d(b.y) & 255) << 24;
+        for (int j = 0; j < NE / 2; j++) exact_pair(j);
+    } else if (far > kNear) {
+#pragma unroll
+        for (int j = 0; j < NE / 2; j++) {
+            float2 m;
+            if (round_pair(j, m) > kNear) exact_pair(j);
         }
     }
 #pragma unroll
@@ -236,6 +249,7 @@ Status launch_quantize_rows(const Rows &x, int type, long long rows, int K, int8
             if (K <= 128 * NE) return vectors(Int<128>{});
             if (K <= 256 * NE) return vectors(Int<256>{});
             if (K <= 512 * NE) return vectors(Int<512>{});
+            if (K <= 1024 * NE) return vectors(Int<1024>{});
         }
         if (K <= 64) return tile(Int<8>{}, Int<8>{});
         if (K <= 256) return tile(Int<32>{}, Int<8>{});
