@@ -335,6 +335,17 @@ PPDL_OPS_API int ppdl_linear_i8(const int8_t * q, long long ldq, const float * q
                                 int act, int M, int N, int K, void * y, long long ldy,
                                 void * stream);
 
+/* ppdl_quantize_rows_i8 of x [M][K] (x_type) into work, then ppdl_linear_i8
+   on it, in one call: the same bits as the two.  work:
+   ppdl_linear_i8_dynamic_workspace(M, K) bytes, 16-byte aligned, for this
+   call alone.  y may not be x. */
+PPDL_OPS_API int ppdl_linear_i8_dynamic(const void * x, long long ldx, int x_type,
+                                        const int8_t * w, long long ldw, const float * w_scale,
+                                        const float * bias, const void * res, long long ldres,
+                                        int type, int act, int M, int N, int K, void * y,
+                                        long long ldy, void * work, void * stream);
+PPDL_OPS_API long long ppdl_linear_i8_dynamic_workspace(int M, int K);
+
 /* Heads of ppdl_rotary: value d of head h of token t of sequence b lies at
    b*batch + t*token + h*head + d (elements). */
 typedef struct {

@@ -41,6 +41,31 @@ bool rows_ok(const void *p, long long ld, long long rows, int D, int type, bool 
     return aligned(p, ppdl::elem_size(type)) && (rows <= 1 || ld >= D);
 }
 
+// ppdl_linear_i8's checks, and its launch
+int linear_i8(const int8_t *q, long long ldq, const float *q_scale, const int8_t *w, long long ldw,
+              const float *w_scale, const float *bias, const void *res, long long ldres, int type,
+              int act, int M, int N, int K, void *y, long long ldy, void *stream, bool launch) {
+    ppdl::set_op_error("");
+    if (!ppdl::elem_type_ok(type) || act < 0 || act > 3)
+        return refuse("linear_i8: unknown element type or activation");
+    if (M < 0 || N <= 0 || K <= 0 || K > 131071) return refuse("linear_i8: bad sizes (K 1..131071)");
+    if (!rows_ok(y, ldy, M, N, type) || !rows_ok(res, ldres, M, N, type, true) ||
+        (M && (!q || !w || !q_scale || !w_scale)) || !aligned(q_scale, 4) || !aligned(w_scale, 4) ||
+        !aligned(bias, 4) || !aligned(q, 16) || !aligned(w, 16) ||
+        (M > 1 && (ldq < K || ldq % 16)) || (N > 1 && (ldw < K || ldw % 16)))
+        return refuse("linear_i8: null or misaligned pointer, rows closer than their width, or q / "
+                      "w rows not on 16-byte strides");
+    // a single row's stride is never stepped
+    if (M == 1) ldq = (K + 15LL) / 16 * 16;
+    if (N == 1) ldw = (K + 15LL) / 16 * 16;
+    ppdl::LinearI8Args a;
+    a.q = q; a.ldq = ldq; a.q_scale = q_scale; a.w = w; a.ldw = ldw; a.w_scale = w_scale;
+    a.bias = bias; a.res = {res, ldres}; a.y = {y, ldy};
+    a.type = type; a.act = act; a.M = M; a.N = N; a.K = K;
+    if (!launch) return PPDL_OK;
+    return status_of(ppdl::launch_linear_i8(a, (cudaStream_t)stream), "linear_i8: sizes too large");
+}
+
 }  // namespace
 
 extern "C" {
@@ -119,24 +144,40 @@ PPDL_OPS_API int ppdl_linear_i8(const int8_t *q, long long ldq, const float *q_s
                                 const float *bias, const void *res, long long ldres, int type,
                                 int act, int M, int N, int K, void *y, long long ldy,
                                 void *stream) {
+    return linear_i8(q, ldq, q_scale, w, ldw, w_scale, bias, res, ldres, type, act, M, N, K, y, ldy,
+                     stream, true);
+}
+
+namespace {
+// work: M rows of 8-bit values on 16-byte strides, then M scales
+long long row_bytes(int K) { return (K + 15LL) / 16 * 16; }
+long long scales_at(int M, int K) { return (long long)M * row_bytes(K); }
+}  // namespace
+
+PPDL_OPS_API long long ppdl_linear_i8_dynamic_workspace(int M, int K) {
+    if (M <= 0 || K <= 0) return 0;
+    return scales_at(M, K) + 4LL * M;
+}
+
+PPDL_OPS_API int ppdl_linear_i8_dynamic(const void *x, long long ldx, int x_type, const int8_t *w,
+                                        long long ldw, const float *w_scale, const float *bias,
+                                        const void *res, long long ldres, int type, int act, int M,
+                                        int N, int K, void *y, long long ldy, void *work,
+                                        void *stream) {
     ppdl::set_op_error("");
-    if (!ppdl::elem_type_ok(type) || act < 0 || act > 3)
-        return refuse("linear_i8: unknown element type or activation");
-    if (M < 0 || N <= 0 || K <= 0 || K > 131071) return refuse("linear_i8: bad sizes (K 1..131071)");
-    if (!rows_ok(y, ldy, M, N, type) || !rows_ok(res, ldres, M, N, type, true) ||
-        (M && (!q || !w || !q_scale || !w_scale)) || !aligned(q_scale, 4) || !aligned(w_scale, 4) ||
-        !aligned(bias, 4) || !aligned(q, 16) || !aligned(w, 16) ||
-        (M > 1 && (ldq < K || ldq % 16)) || (N > 1 && (ldw < K || ldw % 16)))
-        return refuse("linear_i8: null or misaligned pointer, rows closer than their width, or q / "
-                      "w rows not on 16-byte strides");
-    // a single row's stride is never stepped
-    if (M == 1) ldq = (K + 15LL) / 16 * 16;
-    if (N == 1) ldw = (K + 15LL) / 16 * 16;
-    ppdl::LinearI8Args a;
-    a.q = q; a.ldq = ldq; a.q_scale = q_scale; a.w = w; a.ldw = ldw; a.w_scale = w_scale;
-    a.bias = bias; a.res = {res, ldres}; a.y = {y, ldy};
-    a.type = type; a.act = act; a.M = M; a.N = N; a.K = K;
-    return status_of(ppdl::launch_linear_i8(a, (cudaStream_t)stream), "linear_i8: sizes too large");
+    if (M > 0 && (!work || !aligned(work, 16)))
+        return refuse("linear_i8_dynamic: null or misaligned workspace");
+    if (M < 0 || K <= 0) return refuse("linear_i8_dynamic: bad sizes");
+    int8_t *q = (int8_t *)work;
+    float *scale = (float *)(q + scales_at(M, K));
+    // the product's arguments are checked before the quantiser is launched
+    const int ok = linear_i8(q, row_bytes(K), scale, w, ldw, w_scale, bias, res, ldres, type, act,
+                             M, N, K, y, ldy, stream, false);
+    if (ok != PPDL_OK) return ok;
+    const int rc = ppdl_quantize_rows_i8(x, ldx, x_type, M, K, q, row_bytes(K), scale, stream);
+    if (rc != PPDL_OK) return rc;
+    return linear_i8(q, row_bytes(K), scale, w, ldw, w_scale, bias, res, ldres, type, act, M, N, K,
+                     y, ldy, stream, true);
 }
 
 PPDL_OPS_API int ppdl_rotary(const ppdl_rotary_heads *q, const ppdl_rotary_heads *k, int type,

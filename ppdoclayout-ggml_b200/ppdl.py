@@ -18,6 +18,7 @@ and every call fails loudly when the CUDA library is missing.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import os
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -375,34 +376,54 @@ def _declare_block_ops(L) -> None:
     L.ppdl_layernorm_backward_workspace.restype = ll
     L.ppdl_quantize_rows_i8.argtypes = [p, ll, i, ll, i, p, ll, p, p]
     L.ppdl_linear_i8.argtypes = [p, ll, p, p, ll, p, p, p, ll, i, i, i, i, i, p, ll, p]
+    L.ppdl_linear_i8_dynamic.argtypes = [p, ll, i, p, ll, p, p, p, ll, i, i, i, i, i, p, ll, p, p]
+    L.ppdl_linear_i8_dynamic_workspace.argtypes = [i, i]
+    L.ppdl_linear_i8_dynamic_workspace.restype = ll
     L.ppdl_rotary.argtypes = [p, p, i, i, i, i, i, p, i, ll, ll, ll, i, p, p, i, i, p]
 
 
-_types = {}
+# What the functions use of torch, bound by the first call (importing this
+# module does not import torch): a call's arguments are looked at in about
+# 3 us, with as few Python calls as that takes.
+_types, _tt = {}, {}
+
+
+def _bind() -> None:
+    import torch
+    lib()
+    _types.update({torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16})
+    # the current stream's handle without the object around it (2 us)
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+        (lambda i: torch.cuda.current_stream(i).cuda_stream)
+    _tt.update(f32=torch.float32, f64=torch.float64, i8=torch.int8,
+               integers=(torch.int32, torch.int64), empty_like=torch.empty_like, stream=raw,
+               current=torch.cuda.current_device, device=torch.cuda.device)
 
 
 def _type(t, name: str) -> int:
     """The PPDL_* element type of tensor t."""
     if not _types:
-        import torch
-        _types.update({torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16})
+        _bind()
     code = _types.get(t.dtype)
     if code is None:
         raise ValueError(f"{name} must be float32, bfloat16 or float16, not {t.dtype}")
     return code
 
 
-def _rows(t, name: str, width: int, like=None) -> int:
-    """The distance between the rows of width values that t [..., width]
-    consists of; t may be strided as long as its rows lie evenly apart."""
-    if t.dim() == 0 or t.shape[-1] != width or (like is not None and t.shape != like.shape):
-        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected "
-                         f"{tuple(like.shape) if like is not None else (..., width)}")
+def _rows(t, name: str, shape) -> int:
+    """The distance between the rows of shape[-1] values that t, of this
+    shape, consists of; t may be strided as long as its rows lie evenly
+    apart."""
+    if t.shape != shape:
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
+    width = shape[-1] if shape else 0
+    if width > 0x7fffffff or not shape:
+        raise ValueError(f"{name} must have rows of at most 2^31 - 1 values")
     if t.is_contiguous():
         return width
     ld = span = None
     if t.stride(-1) == 1 or width == 1:
-        for n, s in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
+        for n, s in zip(reversed(shape[:-1]), reversed(t.stride()[:-1])):
             if n == 1:
                 continue
             if ld is None:
@@ -413,37 +434,35 @@ def _rows(t, name: str, width: int, like=None) -> int:
         else:
             return width if ld is None else ld
     raise ValueError(f"{name} must consist of contiguous rows at one distance, "
-                     f"not strides {tuple(t.stride())} of shape {tuple(t.shape)}")
+                     f"not strides {tuple(t.stride())} of shape {tuple(shape)}")
 
 
 def _vector(t, name: str, n: int, dtype=None):
-    if t.dim() != 1 or t.shape[0] != n or (n > 1 and t.stride(0) != 1) or \
+    if t.dim() != 1 or t.numel() != n or not (n <= 1 or t.is_contiguous()) or \
             (dtype is not None and t.dtype != dtype):
         raise ValueError(f"{name} must be {n} contiguous values"
                          + (f" of {dtype}" if dtype is not None else ""))
 
 
-def _ptr(t):
-    return None if t is None else t.data_ptr()
+def _device(x, *others) -> int:
+    """The index of the GPU that x and the others (tensors or None) are on."""
+    index = x.get_device()
+    if index < 0:
+        raise ValueError(f"tensors on {x.device}: the operators take CUDA tensors")
+    for t in others:
+        if t is not None and t.get_device() != index:
+            raise ValueError(f"tensors on {x.device} and {t.device}")
+    return index
 
 
-def _call(fn, tensors, *args) -> None:
-    """fn(*args, stream) on the tensors' device, checked."""
-    import torch
-    dev = tensors[0].device
-    for t in tensors:
-        if t is not None and t.device != dev:
-            raise ValueError(f"tensors on {dev} and {t.device}")
-    if dev.type != "cuda":
-        raise ValueError(f"tensors on {dev}: the operators take CUDA tensors")
-    stream = torch.cuda.current_stream(dev).cuda_stream
-    if dev.index == torch.cuda.current_device():
-        status = fn(*args, stream)
-    else:
-        with torch.cuda.device(dev):
-            status = fn(*args, stream)
-    if status != PPDL_OK:
-        raise RuntimeError(f"{fn.__name__} failed ({status}): {last_error()}")
+def _elsewhere(index: int, f, *args, **kw):
+    """f on tensors of a GPU that is not the current one."""
+    with _tt["device"](index):
+        return f(*args, **kw)
+
+
+def _failed(fn, status: int):
+    raise RuntimeError(f"{fn.__name__} failed ({status}): {last_error()}")
 
 
 def layernorm(x, weight=None, bias=None, eps: float = 1e-5, *, residual=None,
@@ -453,36 +472,46 @@ def layernorm(x, weight=None, bias=None, eps: float = 1e-5, *, residual=None,
     of x's type or float32.  Returns y, followed by the sum (return_sum) and
     by the rows' mean and rstd in float32 (return_stats), which the backward
     pass takes."""
-    import torch
-    D = x.shape[-1] if x.dim() else 0
-    t = _type(x, "x")
-    ldx = _rows(x, "x", D)
-    ldr = 0
+    shape = x.shape
+    t = wt = _type(x, "x")
+    ldx = _rows(x, "x", shape)
+    D = shape[-1]
+    ldr, rp, wp, bp = 0, None, None, None
     if residual is not None:
-        ldr = _rows(residual, "residual", D, x)
         if residual.dtype != x.dtype:
             raise ValueError("residual must have x's type")
+        ldr, rp = _rows(residual, "residual", shape), residual.data_ptr()
     elif return_sum:
         raise ValueError("return_sum needs a residual")
-    wt = t
-    for v, name in ((weight, "weight"), (bias, "bias")):
-        if v is not None:
-            _vector(v, name, D)
-            wt = _type(v, name)
-    if weight is not None and bias is not None and weight.dtype != bias.dtype:
-        raise ValueError("weight and bias must have one type")
-    rows = x.numel() // D if D else 0
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    s = torch.empty(x.shape, dtype=x.dtype, device=x.device) if return_sum else None
-    mean = rstd = None
+    if weight is not None:
+        _vector(weight, "weight", D)
+        wt, wp = _type(weight, "weight"), weight.data_ptr()
+    if bias is not None:
+        _vector(bias, "bias", D)
+        wt, bp = _type(bias, "bias"), bias.data_ptr()
+        if weight is not None and weight.dtype != bias.dtype:
+            raise ValueError("weight and bias must have one type")
+    dev = _device(x, residual, weight, bias)
+    if dev != _tt["current"]():
+        return _elsewhere(dev, layernorm, x, weight, bias, eps, residual=residual,
+                          return_sum=return_sum, return_stats=return_stats)
+    # (empty_like keeps a dense x's strides, which are those of rows in order)
+    y = _tt["empty_like"](x)
+    s = mean = rstd = sp = mp = vp = None
+    if return_sum:
+        s = _tt["empty_like"](x)
+        sp = s.data_ptr()
     if return_stats:
-        mean = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
-        rstd = torch.empty_like(mean)
-    _call(lib().ppdl_layernorm, (x, residual, weight, bias), x.data_ptr(), ldx, _ptr(residual), ldr,
-          _ptr(weight), _ptr(bias), t, wt, rows, D, eps, y.data_ptr(), D, _ptr(s), D, _ptr(mean),
-          _ptr(rstd))
-    out = (y,) + ((s,) if return_sum else ()) + ((mean, rstd) if return_stats else ())
-    return out if len(out) > 1 else y
+        mean, rstd = x.new_empty((2,) + shape[:-1], dtype=_tt["f32"]).unbind(0)
+        mp, vp = mean.data_ptr(), rstd.data_ptr()
+    fn = _lib.ppdl_layernorm
+    status = fn(x.data_ptr(), ldx, rp, ldr, wp, bp, t, wt, x.numel() // D if D else 0, D, eps,
+                y.data_ptr(), D, sp, D, mp, vp, _tt["stream"](dev))
+    if status:
+        _failed(fn, status)
+    if not (return_sum or return_stats):
+        return y
+    return (y,) + ((s,) if return_sum else ()) + ((mean, rstd) if return_stats else ())
 
 
 def layernorm_backward(dy, x, weight, mean, rstd, *, dsum=None, param_grads: bool = True):
@@ -492,33 +521,37 @@ def layernorm_backward(dy, x, weight, mean, rstd, *, dsum=None, param_grads: boo
     reaches the sum on its other path; dx is then the gradient of x and of
     the residual alike.  dweight and dbias have weight's type (x's without a
     weight) and are None without param_grads."""
-    import torch
-    D = x.shape[-1] if x.dim() else 0
-    t = _type(x, "x")
-    ldx, lddy = _rows(x, "x", D), _rows(dy, "dy", D, x)
-    ldds = _rows(dsum, "dsum", D, x) if dsum is not None else 0
+    shape = x.shape
+    t = wt = _type(x, "x")
+    ldx, lddy = _rows(x, "x", shape), _rows(dy, "dy", shape)
+    D, lead, f32 = shape[-1], shape[:-1], _tt["f32"]
+    ldds, dsp, wp = 0, None, None
+    if dsum is not None:
+        ldds, dsp = _rows(dsum, "dsum", shape), dsum.data_ptr()
     if dy.dtype != x.dtype or (dsum is not None and dsum.dtype != x.dtype):
         raise ValueError("dy and dsum must have x's type")
-    wt = t
     if weight is not None:
         _vector(weight, "weight", D)
-        wt = _type(weight, "weight")
-    rows = x.numel() // D if D else 0
+        wt, wp = _type(weight, "weight"), weight.data_ptr()
     for v, name in ((mean, "mean"), (rstd, "rstd")):
-        if v.dtype != torch.float32 or v.shape != x.shape[:-1] or not v.is_contiguous():
-            raise ValueError(f"{name} must be contiguous float32 of shape {tuple(x.shape[:-1])}")
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    dw = db = work = None
-    L = lib()
+        if v.dtype != f32 or v.shape != lead or not v.is_contiguous():
+            raise ValueError(f"{name} must be contiguous float32 of shape {tuple(lead)}")
+    dev = _device(x, dy, weight, mean, rstd, dsum)
+    if dev != _tt["current"]():
+        return _elsewhere(dev, layernorm_backward, dy, x, weight, mean, rstd, dsum=dsum,
+                          param_grads=param_grads)
+    rows = x.numel() // D if D else 0
+    dx = _tt["empty_like"](x)
+    dw = db = dwp = dbp = wsp = None
     if param_grads:
-        grads = torch.empty((2, D), dtype=x.dtype if weight is None else weight.dtype,
-                            device=x.device)
-        dw, db = grads[0], grads[1]
-        work = torch.empty(L.ppdl_layernorm_backward_workspace(rows, D), dtype=torch.float32,
-                           device=x.device)
-    _call(L.ppdl_layernorm_backward, (x, dy, weight, mean, rstd, dsum), dy.data_ptr(), lddy,
-          x.data_ptr(), ldx, _ptr(weight), mean.data_ptr(), rstd.data_ptr(), _ptr(dsum), ldds, t,
-          wt, rows, D, dx.data_ptr(), D, _ptr(dw), _ptr(db), _ptr(work))
+        dw, db = (x if weight is None else weight).new_empty((2, D)).unbind(0)
+        work = mean.new_empty(_lib.ppdl_layernorm_backward_workspace(rows, D))
+        dwp, dbp, wsp = dw.data_ptr(), db.data_ptr(), work.data_ptr()
+    fn = _lib.ppdl_layernorm_backward
+    status = fn(dy.data_ptr(), lddy, x.data_ptr(), ldx, wp, mean.data_ptr(), rstd.data_ptr(), dsp,
+                ldds, t, wt, rows, D, dx.data_ptr(), D, dwp, dbp, wsp, _tt["stream"](dev))
+    if status:
+        _failed(fn, status)
     return dx, dw, db
 
 
@@ -527,16 +560,22 @@ def quantize_rows(x):
     int8 [..., K], rows on strides of a multiple of 16 bytes, and scale
     float32 [...]: q * scale[..., None] stands for x.  It quantises weights
     [N, K] channel by channel and activations token by token."""
-    import torch
-    K = x.shape[-1] if x.dim() else 0
+    shape = x.shape
     t = _type(x, "x")
-    ldx = _rows(x, "x", K)
+    ldx = _rows(x, "x", shape)
+    K, lead = shape[-1], shape[:-1]
     ldq = (K + 15) // 16 * 16
-    q = torch.empty(x.shape[:-1] + (ldq,), dtype=torch.int8, device=x.device)
-    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
-    _call(lib().ppdl_quantize_rows_i8, (x,), x.data_ptr(), ldx, t, x.numel() // K if K else 0, K,
-          q.data_ptr(), ldq, scale.data_ptr())
-    return q[..., :K], scale
+    dev = _device(x)
+    if dev != _tt["current"]():
+        return _elsewhere(dev, quantize_rows, x)
+    q = x.new_empty(lead + (ldq,), dtype=_tt["i8"])
+    scale = x.new_empty(lead, dtype=_tt["f32"])
+    fn = _lib.ppdl_quantize_rows_i8
+    status = fn(x.data_ptr(), ldx, t, x.numel() // K if K else 0, K, q.data_ptr(), ldq,
+                scale.data_ptr(), _tt["stream"](dev))
+    if status:
+        _failed(fn, status)
+    return q if ldq == K else q[..., :K], scale
 
 
 def linear_i8(x, weight, w_scale, *, x_scale=None, bias=None, act: str = "none", residual=None,
@@ -548,55 +587,69 @@ def linear_i8(x, weight, w_scale, *, x_scale=None, bias=None, act: str = "none",
     none, relu, silu or gelu; residual [..., N] of the result's type, which is
     x's (for int8 x: residual's, else float32) unless out_dtype says
     otherwise."""
-    import torch
-    if weight.dim() != 2 or weight.dtype != torch.int8:
+    if not _types:
+        _bind()
+    wshape, shape, i8, f32 = weight.shape, x.shape, _tt["i8"], _tt["f32"]
+    if len(wshape) != 2 or weight.dtype != i8:
         raise ValueError("weight must be int8 [N, K]")
-    N, K = weight.shape
-    if act not in ACTS:
+    N, K = wshape
+    code = ACTS.get(act)
+    if code is None:
         raise ValueError(f"act must be one of {', '.join(ACTS)}")
-    ldw = _rows(weight, "weight", K)
-    ldx = _rows(x, "x", K)
-    _vector(w_scale, "w_scale", N, torch.float32)
+    lead = shape[:-1]
+    ldw, ldx = _rows(weight, "weight", wshape), _rows(x, "x", lead + (K,))
+    _vector(w_scale, "w_scale", N, f32)
+    bp = rp = None
     if bias is not None:
-        _vector(bias, "bias", N, torch.float32)
-    lead = x.shape[:-1]
-    M = x.numel() // K if K else 0
-    if x.dtype == torch.int8:
-        if x_scale is None or x_scale.dtype != torch.float32 or x_scale.shape != lead or \
+        _vector(bias, "bias", N, f32)
+        bp = bias.data_ptr()
+    if x.dtype == i8:
+        if x_scale is None or x_scale.dtype != f32 or x_scale.shape != lead or \
                 not x_scale.is_contiguous():
             raise ValueError(f"int8 x needs x_scale, contiguous float32 of shape {tuple(lead)}")
-        dtype = out_dtype or (torch.float32 if residual is None else residual.dtype)
+        dtype = out_dtype or (f32 if residual is None else residual.dtype)
+    elif x_scale is not None:
+        raise ValueError("x_scale goes with int8 x")
     else:
-        if x_scale is not None:
-            raise ValueError("x_scale goes with int8 x")
+        xt = _type(x, "x")
         dtype = out_dtype or x.dtype
-    y = torch.empty(lead + (N,), dtype=dtype, device=x.device)
+    dev = _device(x, x_scale, weight, w_scale, bias, residual)
+    if dev != _tt["current"]():
+        return _elsewhere(dev, linear_i8, x, weight, w_scale, x_scale=x_scale, bias=bias, act=act,
+                          residual=residual, out_dtype=out_dtype)
+    y = x.new_empty(lead + (N,), dtype=dtype)
     t = _type(y, "the result")
     ldr = 0
     if residual is not None:
-        ldr = _rows(residual, "residual", N, y)
         if residual.dtype != dtype:
             raise ValueError("residual must have the result's type")
-    L = lib()
-    if x_scale is None:
-        q = torch.empty((M, (K + 15) // 16 * 16), dtype=torch.int8, device=x.device)
-        x_scale = torch.empty(M, dtype=torch.float32, device=x.device)
-        _call(L.ppdl_quantize_rows_i8, (x,), x.data_ptr(), ldx, _type(x, "x"), M, K, q.data_ptr(),
-              q.shape[1], x_scale.data_ptr())
-        x, ldx = q, q.shape[1]
-    _call(L.ppdl_linear_i8, (x, x_scale, weight, w_scale, bias, residual), x.data_ptr(), ldx,
-          x_scale.data_ptr(), weight.data_ptr(), ldw, w_scale.data_ptr(), _ptr(bias),
-          _ptr(residual), ldr, t, ACTS[act], M, N, K, y.data_ptr(), N)
+        ldr, rp = _rows(residual, "residual", y.shape), residual.data_ptr()
+    M = x.numel() // K if K else 0
+    if M > 0x7fffffff or N > 0x7fffffff:
+        raise ValueError(f"{M} rows and {N} channels: each must fit 31 bits")
+    if x_scale is not None:
+        fn = _lib.ppdl_linear_i8
+        status = fn(x.data_ptr(), ldx, x_scale.data_ptr(), weight.data_ptr(), ldw,
+                    w_scale.data_ptr(), bp, rp, ldr, t, code, M, N, K, y.data_ptr(), N,
+                    _tt["stream"](dev))
+    else:
+        work = weight.new_empty(M * ((K + 15) // 16 * 16 + 4))  # ..._dynamic_workspace(M, K)
+        fn = _lib.ppdl_linear_i8_dynamic
+        status = fn(x.data_ptr(), ldx, xt, weight.data_ptr(), ldw, w_scale.data_ptr(), bp, rp, ldr,
+                    t, code, M, N, K, y.data_ptr(), N, work.data_ptr(), _tt["stream"](dev))
+    if status:
+        _failed(fn, status)
     return y
 
 
-def _heads(x, out, name: str, dim: int, like):
-    if x.dim() != 4 or x.shape[3] != dim or x.shape[:2] != like.shape[:2] or x.dtype != like.dtype:
+def _heads(x, out, name: str, lead, dim: int, dtype):
+    shape = x.shape
+    if len(shape) != 4 or shape[3] != dim or shape[:2] != lead or x.dtype != dtype:
         raise ValueError(f"{name} must be [batch, length, heads, {dim}] of one type")
-    if dim > 1 and x.stride(3) != 1:
-        raise ValueError(f"{name}'s heads must be contiguous")
     i, o = x.stride(), out.stride()
-    return RotaryHeads(x.data_ptr(), out.data_ptr(), x.shape[2], i[0], i[1], i[2], o[0], o[1], o[2])
+    if dim > 1 and i[3] != 1:
+        raise ValueError(f"{name}'s heads must be contiguous")
+    return RotaryHeads(x.data_ptr(), out.data_ptr(), shape[2], *i[:3], *o[:3])
 
 
 def rotary(q, k, positions, freq, sections, *, interleaved: bool = False, inverse: bool = False,
@@ -608,24 +661,35 @@ def rotary(q, k, positions, freq, sections, *, interleaved: bool = False, invers
     [rotated / 2] in radians per position turns the first `rotated` values of
     every head; sections says how many consecutive pairs each axis turns.
     inverse turns back: the backward pass."""
-    import torch
-    dim = q.shape[-1] if q.dim() else 0
     t = _type(q, "q")
-    if positions.dtype not in (torch.int32, torch.int64) or positions.dim() != 3 or \
-            positions.shape[0] != len(sections) or positions.shape[1:] != q.shape[:2]:
+    lead, dim = q.shape[:2], q.shape[-1] if q.dim() else 0
+    axes, pshape = len(sections), positions.shape
+    if positions.dtype not in _tt["integers"] or len(pshape) != 3 or pshape[0] != axes or \
+            pshape[1:] != lead:
         raise ValueError("positions must be int32 or int64 [axes, batch, length], one axis a section")
-    if freq.dtype != torch.float64 or freq.dim() != 1 or not freq.is_contiguous():
+    if freq.dtype != _tt["f64"] or freq.dim() != 1 or not freq.is_contiguous():
         raise ValueError("freq must be contiguous float64 [rotated / 2]")
-    qo = q if inplace else torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    hq = _heads(q, qo, "q", dim, q)
-    ko = hk = None
+    dev = _device(q, k, positions, freq)
+    if dev != _tt["current"]():
+        return _elsewhere(dev, rotary, q, k, positions, freq, sections, interleaved=interleaved,
+                          inverse=inverse, inplace=inplace)
+    # (empty_like keeps a dense tensor's strides, whichever their order)
+    qo, ko, hk = q if inplace else _tt["empty_like"](q), None, None
+    hq = _heads(q, qo, "q", lead, dim, q.dtype)
     if k is not None:
-        ko = k if inplace else torch.empty(k.shape, dtype=k.dtype, device=k.device)
-        hk = _heads(k, ko, "k", dim, q)
-    ps = positions.stride()
-    _call(lib().ppdl_rotary, (q, k, positions, freq), C.byref(hq),
-          C.byref(hk) if hk is not None else None, t, q.shape[0], q.shape[1], dim,
-          2 * freq.shape[0], positions.data_ptr(), positions.element_size(), ps[0], ps[1], ps[2],
-          len(sections), (C.c_int32 * len(sections))(*sections), freq.data_ptr(), int(interleaved),
-          int(inverse))
+        ko = k if inplace else _tt["empty_like"](k)
+        hk = C.byref(_heads(k, ko, "k", lead, dim, q.dtype))
+    if lead[0] > 0x7fffffff or lead[1] > 0x7fffffff:
+        raise ValueError("batch and length must fit 31 bits")
+    fn = _lib.ppdl_rotary
+    status = fn(C.byref(hq), hk, t, *lead, dim, 2 * freq.numel(), positions.data_ptr(),
+                positions.element_size(), *positions.stride(), axes, _sections(tuple(sections)),
+                freq.data_ptr(), interleaved, inverse, _tt["stream"](dev))
+    if status:
+        _failed(fn, status)
     return qo, ko
+
+
+@functools.lru_cache(maxsize=64)
+def _sections(sections):
+    return (C.c_int32 * len(sections))(*sections)
