@@ -161,15 +161,14 @@ layernorm_ring_kernel(const T *x, long long ldx, const T *res, long long ldres, 
     for (int it = 0; it < ring.iters; it++, ring.at.next()) {
         ring.wait();
         typename Tile::Raw r;
-        Tile::load(r, ring.slice(0), D, lane);
+        Tile::load(r, ring.row(0), D, lane);
         if (res) {
             typename Tile::Raw q;
-            Tile::load(q, ring.slice(1), D, lane);
+            Tile::load(q, ring.row(1), D, lane);
 #pragma unroll
             for (int j = 0; j < NE / 2; j++)
                 Tile::set_pair(r, j, add2(Tile::pair(r, j), Tile::pair(q, j)));
         }
-        ring.refill();
         float2 v[NE / 2], t = both(0.0f);
 #pragma unroll
         for (int j = 0; j < NE / 2; j++) {
@@ -180,6 +179,7 @@ layernorm_ring_kernel(const T *x, long long ldx, const T *res, long long ldres, 
         if (sum && real) Tile::store(sum, r, D, lane);
         float s[1] = {t.x + t.y};
         team_sums<TPR>(s, sh[0], team);
+        ring.refill();
         const float mean = s[0] * inv_d;
         t = both(0.0f);
 #pragma unroll
@@ -429,9 +429,9 @@ layernorm_bwd_ring_kernel(const T *dy, long long lddy, const T *x, long long ldx
         typename Tile::Raw rx, rdy, out;
         float2 g[NE / 2], t0 = both(0.0f), t1 = both(0.0f);
         if (real) {
-            Tile::load(rx, ring.slice(0), D, lane);
-            Tile::load(rdy, ring.slice(1), D, lane);
-            if (dsum) Tile::load(out, ring.slice(2), D, lane);
+            Tile::load(rx, ring.row(0), D, lane);
+            Tile::load(rdy, ring.row(1), D, lane);
+            if (dsum) Tile::load(out, ring.row(2), D, lane);
 #pragma unroll
             for (int j = 0; j < NE / 2; j++) {
                 const float2 xh = fma2(Tile::pair(rx, j), both(r), both(mr));
@@ -443,9 +443,9 @@ layernorm_bwd_ring_kernel(const T *dy, long long lddy, const T *x, long long ldx
                 t1 = fma2(g[j], xh, t1);
             }
         }
-        ring.refill();
         float s[2] = {t0.x + t0.y, t1.x + t1.y};
         team_sums<TPR>(s, sh[it & 1], team);
+        ring.refill();
         const float2 m1 = both(-s[0] * inv_d * r), m2 = both(-s[1] * inv_d * r);
         if (real && ring.good) {
 #pragma unroll

@@ -97,7 +97,7 @@ quantize_vector_kernel(const T *x, long long ldx, long long rows, int K, int8_t 
     const bool real = row < rows;
     if (!real) row = rows - 1;
     typename Tile::Raw r;
-    Tile::load_row(r, x + row * ldx, K, lane);
+    Tile::load(r, x + row * ldx, K, lane);
     AbsMax<T> most;
 #pragma unroll
     for (int k = 0; k < kWords; k++) most.add(Tile::word(r, k));

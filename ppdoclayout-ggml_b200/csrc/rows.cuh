@@ -164,8 +164,7 @@ __device__ __forceinline__ void team_sums(float (&v)[N], float *sh, int team) {
 }
 
 // Sixteen-byte vectors of a row held by TPR threads as pairs of FP32 values,
-// NE values a thread.  A warp's vectors are one contiguous slice of the row
-// (the whole row, when TPR < 32), vector after vector across its lanes.
+// NE values a thread: vectors lane, lane + TPR, ...
 template <typename T, int TPR, int NE>
 struct PairTile {
     static constexpr int kVec = 16 / (int)sizeof(T), kVecs = NE / kVec, kPairs = NE / 2;
@@ -174,26 +173,13 @@ struct PairTile {
     struct Raw {
         uint4 u[kVecs];
     };
-    static constexpr int kWide = TPR < 32 ? TPR : 32;    // threads of a slice
-    static constexpr int kSlice = kWide * NE;            // its values
-    static __device__ __forceinline__ int column(int i, int lane) {
-        return lane / kWide * kSlice + (i * kWide + lane % kWide) * kVec;
-    }
+    static __device__ __forceinline__ int column(int i, int lane) { return (i * TPR + lane) * kVec; }
     // column of pair j's first value
     static __device__ __forceinline__ int pair_column(int j, int lane) {
         return column(j / (kVec / 2), lane) + j % (kVec / 2) * 2;
     }
-    // from the slice in shared memory; what lies past D is zero
-    static __device__ __forceinline__ void load(Raw &r, const T *slice, int D, int lane) {
-#pragma unroll
-        for (int i = 0; i < kVecs; i++) {
-            r.u[i] = make_uint4(0, 0, 0, 0);
-            if (column(i, lane) < D)
-                r.u[i] = *reinterpret_cast<const uint4 *>(slice + (i * kWide + lane % kWide) * kVec);
-        }
-    }
-    // from the row in global memory
-    static __device__ __forceinline__ void load_row(Raw &r, const T *row, int D, int lane) {
+    // what lies past D is zero
+    static __device__ __forceinline__ void load(Raw &r, const T *row, int D, int lane) {
 #pragma unroll
         for (int i = 0; i < kVecs; i++) {
             r.u[i] = make_uint4(0, 0, 0, 0);
@@ -248,29 +234,31 @@ struct PairTile {
 // iteration takes a memory latency, and the rows that two or three blocks
 // have in flight are not enough to hide it.
 //
-// Every warp has a ring of its own for its slice of each row (Tile::kSlice
-// values; when TPR < 32 for 32 / TPR whole rows) and refills a stage as soon
-// as its lanes have read it: the copies' issue is spread evenly, and no
-// barrier between warps is needed.  A stage holds N matrices.  Every wait is
-// bounded; a thread that gave up goes on through its rows (barriers stay
-// matched) and stores nothing.
+// A team (the TPR threads of a row, or a warp with its 32 / TPR rows) has a
+// ring of its own; a stage holds N matrices' rows.  A stage is refilled
+// behind a barrier of the team, by one of its warps in turn, so that the
+// copies' issue is neither on one warp's path nor repeated by all (slices of
+// a row for every warp cost the backward pass 8 %).  Every wait is bounded; a
+// thread that gave up goes on through its rows (barriers stay matched) and
+// stores nothing.
 constexpr int kRingStages = 8;  // at most
 
 template <typename T, int TPR, int NE, int THREADS, int N>
 struct RowRing {
     using Tile = PairTile<T, TPR, NE>;
-    static constexpr int kPer = TPR < 32 ? 32 / TPR : 1;  // rows a warp has at a time
-    static constexpr int kRows = THREADS / TPR;           // rows a block has at a time
+    static constexpr int kTeam = TPR < 32 ? 32 : TPR, kTeams = THREADS / kTeam;
+    static constexpr int kPer = kTeam / TPR;     // rows a team has at a time
+    static constexpr int kRows = THREADS / TPR;  // rows a block has at a time
     struct Shared {
-        uint64_t full[THREADS / 32][kRingStages];
+        uint64_t full[kTeams][kRingStages];
         int abort_word;
     };
     // Pointers and counts advance by additions: an instruction here is one for
     // 32 * NE values only.
-    const T *next[N];           // what the lane copies next (lanes < kPer)
+    const T *next[N];            // what the lane copies next (lanes < kPer)
     long long advance[N], step;  // from one stage to the next: in elements, in rows
-    long long first;            // the calling thread's first row
-    uint32_t bytes, slot, stage_bytes, full, ring;
+    long long first;             // the calling thread's first row
+    uint32_t row_bytes, stage_bytes, full, ring;
     const uint8_t *ptr;
     int n, stages, lane, iters, fills, last_count, mine;
     Ring at{1};
@@ -279,8 +267,7 @@ struct RowRing {
 
     // bytes of a stage of a block
     static constexpr long long block_stage(int matrices, int D) {
-        return (long long)(THREADS / 32) * matrices * kPer *
-               (TPR < 32 ? D : Tile::kSlice) * (int)sizeof(T);
+        return (long long)kRows * matrices * D * (int)sizeof(T);
     }
 
     // src[i] null: no such matrix (the last one only).  smem: stages *
@@ -288,54 +275,54 @@ struct RowRing {
     __device__ __forceinline__ void setup(const T *const (&src)[N], const long long (&ld)[N],
                                           uint8_t *smem, Shared *shared, int *err, long long rows,
                                           int D, int stages_) {
-        const int warp = threadIdx.x / 32;
+        const int team = threadIdx.x / kTeam;
         lane = threadIdx.x % 32;
         n = src[N - 1] ? N : N - 1;
         stages = stages_;
-        const int start_column = TPR < 32 ? 0 : threadIdx.x % TPR / 32 * Tile::kSlice;
-        const int values = TPR < 32 ? D : max(0, min(Tile::kSlice, D - start_column));
-        bytes = (uint32_t)values * sizeof(T);
-        slot = (uint32_t)(TPR < 32 ? D : Tile::kSlice) * sizeof(T);
-        stage_bytes = (uint32_t)(n * kPer) * slot;
-        const uint32_t at_byte = (uint32_t)(warp * stages) * stage_bytes;
+        row_bytes = (uint32_t)D * sizeof(T);
+        stage_bytes = (uint32_t)(n * kPer) * row_bytes;
+        const uint32_t at_byte = (uint32_t)(team * stages) * stage_bytes;
         ptr = smem + at_byte;
         ring = smem_u32(smem) + at_byte;
-        full = smem_u32(shared->full[warp]);
+        full = smem_u32(shared->full[team]);
         abort_flag = &shared->abort_word;
         error = err;
         step = (long long)gridDim.x * kRows;
-        const long long warp_first =
-            (long long)blockIdx.x * kRows + (TPR < 32 ? warp * kPer : threadIdx.x / TPR);
-        // rows of the warp, and of the calling thread among them
-        iters = warp_first < rows ? (int)((rows - 1 - warp_first) / step) + 1 : 0;
-        last_count = (int)min((long long)kPer, rows - warp_first - (iters - 1) * step);
-        first = warp_first + (TPR < 32 ? lane / TPR : 0);
+        const long long team_first = (long long)blockIdx.x * kRows + team * kPer;
+        // rows of the team, and of the calling thread among them
+        iters = team_first < rows ? (int)((rows - 1 - team_first) / step) + 1 : 0;
+        last_count = (int)min((long long)kPer, rows - team_first - (iters - 1) * step);
+        first = team_first + (TPR < 32 ? lane / TPR : 0);
         mine = first < rows ? (int)((rows - 1 - first) / step) + 1 : 0;
         fills = 0;
 #pragma unroll
         for (int i = 0; i < N; i++) {
-            next[i] = src[i] + (warp_first + (lane < kPer ? lane : 0)) * ld[i] + start_column;
+            next[i] = src[i] + (team_first + (lane < kPer ? lane : 0)) * ld[i];
             advance[i] = step * ld[i];
         }
         at = Ring(stages);
-        if (lane == 0) {
+        if (threadIdx.x % kTeam == 0) {
             for (int s = 0; s < stages; s++) mbar_init(full + 8 * s, 1);
             asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         }
         if (threadIdx.x == 0) shared->abort_word = 0;
         __syncthreads();
     }
-    // stage s takes the slices of the warp's next rows, as far as there are any
+    // stage s takes the team's next rows, as far as there are any
     __device__ __forceinline__ void fill(int s) {
-        if (fills >= iters || bytes == 0) return;
-        const uint32_t bar = full + 8 * s, dst = ring + (uint32_t)s * stage_bytes;
-        const int count = kPer == 1 ? 1 : fills == iters - 1 ? last_count : kPer;
-        if (lane == 0) mbar_expect_tx(bar, (uint32_t)(n * count) * bytes);
-        if (kPer > 1) __syncwarp();
-        if (lane < count) {
+        if (fills >= iters) return;
+        if (TPR <= 32 || fills % (kTeam / 32) == (int)threadIdx.x % kTeam / 32) {
+            const uint32_t bar = full + 8 * s, dst = ring + (uint32_t)s * stage_bytes;
+            const int count = kPer == 1 ? 1 : fills == iters - 1 ? last_count : kPer;
+            if (lane == 0) mbar_expect_tx(bar, (uint32_t)(n * count) * row_bytes);
+            if (kPer > 1) __syncwarp();
+            if (lane < count) {
 #pragma unroll
-            for (int i = 0; i < N; i++)
-                if (i < n) bulk_load(dst + (uint32_t)(i * kPer + lane) * slot, next[i], bytes, bar);
+                for (int i = 0; i < N; i++)
+                    if (i < n)
+                        bulk_load(dst + (uint32_t)(i * kPer + lane) * row_bytes, next[i], row_bytes,
+                                  bar);
+            }
         }
 #pragma unroll
         for (int i = 0; i < N; i++) next[i] += advance[i];
@@ -345,16 +332,17 @@ struct RowRing {
         for (int s = 0; s < stages; s++) fill(s);
     }
     __device__ __forceinline__ void wait() {
-        if (bytes) good &= mbar_wait_bounded(full + 8 * at.i, at.ph, abort_flag, error);
+        good &= mbar_wait_bounded(full + 8 * at.i, at.ph, abort_flag, error);
     }
-    // the calling thread's slice of matrix i in the present stage
-    __device__ __forceinline__ const T *slice(int i) const {
+    // the calling thread's row of matrix i in the present stage
+    __device__ __forceinline__ const T *row(int i) const {
         return reinterpret_cast<const T *>(ptr + (uint32_t)at.i * stage_bytes +
-                                           (uint32_t)(i * kPer + lane / Tile::kWide) * slot);
+                                           (uint32_t)(i * kPer + (TPR < 32 ? lane / TPR : 0)) *
+                                               row_bytes);
     }
-    // the warp has read the present stage into registers
+    // behind a barrier of the team after its last read of the present stage
     __device__ __forceinline__ void refill() {
-        __syncwarp();
+        if (TPR <= 32) __syncwarp();
         fill(at.i);
     }
 };
