@@ -64,15 +64,83 @@ __global__ void layernorm_row_kernel(const T *x, long long ldx, const T *res, lo
     }
 }
 
-// Rows in registers: TPR threads hold a row of at most TPR * NE values, a
-// block has as many rows as fit 128 threads (one, when TPR is more).  One pass
-// over memory.
-template <typename T, typename WT, int TPR, int NE, bool VEC>
+// Rows of whole 16-byte vectors in registers: TPR threads hold a row of at
+// most TPR * NE values, a block has as many rows as fit 128 threads (one,
+// when TPR is more).  One pass over memory.
+template <typename T, typename WT, int TPR, int NE>
+__global__ void __launch_bounds__(TPR < 128 ? 128 : TPR)
+layernorm_vector_kernel(const T *x, long long ldx, const T *res, long long ldres, T *y,
+                        long long ldy, T *sum, long long ldsum, const WT *w, const WT *b,
+                        float *mean_out, float *rstd_out, long long rows, int D, float eps) {
+    using Tile = PairTile<T, TPR, NE>;
+    pdl_begin();
+    pdl_trigger();
+    __shared__ float sh[2][32];
+    constexpr int kRows = TPR < 128 ? 128 / TPR : 1, kHalf = Tile::kVec / 2;
+    const int lane = threadIdx.x % TPR;
+    long long row = (long long)blockIdx.x * kRows + threadIdx.x / TPR;
+    // rows past the end repeat the last one (its threads take part in the
+    // shuffles) and store nothing
+    const bool real = row < rows;
+    if (!real) row = rows - 1;
+    typename Tile::Raw r;
+    Tile::load(r, x + row * ldx, D, lane);
+    if (res) {
+        typename Tile::Raw q;
+        Tile::load(q, res + row * ldres, D, lane);
+#pragma unroll
+        for (int j = 0; j < NE / 2; j++)
+            Tile::set_pair(r, j, add2(Tile::pair(r, j), Tile::pair(q, j)));
+    }
+    float2 t = both(0.0f);
+#pragma unroll
+    for (int j = 0; j < NE / 2; j++) t = add2(t, Tile::pair(r, j));
+    float s[1] = {t.x + t.y};
+    row_sums<TPR>(s, sh[0]);
+    const float mean = s[0] / (float)D;
+    t = both(0.0f);
+#pragma unroll
+    for (int i = 0; i < Tile::kVecs; i++)
+        // a vector past D holds zeros and takes no part
+        if (Tile::column(i, lane) < D) {
+#pragma unroll
+            for (int j = i * kHalf; j < (i + 1) * kHalf; j++) {
+                const float2 v = add2(Tile::pair(r, j), both(-mean));
+                t = fma2(v, v, t);
+            }
+        }
+    s[0] = t.x + t.y;
+    row_sums<TPR>(s, sh[1]);
+    const float rstd = rsqrtf(s[0] / (float)D + eps);
+    if (!real) return;
+    if (sum) Tile::store(sum + row * ldsum, r, D, lane);
+    const bool wide_w = sizeof(WT) * Tile::kVec >= 16 && ((uintptr_t)w & 15) == 0;
+    const bool wide_b = sizeof(WT) * Tile::kVec >= 16 && ((uintptr_t)b & 15) == 0;
+#pragma unroll
+    for (int i = 0; i < Tile::kVecs; i++) {
+        float2 pw[kHalf], pb[kHalf];
+        Tile::vector_params(pw, w, 1.0f, i, D, lane, wide_w);
+        Tile::vector_params(pb, b, 0.0f, i, D, lane, wide_b);
+#pragma unroll
+        for (int k = 0; k < kHalf; k++) {
+            const float2 v = add2(Tile::pair(r, i * kHalf + k), both(-mean));
+            Tile::set_pair(r, i * kHalf + k, fma2(mul2(v, both(rstd)), pw[k], pb[k]));
+        }
+    }
+    Tile::store(y + row * ldy, r, D, lane);
+    if (lane == 0) {
+        if (mean_out) mean_out[row] = mean;
+        if (rstd_out) rstd_out[row] = rstd;
+    }
+}
+
+// The same for rows of any alignment, value by value.
+template <typename T, typename WT, int TPR, int NE>
 __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR)
 layernorm_tile_kernel(const T *x, long long ldx, const T *res, long long ldres, T *y,
                       long long ldy, T *sum, long long ldsum, const WT *w, const WT *b,
                       float *mean_out, float *rstd_out, long long rows, int D, float eps) {
-    using Tile = RowTile<T, TPR, NE, VEC>;
+    using Tile = RowTile<T, TPR, NE>;
     pdl_begin();
     pdl_trigger();
     __shared__ float sh[2][32];
@@ -126,9 +194,12 @@ layernorm_tile_kernel(const T *x, long long ldx, const T *res, long long ldres, 
 __device__ int g_row_error = 0;
 
 // Persistent blocks with their rows coming through rings in shared memory
-// (RowRing), weights and biases in registers: for many rows of whole 16-byte
-// vectors.  What bounds a 16-bit row is instructions, so a thread has 64 bytes
-// of it: sums, barrier and ring cost a warp about 100 instructions a row.
+// (RowRing), weights and biases in registers: for many wide 16-bit rows of
+// whole 16-byte vectors.  8192 x 4096 BF16 take 30.1 us, 68 % of copy
+// bandwidth: what bounds them is the chain of a row (two sums over 8 warps,
+// about 270 instructions a warp) with two rows on an SM at a time; more rows
+// in smaller registers spilled, and a load from local memory queues behind
+// the stores to y.
 constexpr int ring_threads(int tpr) { return tpr < 256 ? 256 : tpr; }
 constexpr int ring_blocks(int tpr) { return tpr > 256 ? 1 : 2; }
 template <typename T, typename WT, int TPR, int NE>
@@ -270,13 +341,13 @@ __global__ void layernorm_dw_column_kernel(const T *dy, long long lddy, const T 
 // loaded while the present ones are summed.  part[block][2][D] takes the
 // block's sums (null: no weights' gradients).
 constexpr int bwd_threads(int tpr) { return tpr < 256 ? 256 : tpr; }
-template <typename T, typename WT, int TPR, int NE, bool VEC>
+template <typename T, typename WT, int TPR, int NE>
 __global__ void __launch_bounds__(bwd_threads(TPR), TPR > 256 ? 1 : 2)
 layernorm_bwd_tile_kernel(const T *dy, long long lddy, const T *x, long long ldx, const T *dsum,
                           long long lddsum, T *dx, long long lddx, const WT *w,
                           const float *mean_in, const float *rstd_in, long long rows, int D,
                           float *part) {
-    using Tile = RowTile<T, TPR, NE, VEC>;
+    using Tile = RowTile<T, TPR, NE>;
     constexpr int kThreads = bwd_threads(TPR), kRows = kThreads / TPR;
     __shared__ float sh[2][kThreads / 32 * 2];
     __shared__ float red[kRows > 1 ? kThreads * NE : 1];
@@ -573,11 +644,14 @@ Status launch_layernorm(const LayerNormArgs &a, cudaStream_t st) {
                          vector_rows(a.res.p, a.res.ld, a.rows, a.D, size) &&
                          vector_rows(a.y.p, a.y.ld, a.rows, a.D, size) &&
                          vector_rows(a.sum.p, a.sum.ld, a.rows, a.D, size);
-        auto tile = [&](auto tpr, auto ne) {
+        auto tile = [&](auto tpr, auto ne, auto vector) {
             constexpr int TPR = decltype(tpr)::value, NE = decltype(ne)::value;
             constexpr int kThreads = TPR < 128 ? 128 : TPR;
-            auto kernel = vec ? layernorm_tile_kernel<T, WT, TPR, NE, true>
-                              : layernorm_tile_kernel<T, WT, TPR, NE, false>;
+            constexpr bool VEC = decltype(vector)::value != 0;
+            auto kernel = [&] {
+                if constexpr (VEC) return layernorm_vector_kernel<T, WT, TPR, NE>;
+                else return layernorm_tile_kernel<T, WT, TPR, NE>;
+            }();
             pdl_launch(kernel, (unsigned)cdiv(a.rows, kThreads / TPR), kThreads, 0, st,
                        (const T *)a.x.p, a.x.ld, (const T *)a.res.p, a.res.ld, ptr<T>(a.y), a.y.ld,
                        ptr<T>(a.sum), a.sum.ld, (const WT *)a.weight, (const WT *)a.bias, a.mean,
@@ -603,21 +677,34 @@ Status launch_layernorm(const LayerNormArgs &a, cudaStream_t st) {
                        a.rstd, a.rows, a.D, a.eps, stages);
             return true;
         };
-        // FP32 rows fill the bandwidth from the tile kernel's blocks (52500 x
-        // 256 with a residual 33.7 us, by the ring 36.9) unless they are short
-        // (100000 x 96: 22.5 / 13.2); 16-bit ones gain (8192 x 4096 34 / 30)
-        if (vec && (sizeof(T) == 2 || a.D <= 128) && ring_dispatch<kRingNE>(a.D, ring))
-            return cuda_status();
-        // the smallest tile that holds the row, 64 bytes a thread
+        // wide 16-bit rows gain from the rings (16384 x 2000 28.8 us, 31.6
+        // without; 4096 x 8192 33.0 / 36.8); shorter ones do not (20000 x 768
+        // 17.9 / 16.2), nor do FP32 ones (52500 x 256 36.9 / 33.7)
+        if constexpr (sizeof(T) == 2) {
+            if (vec && a.D > 1024 &&
+                (a.D <= 2048 ? ring(Int<128>{}) : a.D <= 4096 ? ring(Int<256>{})
+                 : a.D <= 8192 ? ring(Int<512>{}) : false))
+                return cuda_status();
+        }
+        // the smallest tile that holds the row, 64 bytes a thread (rows up to
+        // 256 values half of that)
         constexpr int NE = sizeof(T) == 2 ? 32 : 16, F = sizeof(T) == 2 ? 1 : 2;
-        if (a.D <= 64) return tile(Int<4>{}, Int<16>{});
-        if (a.D <= 256) return tile(Int<16>{}, Int<16>{});
-        if (a.D <= 512) return tile(Int<16 * F>{}, Int<NE>{});
-        if (a.D <= 1024) return tile(Int<32 * F>{}, Int<NE>{});
-        if (a.D <= 2048) return tile(Int<64 * F>{}, Int<NE>{});
-        if (a.D <= 4096) return tile(Int<128 * F>{}, Int<NE>{});
-        if (a.D <= 8192) return tile(Int<256 * F>{}, Int<NE>{});
-        if (a.D <= 16384) return tile(Int<512 * F>{}, Int<NE>{});
+        auto any = [&](auto v) {
+            bool some = true;
+            if (a.D <= 64) tile(Int<4>{}, Int<16>{}, v);
+            else if (a.D <= 128) tile(Int<8>{}, Int<16>{}, v);
+            else if (a.D <= 256) tile(Int<16>{}, Int<16>{}, v);
+            else if (a.D <= 512) tile(Int<16 * F>{}, Int<NE>{}, v);
+            else if (a.D <= 1024) tile(Int<32 * F>{}, Int<NE>{}, v);
+            else if (a.D <= 2048) tile(Int<64 * F>{}, Int<NE>{}, v);
+            else if (a.D <= 4096) tile(Int<128 * F>{}, Int<NE>{}, v);
+            else if (a.D <= 8192) tile(Int<256 * F>{}, Int<NE>{}, v);
+            else if (a.D <= 16384) tile(Int<512 * F>{}, Int<NE>{}, v);
+            else if (a.D <= 1024 * NE && sizeof(T) == 2) tile(Int<1024>{}, Int<NE>{}, v);
+            else some = false;
+            return some;
+        };
+        if (vec ? any(Int<1>{}) : any(Int<0>{})) return cuda_status();
         pdl_launch(layernorm_row_kernel<T, WT>, (unsigned)a.rows, 512, 0, st,
                    (const T *)a.x.p, a.x.ld, (const T *)a.res.p, a.res.ld, ptr<T>(a.y), a.y.ld,
                    ptr<T>(a.sum), a.sum.ld, (const WT *)a.weight, (const WT *)a.bias, a.mean,
@@ -647,7 +734,7 @@ Status launch_layernorm_backward(const LayerNormBackwardArgs &a, cudaStream_t st
         auto tile = [&](auto tpr, auto ne) {
             constexpr int TPR = decltype(tpr)::value, NE = decltype(ne)::value;
             constexpr int kThreads = bwd_threads(TPR), kRows = kThreads / TPR;
-            auto kernel = layernorm_bwd_tile_kernel<T, WT, TPR, NE, false>;
+            auto kernel = layernorm_bwd_tile_kernel<T, WT, TPR, NE>;
             const int most = TPR > 256 ? kMaxParts / 2 : kMaxParts;
             const long long blocks = (a.rows + kRows - 1) / kRows;
             parts = (int)(blocks < most ? blocks : most);

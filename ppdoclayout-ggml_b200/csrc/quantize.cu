@@ -158,7 +158,7 @@ template <typename T, int TPR, int NE>
 __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR)
 quantize_tile_kernel(const T *x, long long ldx, long long rows, int K, int8_t *q, long long ldq,
                      float *scale) {
-    using Tile = RowTile<T, TPR, NE, false, 4>;
+    using Tile = RowTile<T, TPR, NE, 4>;
     pdl_begin();
     pdl_trigger();
     __shared__ unsigned sh[32];

@@ -14,84 +14,46 @@ namespace ppdl {
 template <int V>
 using Int = std::integral_constant<int, V>;
 
-// TPR threads hold one row of at most TPR * NE values, NE each.  VEC: rows
-// start on 16 bytes and D is a whole number of 16-byte vectors, a thread
-// holds vectors lane, lane + TPR, ...; else single elements, grouped by
-// GROUP neighbours (1: consecutive lanes read consecutive elements).
-template <typename T, int TPR, int NE, bool VEC, int GROUP = 1>
+// TPR threads hold one row of at most TPR * NE values, NE each, value by
+// value (any alignment): neighbours in groups of GROUP (1: consecutive lanes
+// hold consecutive values).
+template <typename T, int TPR, int NE, int GROUP = 1>
 struct RowTile {
-    static constexpr int kVec = VEC ? 16 / (int)sizeof(T) : GROUP;
-    static constexpr int kVecs = NE / kVec;
-    static_assert(NE % kVec == 0, "whole vectors");
+    static constexpr int kVec = GROUP, kVecs = NE / GROUP;
+    static_assert(NE % GROUP == 0, "whole groups");
 
     struct Raw {
         T v[NE];
     };
 
-    // column of the first value of vector i
+    // column of the first value of group i
     static __device__ __forceinline__ int column(int i, int lane) {
-        return (i * TPR + lane) * kVec;
+        return (i * TPR + lane) * GROUP;
     }
     static __device__ __forceinline__ void load(Raw &r, const T *row, int D, int lane) {
 #pragma unroll
-        for (int i = 0; i < kVecs; i++) {
-            const int c = column(i, lane);
-            if constexpr (VEC) {
-                uint4 u = make_uint4(0, 0, 0, 0);
-                if (c < D) u = *reinterpret_cast<const uint4 *>(row + c);
-                *reinterpret_cast<uint4 *>(&r.v[i * kVec]) = u;
-            } else {
-#pragma unroll
-                for (int e = 0; e < kVec; e++) {
-                    r.v[i * kVec + e] = from_float<T>(0.0f);
-                    if (c + e < D) r.v[i * kVec + e] = row[c + e];
-                }
-            }
+        for (int j = 0; j < NE; j++) {
+            r.v[j] = from_float<T>(0.0f);
+            if (inside(j, D, lane)) r.v[j] = row[column(j / GROUP, lane) + j % GROUP];
         }
     }
     static __device__ __forceinline__ void store(T *row, const Raw &r, int D, int lane) {
 #pragma unroll
-        for (int i = 0; i < kVecs; i++) {
-            const int c = column(i, lane);
-            if constexpr (VEC) {
-                if (c < D)
-                    *reinterpret_cast<uint4 *>(row + c) =
-                        *reinterpret_cast<const uint4 *>(&r.v[i * kVec]);
-            } else {
-#pragma unroll
-                for (int e = 0; e < kVec; e++)
-                    if (c + e < D) row[c + e] = r.v[i * kVec + e];
-            }
-        }
+        for (int j = 0; j < NE; j++)
+            if (inside(j, D, lane)) row[column(j / GROUP, lane) + j % GROUP] = r.v[j];
     }
     // true for value j of the tile inside the row
     static __device__ __forceinline__ bool inside(int j, int D, int lane) {
-        return column(j / kVec, lane) + (VEC ? 0 : j % kVec) < D;
+        return column(j / GROUP, lane) + j % GROUP < D;
     }
-    // NE values of a vector of parameters (weights) of type WT at the tile's
-    // columns, `none` where w is null; any alignment of w's element type
+    // parameters (weights) at the tile's columns, `none` where w is null
     template <typename WT>
     static __device__ __forceinline__ void load_params(float (&p)[NE], const WT *w, float none,
                                                        int D, int lane) {
 #pragma unroll
-        for (int i = 0; i < kVecs; i++) {
-            const int c = column(i, lane);
-#pragma unroll
-            for (int e = 0; e < kVec; e++) p[i * kVec + e] = none;
-            if (!w) continue;
-            constexpr int kBytes = kVec * (int)sizeof(WT);
-            if (VEC && kBytes >= 16 && c < D && ((uintptr_t)w & 15) == 0) {
-                WT u[kVec];
-#pragma unroll
-                for (int b = 0; b < kBytes / 16; b++)
-                    reinterpret_cast<uint4 *>(u)[b] = reinterpret_cast<const uint4 *>(w + c)[b];
-#pragma unroll
-                for (int e = 0; e < kVec; e++) p[i * kVec + e] = to_float(u[e]);
-            } else {
-#pragma unroll
-                for (int e = 0; e < kVec; e++)
-                    if (c + e < D) p[i * kVec + e] = to_float(w[c + e]);
-            }
+        for (int j = 0; j < NE; j++) {
+            p[j] = none;
+            if (w && inside(j, D, lane)) p[j] = to_float(w[column(j / GROUP, lane) + j % GROUP]);
         }
     }
 };
@@ -216,6 +178,39 @@ struct PairTile {
             set_word(r, 2 * j + 1, __float_as_uint(v.y));
         }
     }
+    // the parameters (weights) of vector i, `none` where w is null; `wide`: w
+    // is 16-byte aligned and a vector of it is at least as long
+    template <typename WT>
+    static __device__ __forceinline__ void vector_params(float2 (&p)[kVec / 2], const WT *w,
+                                                         float none, int i, int D, int lane,
+                                                         bool wide) {
+        const int c = column(i, lane);
+#pragma unroll
+        for (int k = 0; k < kVec / 2; k++) p[k] = make_float2(none, none);
+        if (!w || c >= D) return;
+        constexpr int kBytes = kVec * (int)sizeof(WT);
+        if constexpr (kBytes >= 16) {
+            if (wide) {
+#pragma unroll
+                for (int h = 0; h < kBytes / 16; h++) {
+                    const uint4 u = reinterpret_cast<const uint4 *>(w + c)[h];
+                    if constexpr (sizeof(WT) == 2) {
+                        p[4 * h] = unpack2<WT>(u.x);
+                        p[4 * h + 1] = unpack2<WT>(u.y);
+                        p[4 * h + 2] = unpack2<WT>(u.z);
+                        p[4 * h + 3] = unpack2<WT>(u.w);
+                    } else {
+                        p[2 * h] = make_float2(__uint_as_float(u.x), __uint_as_float(u.y));
+                        p[2 * h + 1] = make_float2(__uint_as_float(u.z), __uint_as_float(u.w));
+                    }
+                }
+                return;
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < kVec / 2; k++)
+            p[k] = make_float2(to_float(w[c + 2 * k]), to_float(w[c + 2 * k + 1]));
+    }
     // parameters (weights) at the tile's columns, `none` where w is null
     template <typename WT>
     static __device__ __forceinline__ void load_params(float2 (&p)[kPairs], const WT *w, float none,
@@ -237,8 +232,9 @@ struct PairTile {
 // A team (the TPR threads of a row, or a warp with its 32 / TPR rows) has a
 // ring of its own; a stage holds N matrices' rows.  A stage is refilled
 // behind a barrier of the team, by one of its warps in turn, so that the
-// copies' issue is neither on one warp's path nor repeated by all (slices of
-// a row for every warp cost the backward pass 8 %).  Every wait is bounded; a
+// copies' issue is neither on one warp's path nor repeated by all (with a
+// slice of the row for every warp the backward pass of 16384 x 4096 BF16 took
+// 95 us, so 84.4).  Every wait is bounded; a
 // thread that gave up goes on through its rows (barriers stay matched) and
 // stores nothing.
 constexpr int kRingStages = 8;  // at most
