@@ -84,7 +84,7 @@ struct AbsMax<__half> {
 // half the largest value (63.5 steps) alone makes them common, one in some
 // hundreds, so that most warps have one and few pairs do.
 template <typename T, int TPR, int NE>
-__global__ void __launch_bounds__(TPR < 128 ? 128 : TPR)
+__global__ void __launch_bounds__(TPR < 128 ? 128 : TPR, 1024 / (TPR < 128 ? 128 : TPR))
 quantize_vector_kernel(const T *x, long long ldx, long long rows, int K, int8_t *q, long long ldq,
                        float *scale) {
     using Tile = PairTile<T, TPR, NE>;
