@@ -56,6 +56,10 @@ struct LinearI8Args {
     int M = 0, N = 0, K = 0;
 };
 Status launch_linear_i8(const LinearI8Args &a, cudaStream_t st);
+// The same on rows x of x_type in place of q, quantised in the kernel: for a
+// few short rows (false: not these, nothing was launched).
+bool launch_linear_i8_few(const Rows &x, int x_type, const LinearI8Args &a, cudaStream_t st,
+                          Status *status);
 // its device error flag, as tc_error_fetch_and_clear()
 int linear_error_fetch_and_clear();
 

@@ -28,6 +28,11 @@
 // up its share of the tokens over its peers and finishes it.  Integer sums
 // do not depend on the order, so both forms give the same bits.
 //
+// One or two tokens in 16 or 32 bits are quantised by the split form itself:
+// while its weights are on their way, every CTA finds the rows' largest
+// values and quantises its own k-blocks into shared memory, which saves a
+// launch.
+//
 // Every mbarrier wait is bounded; on expiry the kernel raises a device error
 // flag, all roles drain out and TMEM is released (ppdl_op_device_error).
 #include <cuda.h>
@@ -35,6 +40,7 @@
 #include "block.cuh"
 #include "block.h"
 #include "gemm_tc.h"
+#include "quantize.cuh"
 #include "tc_ptx.cuh"
 
 namespace ppdl {
@@ -78,6 +84,12 @@ constexpr int stages(int bt, int form) {
 constexpr int smem_bytes(int bt, int form) {
     return kCtrlBytes + 1024 + stages(bt, form) * stage_bytes(bt, form);
 }
+// the quantising form: a ring of weights alone, and this CTA's k-blocks of
+// quantised tokens behind it
+constexpr int kFuseBlocks = 16;
+constexpr int fuse_smem(int bt) {
+    return kCtrlBytes + 1024 + stages(bt, SPLIT) * kABytes + kFuseBlocks * bt * kBK;
+}
 constexpr uint32_t tmem_cols(int bt, int form) {
     const int c = form == SPLIT ? bt : 2 * bt;
     return c < 32 ? 32 : c;
@@ -94,6 +106,9 @@ struct Args {
     const void *res;
     void *y;
     long long ldres, ldy;
+    const void *x;  // quantising form: M rows of K values
+    long long ldx;
+    int K;
 };
 
 __device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity, volatile int *abort_flag) {
@@ -190,7 +205,8 @@ __device__ __forceinline__ void tile_of(const Args &a, int tile, int &ft, int &t
     tt = g * kGroup + r - ft * width;
 }
 
-// What follows the sum.  acc is rounded to FP32 (2^-24 relative), the two
+// What follows the sum, with every rounding written out (the residual's sum
+// by __fadd_rn as well), so that all forms give the same bits.  acc is rounded to FP32 (2^-24 relative), the two
 // scales are multiplied first (they are the same for a whole row or column).
 template <int C, int ACT>
 __device__ __forceinline__ void finish_all(float (&v)[C], const uint32_t (&acc)[C], const float *sx,
@@ -246,7 +262,8 @@ __device__ __forceinline__ void epilogue_chunk(const Args &a, const uint32_t (&a
                 if constexpr (RES) {
                     const float other = __shfl_xor_sync(0xffffffffu, odd ? v[j] : v[j + 1], 1);
                     const float2 rr = unpack2<T>(r[j / 2]);
-                    out = pack2<T>((odd ? other : v[j]) + rr.x, (odd ? v[j + 1] : other) + rr.y);
+                    out = pack2<T>(__fadd_rn(odd ? other : v[j], rr.x),
+                                   __fadd_rn(odd ? v[j + 1] : other, rr.y));
                 } else {
                     // already at its last rounding: exchange the packed pair
                     // (token j in the low half), then take one half of each
@@ -273,7 +290,7 @@ __device__ __forceinline__ void epilogue_chunk(const Args &a, const uint32_t (&a
     T *yp = (T *)a.y + (long long)t0 * a.ldy + n;
 #pragma unroll
     for (int j = 0; j < C; j++, yp += a.ldy) {
-        const T out = from_float<T>(RES ? v[j] + to_float(r[RES ? j : 0]) : v[j]);
+        const T out = from_float<T>(RES ? __fadd_rn(v[j], to_float(r[RES ? j : 0])) : v[j]);
         if (!EDGE || j < mine) *yp = out;
     }
 }
@@ -302,14 +319,89 @@ __device__ __forceinline__ void epilogue_any(const Args &a, const uint32_t (&acc
     }
 }
 
-template <typename T, int BT, int FORM>
+// The calling 8 warps quantise k-blocks kb0 .. kb0 + kbn - 1 of the a.M <= BT
+// rows of a.x into `to` ([k-block][BT rows of 128 bytes], 128-byte swizzle:
+// 16-byte chunk c of row r at chunk c ^ (r & 7)) and the rows' scales into
+// `scale`; amax is scratch for BT words.  Rows past M are left as they are:
+// no output depends on them.
+template <typename X, int BT>
+__device__ __forceinline__ void quantize_slice(const Args &a, int kb0, int kbn, uint8_t *to,
+                                               float *scale, unsigned *amax) {
+    constexpr int kThreads = 256, kBar = 1;
+    const int tid = threadIdx.x - 32 * kWarpEpi;
+    auto sync = [] { asm volatile("bar.sync %0, %1;" ::"n"(kBar), "n"(kThreads) : "memory"); };
+    const X *x = (const X *)a.x;
+    constexpr int V = 16 / (int)sizeof(X);
+    const bool vec = ((uintptr_t)x & 15) == 0 && a.K % V == 0 && (a.M == 1 || a.ldx % V == 0);
+    // a unit: sixteen neighbouring values of a row; the thread's first unit is
+    // loaded before the rows' largest values are known
+    const int per_row = kbn * 8, units = a.M * per_row;
+    X v[16];
+    auto load = [&](int u) {
+        const int r = u / per_row, k = kb0 * kBK + (u - r * per_row) * 16;
+        const X *row = x + (long long)r * a.ldx + k;
+        if (vec && k + 16 <= a.K) {
+#pragma unroll
+            for (int i = 0; i < 16 / V; i++)
+                reinterpret_cast<uint4 *>(v)[i] = reinterpret_cast<const uint4 *>(row)[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                v[i] = from_float<X>(0.0f);
+                if (k + i < a.K) v[i] = row[i];
+            }
+        }
+    };
+    if (tid < units) load(tid);
+    if (tid < BT) amax[tid] = 0;
+    sync();
+    for (int r = 0; r < a.M; r++) {
+        const X *row = x + (long long)r * a.ldx;
+        unsigned m = 0;
+        if (vec) {
+            for (int c = tid * V; c < a.K; c += kThreads * V) {
+                const uint4 w = *reinterpret_cast<const uint4 *>(row + c);
+                const X *e = reinterpret_cast<const X *>(&w);
+#pragma unroll
+                for (int i = 0; i < V; i++) m = max(m, __float_as_uint(fabsf(to_float(e[i]))));
+            }
+        } else {
+            for (int c = tid; c < a.K; c += kThreads)
+                m = max(m, __float_as_uint(fabsf(to_float(row[c]))));
+        }
+        m = __reduce_max_sync(0xffffffffu, m);
+        if ((tid & 31) == 0) atomicMax(&amax[r], m);
+    }
+    sync();
+    for (int u = tid; u < units; u += kThreads) {
+        if (u != tid) load(u);
+        const int r = u / per_row, at = u - r * per_row, kb = at / 8, c = at % 8;
+        const Divisor d(amax[r]);
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            w[i] = 0;
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                w[i] |= (uint32_t)(d(to_float(v[4 * i + e])) & 255) << (8 * e);
+        }
+        *reinterpret_cast<uint4 *>(to + kb * (BT * kBK) + r * kBK + ((c ^ (r & 7)) * 16)) =
+            make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    if (tid < a.M) scale[tid] = Divisor(amax[tid]).s;
+}
+
+// X: int8_t, or the type of the rows that the split form quantises itself.
+template <typename T, int BT, int FORM, typename X = int8_t>
 __global__ void __launch_bounds__(threads(BT, FORM), FORM == SPLIT ? 2 : 1)
 linear_i8_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmQ,
                  const __grid_constant__ Args a) {
     constexpr int S = stages(BT, FORM), kAcc = FORM == SPLIT ? 1 : 2;
     constexpr int kEpiWarps = epi_warps(BT, FORM), kLoadT = load_tokens(BT, FORM);
     constexpr int kTileF = FORM == PAIR ? 2 * kFeat : kFeat;  // channels per tile
-    constexpr uint32_t kStage = stage_bytes(BT, FORM), kCols = tmem_cols(BT, FORM);
+    constexpr bool FUSE = sizeof(X) > 1;
+    static_assert(!FUSE || FORM == SPLIT, "only the split form quantises");
+    constexpr uint32_t kStage = FUSE ? kABytes : stage_bytes(BT, FORM), kCols = tmem_cols(BT, FORM);
     extern __shared__ uint8_t smem_raw[];
     const uint32_t ctrl = smem_u32(smem_raw);
     // full[s]: a stage's bytes landed (pair: both CTAs', in the leader);
@@ -333,10 +425,11 @@ linear_i8_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
         for (int i = 0; i < 2; i++) {
             mbar_init(bar_tfull + 8 * i, 1);
             mbar_init(bar_tempty + 8 * i, FORM == PAIR ? 2 * kEpiWarps : kEpiWarps);
-            mbar_init(bar_sfull + 8 * i, 1);
+            if (!FUSE) mbar_init(bar_sfull + 8 * i, 1);
             mbar_init(bar_sempty + 8 * i, kEpiWarps);
         }
         mbar_init(bar_done, 1);
+        if (FUSE) mbar_init(bar_sfull, kEpiWarps);  // the tokens are quantised
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -362,7 +455,7 @@ linear_i8_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
     const uint32_t tmem = *tmem_slot;
     if (warp == kWarpTma && lane == 0) {
         prefetch_tensor_map(&tmW);
-        prefetch_tensor_map(&tmQ);
+        if (!FUSE) prefetch_tensor_map(&tmQ);
     }
     pdl_begin();
     pdl_trigger();
@@ -398,7 +491,7 @@ linear_i8_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
                         const uint32_t fb = bar_full + 8 * rs.i;
                         mbar_expect_tx(fb, kStage);
                         tma_load_2d(st, &tmW, fb, k, ft * kTileF);
-                        tma_load_2d(st + kABytes, &tmQ, fb, k, tt * BT);
+                        if constexpr (!FUSE) tma_load_2d(st + kABytes, &tmQ, fb, k, tt * BT);
                     }
                 }
             }
@@ -425,6 +518,7 @@ linear_i8_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
             bool ok = true;
             for (int tile = first; tile < a.tiles && ok; tile += step, ra.next()) {
                 if (!wait_for(bar_tempty + 8 * ra.i, ra.ph ^ 1, abort_flag)) break;
+                if (FUSE && !wait_for(bar_sfull, 0, abort_flag)) break;
                 tc_fence_after();
                 const uint32_t d = tmem + (uint32_t)(ra.i * BT);
                 for (int kb = 0; kb < kbn; kb++, rs.next()) {
@@ -437,7 +531,8 @@ linear_i8_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
                     // a K = 32 step is 32 bytes into the swizzled row: +2 in the
                     // descriptors' start address
                     const uint64_t da = smem_desc(st, 16, 1024, 2);
-                    const uint64_t db = smem_desc(st + kABytes, 16, 1024, 2);
+                    const uint64_t db = smem_desc(
+                        FUSE ? stage0 + S * kStage + kb * (BT * kBK) : st + kABytes, 16, 1024, 2);
 #pragma unroll
                     for (int k = 0; k < kBK / 32; k++) {
                         if constexpr (FORM == PAIR)
@@ -493,6 +588,14 @@ linear_i8_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
         const int quad = warp & 3, part = (warp - kWarpEpi) >> 2;
         const uint32_t lane_base = (uint32_t)(quad * 32) << 16;
         Ring ra(kAcc);
+        if constexpr (FUSE) {
+            quantize_slice<X, BT>(a, kb0, kbn, smem_raw + (stage0 - ctrl) + S * kStage, scales,
+                                  reinterpret_cast<unsigned *>(scales + BT));
+            // written through the generic proxy, read by the MMAs' async one
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar_sfull);
+        }
         for (int tile = first; tile < a.tiles; tile += step, ra.next()) {
             int ft, tt;
             tile_of(a, tile, ft, tt);
@@ -561,7 +664,7 @@ linear_i8_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
                 s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
             }
             const int t = tt * BT + j;
-            const float sx = __ldg(a.q_scale + t);
+            const float sx = FUSE ? scales[j] : __ldg(a.q_scale + t);
             const int sums[4] = {s.x, s.y, s.z, s.w};
 #pragma unroll
             for (int i = 0; i < 4; i++) {
@@ -569,7 +672,8 @@ linear_i8_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
                 float v = __fmaf_rn((float)sums[i], sx * __ldg(a.w_scale + n + i),
                                     a.bias ? __ldg(a.bias + n + i) : 0.0f);
                 v = act_apply(v, a.act);
-                if (a.res) v += to_float(((const T *)a.res)[(long long)t * a.ldres + n + i]);
+                if (a.res)
+                    v = __fadd_rn(v, to_float(((const T *)a.res)[(long long)t * a.ldres + n + i]));
                 ((T *)a.y)[(long long)t * a.ldy + n + i] = from_float<T>(v);
             }
         }
@@ -599,14 +703,16 @@ int sm_count() {
     return n > 0 ? n : 148;
 }
 
-template <typename T, int BT, int FORM>
+template <typename T, int BT, int FORM, typename X = int8_t>
 Status launch(const LinearI8Args &p, Args a, int splits, cudaStream_t st) {
     CUtensorMap tmW, tmQ;
     if (!tma_encode_bytes(&tmW, p.w, p.K, p.N, p.ldw, kBK, kFeat) ||
-        !tma_encode_bytes(&tmQ, p.q, p.K, p.M, p.ldq, kBK, load_tokens(BT, FORM)))
+        !(sizeof(X) > 1 ||
+          tma_encode_bytes(&tmQ, p.q, p.K, p.M, p.ldq, kBK, load_tokens(BT, FORM))))
         return ERR_SHAPE;
-    auto kernel = linear_i8_kernel<T, BT, FORM>;
-    constexpr int smem = smem_bytes(BT, FORM);
+    if (sizeof(X) > 1) tmQ = tmW;  // not read
+    auto kernel = linear_i8_kernel<T, BT, FORM, X>;
+    constexpr int smem = sizeof(X) > 1 ? fuse_smem(BT) : smem_bytes(BT, FORM);
     if (!smem_attr_once((const void *)kernel, smem)) {
         cudaGetLastError();
         return ERR_CUDA;
@@ -691,9 +797,10 @@ Choice choose(int M, int N, int kblocks) {
 
 }  // namespace
 
-Status launch_linear_i8(const LinearI8Args &p, cudaStream_t st) {
-    if (p.M == 0) return OK;
-    if (p.M < 0 || p.N <= 0 || p.K <= 0) return ERR_SHAPE;
+namespace {
+
+// p as the kernels take it; q and its scales apart
+Args kernel_args(const LinearI8Args &p) {
     Args a = {};
     a.M = p.M; a.N = p.N; a.kblocks = cdiv(p.K, kBK);
     a.act = p.act;
@@ -702,6 +809,15 @@ Status launch_linear_i8(const LinearI8Args &p, cudaStream_t st) {
     a.y = (void *)p.y.p; a.ldy = p.y.ld;
     a.pairs = p.type != T_F32 && ((uintptr_t)a.y & 3) == 0 && (p.M == 1 || a.ldy % 2 == 0) &&
               (!a.res || (((uintptr_t)a.res & 3) == 0 && (p.M == 1 || a.ldres % 2 == 0)));
+    return a;
+}
+
+}  // namespace
+
+Status launch_linear_i8(const LinearI8Args &p, cudaStream_t st) {
+    if (p.M == 0) return OK;
+    if (p.M < 0 || p.N <= 0 || p.K <= 0) return ERR_SHAPE;
+    const Args a = kernel_args(p);
     const Choice c = choose(p.M, p.N, a.kblocks);
     return with_type(p.type, [&](auto t) {
         using T = decltype(t);
@@ -717,6 +833,29 @@ Status launch_linear_i8(const LinearI8Args &p, cudaStream_t st) {
             default: return launch<T, 256, WHOLE>(p, a, 1, st);
         }
     });
+}
+
+bool launch_linear_i8_few(const Rows &x, int x_type, const LinearI8Args &p, cudaStream_t st,
+                          Status *status) {
+    // every CTA reads all rows for their largest values, one after another.
+    // K = N = 4096, BF16, against the two kernels: 1 row 8.9 / 9.5 us, 2 rows
+    // 9.4 / 9.4, 4 rows 10.5 / 9.7, 16 rows 26 / 10; and a launch less, 2.5 us
+    // of the host's time
+    if (p.M <= 0 || p.M > 2 || (long long)p.M * p.K > 65536) return false;
+    Args a = kernel_args(p);
+    a.x = x.p; a.ldx = x.ld; a.K = p.K;
+    const Choice c = choose(p.M, p.N, a.kblocks);
+    // (the whole-K form of 16 tokens as a split in one)
+    if (c.bt != 16 || cdiv(a.kblocks, c.splits) > kFuseBlocks ||
+        (c.form != SPLIT && cdiv(p.N, kFeat) > 2 * sm_count()))
+        return false;
+    *status = with_type(p.type, [&](auto t) {
+        using T = decltype(t);
+        return with_type(x_type, [&](auto xt) {
+            return launch<T, 16, SPLIT, decltype(xt)>(p, a, c.splits, st);
+        });
+    });
+    return true;
 }
 
 int linear_error_fetch_and_clear() {

@@ -41,10 +41,19 @@ bool rows_ok(const void *p, long long ld, long long rows, int D, int type, bool 
     return aligned(p, ppdl::elem_size(type)) && (rows <= 1 || ld >= D);
 }
 
-// ppdl_linear_i8's checks, and its launch
+// The rows that ppdl_linear_i8_dynamic quantises
+struct Dynamic {
+    const void *x;
+    long long ldx;
+    int type;
+};
+
+// ppdl_linear_i8; with `dynamic`, q and q_scale are workspace that its rows
+// are first quantised into, unless the product's kernel quantises them itself
 int linear_i8(const int8_t *q, long long ldq, const float *q_scale, const int8_t *w, long long ldw,
               const float *w_scale, const float *bias, const void *res, long long ldres, int type,
-              int act, int M, int N, int K, void *y, long long ldy, void *stream, bool launch) {
+              int act, int M, int N, int K, void *y, long long ldy, void *stream,
+              const Dynamic *dynamic) {
     ppdl::set_op_error("");
     if (!ppdl::elem_type_ok(type) || act < 0 || act > 3)
         return refuse("linear_i8: unknown element type or activation");
@@ -62,7 +71,18 @@ int linear_i8(const int8_t *q, long long ldq, const float *q_scale, const int8_t
     a.q = q; a.ldq = ldq; a.q_scale = q_scale; a.w = w; a.ldw = ldw; a.w_scale = w_scale;
     a.bias = bias; a.res = {res, ldres}; a.y = {y, ldy};
     a.type = type; a.act = act; a.M = M; a.N = N; a.K = K;
-    if (!launch) return PPDL_OK;
+    if (dynamic) {
+        const Dynamic &d = *dynamic;
+        if (!ppdl::elem_type_ok(d.type) || !rows_ok(d.x, d.ldx, M, K, d.type))
+            return refuse("linear_i8_dynamic: unknown element type, null or misaligned rows, or "
+                          "rows closer than K elements");
+        ppdl::Status s = ppdl::OK;
+        if (ppdl::launch_linear_i8_few({d.x, d.ldx}, d.type, a, (cudaStream_t)stream, &s))
+            return status_of(s, "linear_i8_dynamic: sizes too large");
+        s = ppdl::launch_quantize_rows({d.x, d.ldx}, d.type, M, K, (int8_t *)q, ldq,
+                                       (float *)q_scale, (cudaStream_t)stream);
+        if (s != ppdl::OK) return status_of(s, "linear_i8_dynamic: sizes too large");
+    }
     return status_of(ppdl::launch_linear_i8(a, (cudaStream_t)stream), "linear_i8: sizes too large");
 }
 
@@ -145,7 +165,7 @@ PPDL_OPS_API int ppdl_linear_i8(const int8_t *q, long long ldq, const float *q_s
                                 int act, int M, int N, int K, void *y, long long ldy,
                                 void *stream) {
     return linear_i8(q, ldq, q_scale, w, ldw, w_scale, bias, res, ldres, type, act, M, N, K, y, ldy,
-                     stream, true);
+                     stream, nullptr);
 }
 
 namespace {
@@ -169,15 +189,9 @@ PPDL_OPS_API int ppdl_linear_i8_dynamic(const void *x, long long ldx, int x_type
         return refuse("linear_i8_dynamic: null or misaligned workspace");
     if (M < 0 || K <= 0) return refuse("linear_i8_dynamic: bad sizes");
     int8_t *q = (int8_t *)work;
-    float *scale = (float *)(q + scales_at(M, K));
-    // the product's arguments are checked before the quantiser is launched
-    const int ok = linear_i8(q, row_bytes(K), scale, w, ldw, w_scale, bias, res, ldres, type, act,
-                             M, N, K, y, ldy, stream, false);
-    if (ok != PPDL_OK) return ok;
-    const int rc = ppdl_quantize_rows_i8(x, ldx, x_type, M, K, q, row_bytes(K), scale, stream);
-    if (rc != PPDL_OK) return rc;
-    return linear_i8(q, row_bytes(K), scale, w, ldw, w_scale, bias, res, ldres, type, act, M, N, K,
-                     y, ldy, stream, true);
+    const Dynamic rows = {x, ldx, x_type};
+    return linear_i8(q, row_bytes(K), (const float *)(q + scales_at(M, K)), w, ldw, w_scale, bias,
+                     res, ldres, type, act, M, N, K, y, ldy, stream, &rows);
 }
 
 PPDL_OPS_API int ppdl_rotary(const ppdl_rotary_heads *q, const ppdl_rotary_heads *k, int type,

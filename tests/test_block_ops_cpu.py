@@ -43,6 +43,13 @@ def linear(**kw):
     return L().ppdl_linear_i8(*a.values(), None)
 
 
+def dynamic(**kw):
+    a = dict(x=P, ldx=16, xt=0, w=P, ldw=16, ws=P, bias=None, res=None, ldres=0, type=0, act=0, M=4,
+             N=4, K=16, y=P, ldy=4, work=P)
+    a.update(kw)
+    return L().ppdl_linear_i8_dynamic(*a.values(), None)
+
+
 def rotary(heads=None, sections=(4,), **kw):
     h = dict(in_=P, out=P, heads=2, in_batch=64, in_token=16, in_head=8, out_batch=64, out_token=16,
              out_head=8)
@@ -74,6 +81,9 @@ def rotary(heads=None, sections=(4,), **kw):
     (linear, dict(y=None)), (linear, dict(ldq=8)), (linear, dict(ldw=20)), (linear, dict(q=P + 1)),
     (linear, dict(w=P + 8)), (linear, dict(ldy=3)), (linear, dict(res=P, ldres=3)),
     (linear, dict(bias=P + 2)), (linear, dict(K=17)),
+    (dynamic, dict(x=None)), (dynamic, dict(xt=7)), (dynamic, dict(ldx=8)), (dynamic, dict(x=P + 2)),
+    (dynamic, dict(work=None)), (dynamic, dict(work=P + 8)), (dynamic, dict(M=-1)), (dynamic, dict(K=0)),
+    (dynamic, dict(w=None)), (dynamic, dict(act=9)), (dynamic, dict(ldy=2)), (dynamic, dict(type=5)),
     (rotary, dict(type=3)), (rotary, dict(dim=0)), (rotary, dict(dim=1025)), (rotary, dict(rotated=7)),
     (rotary, dict(rotated=0, sections=(0,))), (rotary, dict(rotated=10, sections=(5,))),
     (rotary, dict(sections=(3,))), (rotary, dict(sections=(5, -1))),
@@ -89,7 +99,8 @@ def test_refused(call, bad):
 
 
 @pytest.mark.parametrize("call,none", [(ln, dict(rows=0)), (quant, dict(rows=0)),
-                                       (linear, dict(M=0)), (rotary, dict(batch=0)),
+                                       (linear, dict(M=0)), (dynamic, dict(M=0, work=None)),
+                                       (rotary, dict(batch=0)),
                                        (rotary, dict(length=0)),
                                        (ln_bwd, dict(rows=0, dw=None, db=None))])
 def test_nothing_to_do(call, none):
@@ -101,6 +112,12 @@ def test_backward_workspace_size():
     f = L().ppdl_layernorm_backward_workspace
     assert f(0, 8) == 0 and f(8, 0) == 0 and f(-1, 8) == 0
     assert f(1, 8) >= 16 and f(1 << 20, 4096) >= 2 * 4096
+
+
+def test_dynamic_workspace_size():
+    f = L().ppdl_linear_i8_dynamic_workspace
+    assert f(0, 8) == 0 and f(8, 0) == 0
+    assert f(3, 17) == 3 * 32 + 12 and f(1 << 20, 131071) == (131072 + 4) << 20
 
 
 def rejects(f, *args, **kw):

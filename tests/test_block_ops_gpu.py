@@ -339,7 +339,7 @@ def lin_want(q, qs, w, ws, bias, act, residual, T):
     return y, tol + (half(T) + U) * y.abs() + (2.0 ** -25 if T == torch.float16 else 1e-38)
 
 
-LIN_SHAPES = [(1, 1, 1), (1, 16, 7), (2, 17, 3), (1, 4096, 512), (1, 1000, 333), (3, 300, 129),
+LIN_SHAPES = [(16, 4096, 300), (5, 2047, 260), (1, 65000, 33), (7, 8192, 129), (1, 2048, 40000), (1, 1, 1), (1, 16, 7), (2, 17, 3), (1, 4096, 512), (1, 1000, 333), (3, 300, 129),
               (8, 2048, 256), (16, 512, 1000), (17, 515, 130), (33, 64, 64), (64, 128, 200),
               (100, 256, 300), (128, 128, 128), (129, 130, 257), (300, 256, 1024), (300, 2048, 256),
               (511, 1111, 127), (1000, 96, 2047), (2400, 256, 256), (777, 1111, 513), (5000, 40, 40),
@@ -421,6 +421,29 @@ def test_linear_i8_bad_rows_stay_their_own(cuda):
     y = ppdl.linear_i8(x, wq, ws)
     keep = [i for i in range(40) if i not in (3, 17)]
     assert torch.equal(y[keep], clean[keep]) and y[3].isnan().all() and y[17].isnan().all()
+
+
+@pytest.mark.parametrize("M,K", [(1, 512), (2, 300), (1, 1003), (2, 4096), (9, 300), (16, 1000)])
+def test_linear_i8_few_rows(cuda, M, K):
+    """Few rows in place: strided and unaligned ones, ties, and bad, zero and
+    tiny rows, quantised in the product's kernel to the same bits."""
+    g = gen(M + K)
+    wq, ws = ppdl.quantize_rows(normal(g, 200, K))
+    for T in TYPES.values():
+        for x in (normal(g, M, K, t=T), normal(g, M, K + 1, t=T)[:, 1:], normal(g, M, 2 * K, t=T)[:, K:]):
+            x[0, 3:40] = x.abs().max() / 2            # 63.5 steps when it is the row's largest
+            if M == 2:
+                x[1] = {300: 0.0, 4096: float("nan")}[K]
+            if M > 8:
+                x[1], x[2] = 0, x[2] * 1e-6
+                x[3] = x[3] * 2.0 ** -120 if T != torch.float16 else x[3]
+                x[4, K - 1], x[5, 0] = float("nan"), float("-inf")
+            q, s = ppdl.quantize_rows(x)
+            want = ppdl.linear_i8(q, wq, ws, x_scale=s, out_dtype=T)
+            got = ppdl.linear_i8(x, wq, ws)
+            assert torch.equal(got.nan_to_num(7.0), want.nan_to_num(7.0))
+            if M > 8:
+                assert got[4].isnan().all() and got[5].isnan().all() and (got[1] == 0).all()
 
 
 def test_linear_i8_in_place_residual(cuda):
