@@ -351,7 +351,7 @@ PPDL_OPS_API long long ppdl_linear_i8_dynamic_workspace(int M, int K);
 typedef struct {
     const void * in;
     void *       out;    /* may be in, with the same strides */
-    int32_t      heads;  /* 0: none */
+    int32_t      heads;  /* at most 65535; 0: none */
     int64_t      in_batch, in_token, in_head;
     int64_t      out_batch, out_token, out_head;
 } ppdl_rotary_heads;
@@ -380,7 +380,8 @@ PPDL_OPS_API int ppdl_rotary(const ppdl_rotary_heads * q, const ppdl_rotary_head
 PPDL_OPS_API const char * ppdl_op_last_error(void);
 
 /* Extension (the reference aborts through GGML_ASSERT and has no device-side
-   error state): the tensor-core kernels bound every wait inside the kernel
+   error state): the tensor-core kernels, and the layer norms whose rows come
+   through rings in shared memory, bound every wait inside the kernel
    (about 2 s); a wait that gives up leaves its output unwritten, and the
    kernel raises a device-wide flag.  After synchronising the stream of the
    launches in question, this returns 1 if the flag was raised since the last

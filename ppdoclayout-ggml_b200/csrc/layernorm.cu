@@ -76,7 +76,7 @@ layernorm_vector_kernel(const T *x, long long ldx, const T *res, long long ldres
     using Tile = PairTile<T, TPR, NE>;
     pdl_begin();
     pdl_trigger();
-    __shared__ float sh[2][32];
+    __shared__ __align__(16) float sh[2][32];
     constexpr int kRows = TPR < 128 ? 128 / TPR : 1, kHalf = Tile::kVec / 2;
     const int lane = threadIdx.x % TPR;
     long long row = (long long)blockIdx.x * kRows + threadIdx.x / TPR;
@@ -97,7 +97,7 @@ layernorm_vector_kernel(const T *x, long long ldx, const T *res, long long ldres
 #pragma unroll
     for (int j = 0; j < NE / 2; j++) t = add2(t, Tile::pair(r, j));
     float s[1] = {t.x + t.y};
-    row_sums<TPR>(s, sh[0]);
+    team_sums<TPR>(s, sh[0], threadIdx.x / TPR);
     const float mean = s[0] / (float)D;
     t = both(0.0f);
 #pragma unroll
@@ -111,7 +111,7 @@ layernorm_vector_kernel(const T *x, long long ldx, const T *res, long long ldres
             }
         }
     s[0] = t.x + t.y;
-    row_sums<TPR>(s, sh[1]);
+    team_sums<TPR>(s, sh[1], threadIdx.x / TPR);
     const float rstd = rsqrtf(s[0] / (float)D + eps);
     if (!real) return;
     if (sum) Tile::store(sum + row * ldsum, r, D, lane);
@@ -144,7 +144,7 @@ layernorm_tile_kernel(const T *x, long long ldx, const T *res, long long ldres, 
     using Tile = RowTile<T, TPR, NE>;
     pdl_begin();
     pdl_trigger();
-    __shared__ float sh[2][32];
+    __shared__ __align__(16) float sh[2][32];
     constexpr int kRows = TPR < 128 ? 128 / TPR : 1;
     const int lane = threadIdx.x % TPR;
     long long row = (long long)blockIdx.x * kRows + threadIdx.x / TPR;
@@ -166,7 +166,7 @@ layernorm_tile_kernel(const T *x, long long ldx, const T *res, long long ldres, 
         v[j] = to_float(r.v[j]);
         s[0] += v[j];
     }
-    row_sums<TPR>(s, sh[0]);
+    team_sums<TPR>(s, sh[0], threadIdx.x / TPR);
     const float mean = s[0] / (float)D;
     s[0] = 0.0f;
 #pragma unroll
@@ -174,7 +174,7 @@ layernorm_tile_kernel(const T *x, long long ldx, const T *res, long long ldres, 
         v[j] -= mean;
         if (Tile::inside(j, D, lane)) s[0] += v[j] * v[j];
     }
-    row_sums<TPR>(s, sh[1]);
+    team_sums<TPR>(s, sh[1], threadIdx.x / TPR);
     const float rstd = rsqrtf(s[0] / (float)D + eps);
     if (!real) return;
     if (sum) Tile::store(sum + row * ldsum, r, D, lane);
@@ -350,7 +350,7 @@ layernorm_bwd_tile_kernel(const T *dy, long long lddy, const T *x, long long ldx
                           float *part) {
     using Tile = RowTile<T, TPR, NE>;
     constexpr int kThreads = bwd_threads(TPR), kRows = kThreads / TPR;
-    __shared__ float sh[2][kThreads / 32 * 2];
+    __shared__ __align__(16) float sh[2][kThreads / 32 * 2];
     __shared__ float red[kRows > 1 ? kThreads * NE : 1];
     pdl_begin();
     pdl_trigger();
@@ -397,7 +397,7 @@ layernorm_bwd_tile_kernel(const T *dy, long long lddy, const T *x, long long ldx
         }
         typename Tile::Raw out;
         if (dsum && real) Tile::load(out, dsum + row * lddsum, D, lane);
-        row_sums<TPR>(s, sh[parity]);
+        team_sums<TPR>(s, sh[parity], group);
         const float m1 = s[0] / (float)D, m2 = s[1] / (float)D;
         if (real) {
 #pragma unroll

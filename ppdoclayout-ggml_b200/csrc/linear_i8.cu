@@ -799,6 +799,12 @@ Choice choose(int M, int N, int kblocks) {
 
 namespace {
 
+// tile origins stay below 2^31
+bool sizes_ok(const LinearI8Args &p) {
+    constexpr int kMost = 0x7fffffff - 512;
+    return p.M > 0 && p.M <= kMost && p.N > 0 && p.N <= kMost && p.K > 0;
+}
+
 // p as the kernels take it; q and its scales apart
 Args kernel_args(const LinearI8Args &p) {
     Args a = {};
@@ -816,7 +822,7 @@ Args kernel_args(const LinearI8Args &p) {
 
 Status launch_linear_i8(const LinearI8Args &p, cudaStream_t st) {
     if (p.M == 0) return OK;
-    if (p.M < 0 || p.N <= 0 || p.K <= 0) return ERR_SHAPE;
+    if (!sizes_ok(p)) return ERR_SHAPE;
     const Args a = kernel_args(p);
     const Choice c = choose(p.M, p.N, a.kblocks);
     return with_type(p.type, [&](auto t) {
@@ -841,7 +847,7 @@ bool launch_linear_i8_few(const Rows &x, int x_type, const LinearI8Args &p, cuda
     // K = N = 4096, BF16, against the two kernels: 1 row 8.9 / 9.5 us, 2 rows
     // 9.4 / 9.4, 4 rows 10.5 / 9.7, 16 rows 26 / 10; and a launch less, 2.5 us
     // of the host's time
-    if (p.M <= 0 || p.M > 2 || (long long)p.M * p.K > 65536) return false;
+    if (!sizes_ok(p) || p.M > 2 || (long long)p.M * p.K > 65536) return false;
     Args a = kernel_args(p);
     a.x = x.p; a.ldx = x.ld; a.K = p.K;
     const Choice c = choose(p.M, p.N, a.kblocks);

@@ -222,7 +222,7 @@ PPDL_OPS_API int ppdl_rotary(const ppdl_rotary_heads *q, const ppdl_rotary_heads
     const ppdl_rotary_heads *h[2] = {q, k};
     for (int i = 0; i < 2; i++) {
         if (!h[i] || h[i]->heads == 0) continue;
-        if (h[i]->heads < 0 || (some && (!h[i]->in || !h[i]->out)) ||
+        if (h[i]->heads < 0 || h[i]->heads > 65535 || (some && (!h[i]->in || !h[i]->out)) ||
             !aligned(h[i]->in, ppdl::elem_size(type)) || !aligned(h[i]->out, ppdl::elem_size(type)))
             return refuse("rotary: bad number of heads, or null or misaligned heads");
         ppdl::RotaryHeads &o = a.h[i];

@@ -58,36 +58,11 @@ struct RowTile {
     }
 };
 
-// Sums of N values over the TPR threads of each row, known to all of them.
-// TPR <= 32: shuffles within the row's lanes.  Wider: the warps' sums go
-// through sh[warps of the block][N] and one barrier of the whole block; a
-// block that sums again gives another sh (or has a barrier in between).
-template <int TPR, int N>
-__device__ __forceinline__ void row_sums(float (&v)[N], float *sh) {
-    constexpr int kWidth = TPR < 32 ? TPR : 32;
-#pragma unroll
-    for (int o = kWidth / 2; o > 0; o >>= 1)
-#pragma unroll
-        for (int i = 0; i < N; i++) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
-    if constexpr (TPR > 32) {
-        constexpr int kWarps = TPR / 32;
-        const int warp = threadIdx.x >> 5;
-        if ((threadIdx.x & 31) == 0)
-#pragma unroll
-            for (int i = 0; i < N; i++) sh[warp * N + i] = v[i];
-        __syncthreads();
-        sh += warp / kWarps * (kWarps * N);
-#pragma unroll
-        for (int i = 0; i < N; i++) v[i] = sh[i];
-#pragma unroll
-        for (int w = 1; w < kWarps; w++)
-#pragma unroll
-            for (int i = 0; i < N; i++) v[i] += sh[w * N + i];
-    }
-}
-
-// The same for a block of several teams of TPR threads (of a warp, when TPR
-// <= 32) that run on their own: a team's barrier is the named one 1 + team.
+// Sums of N values over the TPR threads of each row, known to all of them, in
+// an order of their own.  TPR <= 32: shuffles within the row's lanes.  Wider:
+// the row's threads are a team with a named barrier (1 + team) of its own;
+// the warps' sums go through sh[warps of the block][N], 16-byte aligned.  A
+// team that sums again gives another sh (or has a barrier in between).
 template <int TPR, int N>
 __device__ __forceinline__ void team_sums(float (&v)[N], float *sh, int team) {
     constexpr int kWidth = TPR < 32 ? TPR : 32;

@@ -90,7 +90,7 @@ def rotary(heads=None, sections=(4,), **kw):
     (rotary, dict(sections=(1, 1, 1, 1, 0))), (rotary, dict(axes=0)), (rotary, dict(pb=2)),
     (rotary, dict(pos=None)), (rotary, dict(pos=P + 4)), (rotary, dict(freq=None)),
     (rotary, dict(freq=P + 4)), (rotary, dict(batch=-1)), (rotary, dict(length=-1)),
-    (rotary, dict(heads=dict(heads=-1))), (rotary, dict(heads=dict(in_=None))),
+    (rotary, dict(heads=dict(heads=-1))), (rotary, dict(heads=dict(heads=65536))), (rotary, dict(heads=dict(in_=None))),
     (rotary, dict(heads=dict(out=None))), (rotary, dict(heads=dict(in_=P + 2))),
 ])
 def test_refused(call, bad):

@@ -661,6 +661,70 @@ def test_two_streams_at_once(cuda):
         assert all(torch.equal(v, want[i]) for v in got[i])
 
 
+FIRST = """
+import sys
+sys.path.insert(0, sys.argv[1])
+import torch, ppdl
+x, w = torch.randn(300, 2048, device="cuda").bfloat16(), torch.randn(2048, device="cuda")
+wq, ws = torch.randint(-127, 128, (512, 2048), device="cuda").to(torch.int8), torch.rand(512, device="cuda")
+pos, freq = torch.arange(300, device="cuda").view(1, 1, 300), torch.ones(64, dtype=torch.float64, device="cuda")
+def step():
+    y, s, mean, rstd = ppdl.layernorm(x, w, w, residual=x, return_sum=True, return_stats=True)
+    return (y, *ppdl.layernorm_backward(x, s, w, mean, rstd), ppdl.linear_i8(x, wq, ws), ppdl.linear_i8(x[:1], wq, ws),
+            ppdl.rotary(x.view(1, 300, 16, 128), None, pos, freq, (64,))[0])
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    got = step()
+graph.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(got, step()))
+assert ppdl.lib().ppdl_op_device_error() == 0
+"""
+
+
+def test_first_calls_inside_a_capture(cuda):
+    """A process whose first call of each operator is a captured one."""
+    import os
+    import subprocess
+    import sys
+    subprocess.run([sys.executable, "-c", FIRST, os.path.dirname(ppdl.__file__)], check=True, timeout=300)
+
+
+def test_tensors_of_another_device(cuda, monkeypatch):
+    """Tensors of a GPU that is not the current one: the call is made with
+    theirs current (shown on one GPU, by a current device that claims to be
+    another until it is set)."""
+    x, w = torch.randn(5, 64, device="cuda"), torch.ones(64, device="cuda")
+    wq, ws = ppdl.quantize_rows(torch.randn(8, 64, device="cuda"))
+    h, pos = x.view(1, 5, 1, 64), torch.arange(5, device="cuda").view(1, 1, 5)
+    freq = torch.ones(32, dtype=torch.float64, device="cuda")
+    _, mean, rstd = ppdl.layernorm(x, w, return_stats=True)
+    calls = [lambda: ppdl.layernorm(x, w, w), lambda: ppdl.layernorm_backward(x, x, w, mean, rstd),
+             lambda: ppdl.quantize_rows(x), lambda: ppdl.linear_i8(x, wq, ws),
+             lambda: ppdl.rotary(h, h, pos, freq, (32,))]
+    want = [f() for f in calls]
+    entered = []
+
+    class Device:
+        def __init__(self, index):
+            self.index = index
+
+        def __enter__(self):
+            entered.append(self.index)
+
+        def __exit__(self, *a):
+            pass
+
+    for f, expected in zip(calls, want):
+        n = len(entered)
+        monkeypatch.setitem(ppdl._tt, "device", Device)
+        monkeypatch.setitem(ppdl._tt, "current", lambda: 0 if len(entered) > n else 7)
+        got = f()
+        assert entered[n:] == [0]
+        pairs = zip(got, expected) if isinstance(got, tuple) else [(got, expected)]
+        assert all(torch.equal(a, b) for a, b in pairs)
+
+
 def test_no_kernel_gave_up(cuda):
     torch.cuda.synchronize()
     assert ppdl.lib().ppdl_op_device_error() == 0
