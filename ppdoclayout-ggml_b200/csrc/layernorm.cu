@@ -15,6 +15,8 @@
 #include "block.cuh"
 #include "block.h"
 #include "rows.cuh"
+
+#include <initializer_list>
 #include "tc_ptx.cuh"
 
 namespace ppdl {
@@ -283,6 +285,88 @@ layernorm_ring_kernel(const T *x, long long ldx, const T *res, long long ldres, 
         if (mean_out) mean_out += ring.step;
         if (rstd_out) rstd_out += ring.step;
     }
+}
+
+// Dense rows that are no whole 16-byte vectors, groups of them through shared
+// memory (GroupRing): one block of 512 threads on each SM, TPR threads a row,
+// weights and biases in registers.
+constexpr int kGroupThreads = 512, kGroupMaxRows = 128;
+template <typename T, typename WT, int TPR, int NP>
+__global__ void __launch_bounds__(kGroupThreads, 1)
+layernorm_group_kernel(const T *x, const T *res, T *y, T *sum, const WT *w, const WT *b,
+                       float *mean_out, float *rstd_out, long long rows, int D, float eps,
+                       int rows_at, int stages) {
+    using Tile = WordTile<T, TPR, NP>;
+    using Groups = GroupRing<T, 2>;
+    extern __shared__ __align__(16) uint8_t ring_smem[];
+    __shared__ typename Groups::Shared shared;
+    __shared__ __align__(16) float sh[2][kGroupThreads / 32];
+    // an even number of teams: a team's rows start in the same half of a word
+    const int lane = threadIdx.x % TPR, team = threadIdx.x / TPR, teams = blockDim.x / TPR;
+    const Tile tile(lane, team & D & 1, D);
+    Groups ring;
+    ring.setup({x, res}, ring_smem, &shared, &g_row_error, rows, D, rows_at, stages);
+    pdl_begin();
+    pdl_trigger();
+    ring.start();
+    float2 pw[NP], pb[NP];
+    tile.load_params(pw, w, 1.0f);
+    tile.load_params(pb, b, 0.0f);
+    const float inv_d = 1.0f / (float)D;
+    for (int it = 0; it < ring.iters; it++) {
+        ring.wait();
+        const int count = ring.count(ring.group);
+        const long long row0 = ring.group * rows_at;
+        for (int q0 = 0; q0 < count; q0 += teams) {
+            const int q = q0 + team;
+            const bool real = q < count;
+            T *row = ring.buffer(0) + q * D;
+            typename Tile::Raw r = {};
+            if (real) {
+                tile.load(r, row);
+                if (res) {
+                    T *other = ring.buffer(1) + q * D;
+                    typename Tile::Raw o;
+                    tile.load(o, other);
+#pragma unroll
+                    for (int j = 0; j < NP; j++)
+                        Tile::set_pair(r, j, add2(Tile::pair(r, j), Tile::pair(o, j)));
+                    if (sum) tile.store(other, r);
+                }
+            }
+            float2 v[NP], t = both(0.0f);
+#pragma unroll
+            for (int j = 0; j < NP; j++) {
+                v[j] = Tile::pair(r, j);
+                t = add2(t, v[j]);
+            }
+            float s[1] = {t.x + t.y};
+            team_sums<TPR>(s, sh[0], team);
+            const float mean = s[0] * inv_d;
+            t = both(0.0f);
+#pragma unroll
+            for (int j = 0; j < NP; j++) {
+                v[j] = add2(v[j], both(-mean));
+                if (!tile.inside(j, 0)) v[j].x = 0.0f;
+                if (!tile.inside(j, 1)) v[j].y = 0.0f;
+                t = fma2(v[j], v[j], t);
+            }
+            s[0] = t.x + t.y;
+            team_sums<TPR>(s, sh[1], team);
+            const float rstd = rsqrtf(s[0] * inv_d + eps);
+            if (!real) continue;
+#pragma unroll
+            for (int j = 0; j < NP; j++)
+                Tile::set_pair(r, j, fma2(mul2(v[j], both(rstd)), pw[j], pb[j]));
+            tile.store(row, r);
+            if (lane == 0 && ring.good) {
+                if (mean_out) mean_out[row0 + q] = mean;
+                if (rstd_out) rstd_out[row0 + q] = rstd;
+            }
+        }
+        ring.store(it, 0, y, 1, sum);
+    }
+    ring.finish();
 }
 
 // dx, one block per row, any width.
@@ -567,6 +651,106 @@ layernorm_bwd_ring_kernel(const T *dy, long long lddy, const T *x, long long ldx
     }
 }
 
+// The same for dense rows that are no whole 16-byte vectors, groups of them
+// through shared memory as in layernorm_group_kernel.
+template <typename T, typename WT, int TPR, int NP>
+__global__ void __launch_bounds__(kGroupThreads, 1)
+layernorm_bwd_group_kernel(const T *dy, const T *x, const T *dsum, T *dx, const WT *w,
+                           const float *mean_in, const float *rstd_in, long long rows, int D,
+                           float *part, int rows_at, int stages) {
+    using Tile = WordTile<T, TPR, NP>;
+    using Groups = GroupRing<T, 3>;
+    extern __shared__ __align__(16) uint8_t ring_smem[];
+    __shared__ typename Groups::Shared shared;
+    __shared__ __align__(16) float sh[2][kGroupThreads / 32 * 2];
+    __shared__ float2 stats[2][kGroupMaxRows];  // the present group's and the next one's
+    // an even number of teams: a team's rows start in the same half of a word
+    const int lane = threadIdx.x % TPR, team = threadIdx.x / TPR, teams = blockDim.x / TPR;
+    const Tile tile(lane, team & D & 1, D);
+    Groups ring;
+    ring.setup({x, dy, dsum}, ring_smem, &shared, &g_row_error, rows, D, rows_at, stages);
+    pdl_begin();
+    pdl_trigger();
+    ring.start();
+    float2 p[NP], dw[NP], db[NP];
+    tile.load_params(p, w, 1.0f);
+#pragma unroll
+    for (int j = 0; j < NP; j++) dw[j] = db[j] = both(0.0f);
+    // thread q looks after row q's statistics, a group ahead
+    float2 next = both(0.0f);
+    auto look = [&](long long group) {
+        const long long row = group * rows_at + threadIdx.x;
+        if ((int)threadIdx.x < rows_at && row < rows) next = make_float2(mean_in[row], rstd_in[row]);
+    };
+    look(ring.group);
+    const float inv_d = 1.0f / (float)D;
+    int parity = 0;
+    for (int it = 0; it < ring.iters; it++) {
+        if ((int)threadIdx.x < rows_at) stats[it & 1][threadIdx.x] = next;
+        look(ring.group + gridDim.x);
+        ring.wait();
+        __syncthreads();
+        const int count = ring.count(ring.group);
+        for (int q0 = 0; q0 < count; q0 += teams, parity ^= 1) {
+            const int q = q0 + team;
+            const bool real = q < count;
+            T *row = ring.buffer(0) + q * D;
+            typename Tile::Raw rx = {}, rd = {};
+            float2 g[NP], t0 = both(0.0f), t1 = both(0.0f);
+            float r = 0.0f, mr = 0.0f;
+            if (real) {
+                tile.load(rx, row);
+                tile.load(rd, ring.buffer(1) + q * D);
+                // x r - mean r: off by the rounding of mean r, u |mean| r
+                r = stats[it & 1][q].y;
+                mr = -stats[it & 1][q].x * r;
+#pragma unroll
+                for (int j = 0; j < NP; j++) {
+                    const float2 xh = fma2(Tile::pair(rx, j), both(r), both(mr));
+                    const float2 d = Tile::pair(rd, j);
+                    dw[j] = fma2(d, xh, dw[j]);
+                    db[j] = add2(db[j], d);
+                    g[j] = mul2(d, p[j]);
+                    t0 = add2(t0, g[j]);
+                    t1 = fma2(g[j], xh, t1);
+                }
+            }
+            float s[2] = {t0.x + t0.y, t1.x + t1.y};
+            team_sums<TPR>(s, sh[parity], team);
+            if (!real) continue;
+            const float2 m1 = both(-s[0] * inv_d * r), m2 = both(-s[1] * inv_d * r);
+            if (dsum) tile.load(rd, ring.buffer(2) + q * D);
+#pragma unroll
+            for (int j = 0; j < NP; j++) {
+                const float2 xh = fma2(Tile::pair(rx, j), both(r), both(mr));
+                float2 v = fma2(g[j], both(r), fma2(xh, m2, m1));
+                if (dsum) v = add2(v, Tile::pair(rd, j));
+                Tile::set_pair(rx, j, v);
+            }
+            tile.store(row, rx);
+        }
+        ring.store(it, 0, dx, 0, nullptr);
+    }
+    ring.finish();
+    if (!part) return;
+    part += (long long)blockIdx.x * 2 * D;
+    // the teams' sums in order, through the ring (all its copies are done)
+    float *red = reinterpret_cast<float *>(ring_smem);
+    for (int which = 0; which < 2; which++) {
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < NP; j++)
+            reinterpret_cast<float2 *>(red)[(team * NP + j) * TPR + lane] = which ? db[j] : dw[j];
+        __syncthreads();
+        for (int c = threadIdx.x; c < D; c += blockDim.x) {
+            float total = 0.0f;
+            for (int q = 0; q < teams; q++)
+                total += red[q * NP * TPR * 2 + Tile::place(c, q & D & 1)];
+            part[which * D + c] = total;
+        }
+    }
+}
+
 // dw (blockIdx.y 0) and db (1): the parts' sums, 32 columns a block, 8
 // threads a column, each every eighth part, then the 8 in order.
 template <typename WT>
@@ -619,6 +803,59 @@ bool ring_dispatch(int D, F f) {
     if (D <= 128 * NE) return f(Int<128>{});
     if (D <= 256 * NE) return f(Int<256>{});
     if (D <= 512 * NE) return f(Int<512>{});
+    return false;
+}
+
+// Rows of a group for TPR threads a row: whole 16-byte vectors together, one
+// for every team, and 8 KB (a shorter copy is not worth its barrier); 0 when
+// the matrices (null, or dense and 16-byte aligned) or the shared memory do
+// not allow it.  `read` of them go through the ring; `stages` gets what fits,
+// at least 3: one in work, one leaving, one coming.
+struct Groups {
+    int rows_at, stages, threads, blocks;
+    unsigned grid;
+    size_t smem;
+};
+constexpr int kGroupSmem = 212 * 1024;
+bool group_shape(Groups &g, std::initializer_list<const Rows *> all, int read, long long rows,
+                 int D, int size, int tpr, int most) {
+    for (const Rows *m : all)
+        if (m->p && ((uintptr_t)m->p & 15 || (rows > 1 && m->ld != D))) return false;
+    for (int blocks = tpr > kGroupThreads / 4 ? 1 : most; blocks > 0; blocks--) {
+        const int threads = blocks > 1 ? kGroupThreads / 2 : kGroupThreads;
+        int at = threads / tpr;
+        while (at <= kGroupMaxRows &&
+               ((long long)at * D * size % 16 || (long long)at * D * size < 8192))
+            at *= 2;
+        const long long stage = (long long)read * at * D * size;
+        const long long fit = (blocks == 1 ? kGroupSmem : blocks == 2 ? 108 * 1024 : 71 * 1024) / stage;
+        if (at > kGroupMaxRows || fit < 3) continue;
+        g.rows_at = at;
+        g.stages = fit > kRingStages ? kRingStages : (int)fit;
+        g.threads = threads;
+        const long long groups = (rows + at - 1) / at;
+        g.grid = (unsigned)(groups < kSms * blocks ? groups : kSms * blocks);
+        g.smem = (size_t)g.stages * stage;
+        return true;
+    }
+    return false;
+}
+// f(TPR, NP) with the fewest places for rows of D (NARROW: from 33 on, else
+// from 257 on) that keeps WordTile's promise
+template <bool NARROW, typename F>
+bool group_dispatch(int D, F &&f) {
+    if constexpr (NARROW) {
+        if (D <= 80) return f(Int<8>{}, Int<5>{});
+        if (D <= 160) return f(Int<16>{}, Int<5>{});
+    }
+    if (D <= 320) return f(Int<32>{}, Int<5>{});
+    if (D <= 512) return f(Int<32>{}, Int<8>{});
+    if (D <= 640) return f(Int<64>{}, Int<5>{});
+    if (D <= 1024) return f(Int<64>{}, Int<8>{});
+    if (D <= 1280) return f(Int<128>{}, Int<5>{});
+    if (D <= 2048) return f(Int<128>{}, Int<8>{});
+    if (D <= 2560) return f(Int<256>{}, Int<5>{});
+    if (D <= 4096) return f(Int<256>{}, Int<8>{});
     return false;
 }
 
@@ -687,6 +924,27 @@ Status launch_layernorm(const LayerNormArgs &a, cudaStream_t st) {
                  : a.D <= 8192 ? ring(Int<512>{}) : false))
                 return cuda_status();
         }
+        auto group = [&](auto tpr, auto np) {
+            constexpr int TPR = decltype(tpr)::value, NP = decltype(np)::value;
+            Groups g;
+            auto kernel = layernorm_group_kernel<T, WT, TPR, NP>;
+            if (!group_shape(g, {&a.x, &a.res, &a.y, &a.sum}, a.res.p ? 2 : 1, a.rows, a.D, size,
+                             TPR, NP > 5 ? 2 : 3) ||
+                !smem_attr_once((const void *)kernel, kGroupSmem))
+                return false;
+            pdl_launch(kernel, g.grid, g.threads, g.smem, st, (const T *)a.x.p,
+                       (const T *)a.res.p, ptr<T>(a.y), ptr<T>(a.sum), (const WT *)a.weight,
+                       (const WT *)a.bias, a.mean, a.rstd, a.rows, a.D, a.eps, g.rows_at, g.stages);
+            return true;
+        };
+        // other dense rows through groups (50000 x 1153 FP16 63 us, 195 by the
+        // tile; FP32 81 / 110; 200000 x 257 BF16 70 / 129), unless they are
+        // narrow (200000 x 100 BF16 33.0 / 31.4) or few (300 x 1153 FP32 2.8 /
+        // 2.3, 2400 x 641 4.7 / 5.1; the tile's 16-bit loads cost it more: 300
+        // x 1153 BF16 5.0 / 8.3)
+        if (!vec && a.D > 256 && (sizeof(T) == 2 ? a.rows >= kSms : a.rows * a.D >= 3 << 19) &&
+            group_dispatch<false>(a.D, group))
+            return cuda_status();
         // the smallest tile that holds the row, 64 bytes a thread (rows up to
         // 256 values half of that)
         constexpr int NE = sizeof(T) == 2 ? 32 : 16, F = sizeof(T) == 2 ? 1 : 2;
@@ -762,13 +1020,34 @@ Status launch_layernorm_backward(const LayerNormBackwardArgs &a, cudaStream_t st
                        grads ? a.work : nullptr, stages);
             return true;
         };
+        auto group = [&](auto tpr, auto np) {
+            constexpr int TPR = decltype(tpr)::value, NP = decltype(np)::value;
+            Groups g;
+            auto kernel = layernorm_bwd_group_kernel<T, WT, TPR, NP>;
+            if (!group_shape(g, {&a.x, &a.dy, &a.dsum, &a.dx}, a.dsum.p ? 3 : 2, a.rows, a.D, size,
+                             TPR, 2) ||
+                !smem_attr_once((const void *)kernel, kGroupSmem))
+                return false;
+            parts = (int)g.grid;
+            const size_t reduce = (size_t)g.threads * NP * 8;
+            pdl_launch(kernel, g.grid, g.threads, g.smem > reduce ? g.smem : reduce, st,
+                       (const T *)a.dy.p, (const T *)a.x.p, (const T *)a.dsum.p, ptr<T>(a.dx),
+                       (const WT *)a.weight, a.mean, a.rstd, a.rows, a.D, grads ? a.work : nullptr,
+                       g.rows_at, g.stages);
+            return true;
+        };
         // two vectors a thread: 16 values of 16 bits or 8 of 32 (with 16, FP32
         // rows spill; wider than 4096 they have to)
         constexpr int kNE = 32 / (int)sizeof(T);
+        // dense rows that are no vectors go through groups (50000 x 1153 FP16
+        // 112 us, 161 by the tile; FP32 123 / 186; 200000 x 79 BF16 34 / 75),
+        // unless they are narrow (200000 x 51 BF16 36 / 26) or few (4800 x 641
+        // BF16 17.3 / 14.3, 4800 x 1153 19.1 / 24.4)
         const bool done =
             a.rows == 0 ||
-            (vec && (ring_dispatch<kNE>(a.D, [&](auto tpr) { return ring(tpr, Int<kNE>{}); }) ||
-                     (sizeof(T) == 4 && a.D > 4096 && a.D <= 8192 && ring(Int<512>{}, Int<16>{}))));
+            (vec ? ring_dispatch<kNE>(a.D, [&](auto tpr) { return ring(tpr, Int<kNE>{}); }) ||
+                       (sizeof(T) == 4 && a.D > 4096 && a.D <= 8192 && ring(Int<512>{}, Int<16>{}))
+                 : a.D > 64 && a.rows * a.D >= 1 << 22 && group_dispatch<true>(a.D, group));
         if (done) {
         } else if (a.D <= 64) {
             tile(Int<8>{}, Int<8>{});

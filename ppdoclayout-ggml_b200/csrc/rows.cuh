@@ -318,6 +318,229 @@ struct RowRing {
     }
 };
 
+// Values of a row in shared memory at any alignment held by TPR threads as NP
+// pairs each.  16-bit values are read and written as the memory's 32-bit
+// words lane, lane + TPR, ...: a row that starts in the middle of a word
+// (shift 1) holds column c in half (c + 1) % 2 of word (c + 1) / 2, and the
+// words it shares with its neighbours are touched by halves.  FP32 values:
+// columns lane + 2 j TPR and TPR behind it.  The caller promises D >= 2 TPR
+// (NP / 2), so that pairs 1 .. NP / 2 - 1 need no check.
+template <typename T, int TPR, int NP>
+struct WordTile {
+    static constexpr bool kWords = sizeof(T) == 2;
+    struct Raw {
+        uint32_t u[kWords ? NP : 2 * NP];
+    };
+    int lane, shift;
+    uint32_t in[2];  // bit j: the pair's first, second value lies in the row
+
+    __device__ __forceinline__ WordTile(int lane_, int shift_, int D)
+        : lane(lane_), shift(kWords ? shift_ : 0), in{0, 0} {
+#pragma unroll
+        for (int j = 0; j < NP; j++)
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+                if ((unsigned)column(j, h) < (unsigned)D) in[h] |= 1u << j;
+    }
+    __device__ __forceinline__ int column(int j, int h) const {
+        return kWords ? 2 * (lane + j * TPR) + h - shift : lane + (2 * j + h) * TPR;
+    }
+    __device__ __forceinline__ bool inside(int j, int h) const {
+        return (j >= 1 && j < NP / 2) || (in[h] >> j & 1);
+    }
+    // what lies outside is zero
+    __device__ __forceinline__ void load(Raw &r, const T *row) const {
+        if constexpr (kWords) {
+            const uint16_t *v = reinterpret_cast<const uint16_t *>(row) + 2 * lane - shift;
+#pragma unroll
+            for (int j = 0; j < NP; j++, v += 2 * TPR) {
+                r.u[j] = 0;
+                if (inside(j, 0) && inside(j, 1)) r.u[j] = *reinterpret_cast<const uint32_t *>(v);
+                else if (inside(j, 0)) r.u[j] = v[0];
+                else if (inside(j, 1)) r.u[j] = (uint32_t)v[1] << 16;
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 2 * NP; j++) {
+                r.u[j] = 0;
+                if (inside(j / 2, j % 2)) r.u[j] = __float_as_uint(row[lane + j * TPR]);
+            }
+        }
+    }
+    __device__ __forceinline__ void store(T *row, const Raw &r) const {
+        if constexpr (kWords) {
+            uint16_t *v = reinterpret_cast<uint16_t *>(row) + 2 * lane - shift;
+#pragma unroll
+            for (int j = 0; j < NP; j++, v += 2 * TPR) {
+                if (inside(j, 0) && inside(j, 1)) *reinterpret_cast<uint32_t *>(v) = r.u[j];
+                else if (inside(j, 0)) v[0] = (uint16_t)r.u[j];
+                else if (inside(j, 1)) v[1] = (uint16_t)(r.u[j] >> 16);
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 2 * NP; j++)
+                if (inside(j / 2, j % 2)) row[lane + j * TPR] = __uint_as_float(r.u[j]);
+        }
+    }
+    static __device__ __forceinline__ float2 pair(const Raw &r, int j) {
+        if constexpr (kWords) return unpack2<T>(r.u[j]);
+        else return make_float2(__uint_as_float(r.u[2 * j]), __uint_as_float(r.u[2 * j + 1]));
+    }
+    static __device__ __forceinline__ void set_pair(Raw &r, int j, float2 v) {
+        if constexpr (kWords) {
+            r.u[j] = pack2<T>(v.x, v.y);
+        } else {
+            r.u[2 * j] = __float_as_uint(v.x);
+            r.u[2 * j + 1] = __float_as_uint(v.y);
+        }
+    }
+    template <typename WT>
+    __device__ __forceinline__ void load_params(float2 (&p)[NP], const WT *w, float none) const {
+#pragma unroll
+        for (int j = 0; j < NP; j++) {
+            p[j] = both(none);
+            if (w && inside(j, 0)) p[j].x = to_float(w[column(j, 0)]);
+            if (w && inside(j, 1)) p[j].y = to_float(w[column(j, 1)]);
+        }
+    }
+    // where column c of a row with this shift lies in [NP][TPR][2]
+    static __device__ __forceinline__ int place(int c, int shift) {
+        if constexpr (kWords) return c + shift;
+        else return (c / (2 * TPR) * TPR + c % TPR) * 2 + c / TPR % 2;
+    }
+};
+
+// Dense matrices whose rows are no whole 16-byte vectors (an odd number of
+// 16-bit values, say), a group of rows at a time: `rows_at` rows, so many
+// that a group is whole vectors and starts on one.  Groups come through a
+// ring by bulk copies and results, written over what they came from, leave
+// by bulk copies; between the two the rows are read and written in shared
+// memory by WordTile, where neither alignment nor the width of an access
+// costs memory transactions.  The bytes of the last group past its last whole vector
+// are moved by plain loads and stores.  Every wait is bounded; a block that
+// gave up goes on and stores nothing.
+template <typename T, int N>
+struct GroupRing {
+    struct Shared {
+        uint64_t full[kRingStages];
+        int abort_word;
+    };
+    const T *src[N];  // null: no such matrix (the last one only)
+    long long rows, group;  // the present group
+    uint32_t matrix_bytes, full, ring;
+    uint8_t *ptr;
+    int n, stages, D, rows_at, iters;
+    Ring at{1};
+    int *abort_flag, *error;
+    bool good = true;
+
+    __device__ __forceinline__ void setup(const T *const (&s)[N], uint8_t *smem, Shared *shared,
+                                          int *err, long long rows_, int D_, int rows_at_,
+                                          int stages_) {
+#pragma unroll
+        for (int i = 0; i < N; i++) src[i] = s[i];
+        n = src[N - 1] ? N : N - 1;
+        rows = rows_;
+        D = D_;
+        rows_at = rows_at_;
+        stages = stages_;
+        matrix_bytes = (uint32_t)(rows_at * D) * sizeof(T);
+        ptr = smem;
+        ring = smem_u32(smem);
+        full = smem_u32(shared->full);
+        abort_flag = &shared->abort_word;
+        error = err;
+        group = blockIdx.x;
+        const long long groups = (rows + rows_at - 1) / rows_at;
+        iters = group < groups ? (int)((groups - 1 - group) / gridDim.x) + 1 : 0;
+        at = Ring(stages);
+        if (threadIdx.x == 0) {
+            for (int i = 0; i < stages; i++) mbar_init(full + 8 * i, 1);
+            shared->abort_word = 0;
+            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        }
+        __syncthreads();
+    }
+    __device__ __forceinline__ int count(long long g) const {
+        return (int)min((long long)rows_at, rows - g * rows_at);
+    }
+    __device__ __forceinline__ uint32_t group_bytes(long long g) const {
+        return (uint32_t)(count(g) * D) * sizeof(T);
+    }
+    // thread 0: the block's group `it` into its stage
+    __device__ __forceinline__ void fill(int it) {
+        if (it >= iters) return;
+        const int s = it % stages;
+        const long long g = blockIdx.x + (long long)it * gridDim.x;
+        const uint32_t whole = group_bytes(g) & ~15u;
+        mbar_expect_tx(full + 8 * s, (uint32_t)n * whole);
+        if (!whole) return;
+#pragma unroll
+        for (int i = 0; i < N; i++)
+            if (i < n)
+                bulk_load(ring + (uint32_t)(s * n + i) * matrix_bytes, src[i] + g * rows_at * D,
+                          whole, full + 8 * s);
+    }
+    __device__ __forceinline__ void start() {
+        if (threadIdx.x == 0)
+            for (int it = 0; it < stages; it++) fill(it);
+    }
+    __device__ __forceinline__ T *buffer(int i) const {
+        return reinterpret_cast<T *>(ptr + (uint32_t)(at.i * n + i) * matrix_bytes);
+    }
+    // all threads: the present group is in its buffers
+    __device__ __forceinline__ void wait() {
+        good &= mbar_wait_bounded(full + 8 * at.i, at.ph, abort_flag, error);
+        const uint32_t bytes = group_bytes(group);
+        if (bytes & 15u) {
+            const int first = (int)((bytes & ~15u) / sizeof(T)), last = (int)(bytes / sizeof(T));
+            if ((int)threadIdx.x < last - first)
+#pragma unroll
+                for (int i = 0; i < N; i++)
+                    if (i < n)
+                        buffer(i)[first + threadIdx.x] =
+                            src[i][group * rows_at * D + first + threadIdx.x];
+            __syncthreads();
+        }
+    }
+    // all threads, their results written: matrix i of the stage goes to dst,
+    // and j (when given one) to dst2; the stage before this one, read out by
+    // now, is filled again
+    __device__ __forceinline__ void store(int it, int i, T *dst, int j, T *dst2) {
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncthreads();
+        const uint32_t bytes = group_bytes(group), whole = bytes & ~15u;
+        const long long at_value = group * rows_at * D;
+        if (threadIdx.x == 0) {
+            if (*(volatile int *)abort_flag) good = false;
+            if (good && whole) {
+                bulk_store(dst + at_value, ring + (uint32_t)(at.i * n + i) * matrix_bytes, whole);
+                if (dst2)
+                    bulk_store(dst2 + at_value, ring + (uint32_t)(at.i * n + j) * matrix_bytes,
+                               whole);
+            }
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+            if (it > 0) {
+                asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+                fill(it - 1 + stages);
+            }
+        }
+        if ((bytes & 15u) && good) {
+            const int first = (int)(whole / sizeof(T)), last = (int)(bytes / sizeof(T));
+            if ((int)threadIdx.x < last - first) {
+                dst[at_value + first + threadIdx.x] = buffer(i)[first + threadIdx.x];
+                if (dst2) dst2[at_value + first + threadIdx.x] = buffer(j)[first + threadIdx.x];
+            }
+        }
+        at.next();
+        group += gridDim.x;
+    }
+    // thread 0 leaves last: its stores have been written
+    __device__ __forceinline__ void finish() {
+        if (threadIdx.x == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    }
+};
+
 // stages of a block's rings in `bytes` of shared memory
 inline int ring_stages(long long bytes, long long stage) {
     const long long n = bytes / stage;

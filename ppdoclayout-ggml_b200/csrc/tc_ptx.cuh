@@ -68,6 +68,14 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_
         "l"(src), "r"(bytes), "r"(bar)
         : "memory");
 }
+// `bytes` (a multiple of 16) from shared to global memory, both 16-byte
+// aligned, in the calling thread's bulk group; the source is published by
+// fence.proxy.async first
+__device__ __forceinline__ void bulk_store(void *dst, uint32_t src, uint32_t bytes) {
+    asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(src),
+                 "r"(bytes)
+                 : "memory");
+}
 // Position in a ring of n stages or slots: index and mbarrier phase parity,
 // advanced by one step at a time (no division on the issue paths).
 struct Ring {

@@ -218,6 +218,51 @@ def test_layernorm_backward_strided(cuda, D):
             close(a, b, c)
 
 
+DENSE = [(148, 1), (153, 3), (161, 33), (2501, 79), (149, 257), (1000, 322), (5, 1153), (64001, 79),
+         (35003, 129), (17001, 257), (13101, 322), (8195, 513), (6601, 641), (4098, 1027), (3651, 1153),
+         (3303, 1281), (2051, 2049), (1661, 2561), (1027, 4095), (1031, 4097), (50001, 100)]
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("rows,D", DENSE)
+def test_layernorm_dense_odd_rows(cuda, rows, D, t):
+    """Dense rows that are no whole vectors, the last ones of which end inside
+    one: both directions, results over inputs, and nothing behind the last row."""
+    T = TYPES[t]
+    g = gen(rows + D)
+
+    def guarded(v):
+        room = torch.full((rows * D + 64,), 7.0, device="cuda", dtype=T)
+        room[:rows * D] = v.reshape(-1)
+        return room, room[:rows * D].view(rows, D)
+
+    (xr, x), (rr, r) = guarded(normal(g, rows, D, t=T, scale=2.0, shift=0.7)), guarded(normal(g, rows, D, t=T))
+    w, b = normal(g, D, t=T, shift=1.0, scale=0.3), normal(g, D, t=T, scale=0.3)
+    want = ln_want(x, w, b, 1e-5, r)
+    y, s, mean, rstd = ppdl.layernorm(x, w, b, 1e-5, residual=r, return_sum=True, return_stats=True)
+    close(y, want[0], want[4])
+    assert torch.equal(s.double(), want[1])
+    close(mean, want[2], want[5] + U * want[2].abs())
+    close(rstd, want[3], want[6] + U * want[3])
+    plain, bare = ppdl.layernorm(x, w, b, 1e-5), ln_want(x, w, b, 1e-5)
+    close(plain, bare[0], bare[4])
+    code, stream = {"f32": 0, "bf16": 1, "f16": 2}[t], torch.cuda.current_stream().cuda_stream
+    dyr, dy = guarded(normal(g, rows, D, t=T))
+    dx, dw, db = ppdl.layernorm_backward(dy, s, w, mean, rstd, dsum=r)
+    wants, tol = bwd_want(dy, s, w, mean, rstd, r)
+    for got, a, c in zip((dx, dw, db), wants, tol):
+        close(got, a, c)
+    ppdl.check(ppdl.lib().ppdl_layernorm_backward(
+        dy.data_ptr(), D, s.data_ptr(), D, w.data_ptr(), mean.data_ptr(), rstd.data_ptr(), r.data_ptr(), D,
+        code, code, rows, D, dy.data_ptr(), D, None, None, None, stream))
+    assert torch.equal(dy, dx) and (dyr[rows * D:] == 7).all()
+    ppdl.check(ppdl.lib().ppdl_layernorm(
+        x.data_ptr(), D, r.data_ptr(), D, w.data_ptr(), b.data_ptr(), code, code, rows, D, 1e-5,
+        x.data_ptr(), D, r.data_ptr(), D, None, None, stream))
+    assert torch.equal(x, y) and torch.equal(r, s)
+    assert (xr[rows * D:] == 7).all() and (rr[rows * D:] == 7).all()
+
+
 def test_layernorm_backward_no_rows(cuda):
     """No rows: the weights' gradients are zeros, not what the memory held."""
     x, s = torch.empty((0, 300), device="cuda"), torch.empty(0, device="cuda")
