@@ -17,6 +17,7 @@
 #include "rows.cuh"
 
 #include <initializer_list>
+#include <type_traits>
 #include "tc_ptx.cuh"
 
 namespace ppdl {
@@ -399,24 +400,134 @@ __global__ void layernorm_dx_row_kernel(const T *dy, long long lddy, const T *x,
     }
 }
 
-// Column sums of dy xh and dy over the row chunk blockIdx.y, one column per
-// thread, into part[chunk][2][D].
-template <typename T>
-__global__ void layernorm_dw_column_kernel(const T *dy, long long lddy, const T *x, long long ldx,
-                                           const float *mean, const float *rstd, long long rows,
-                                           int D, long long chunk, float *part) {
+// dx, one block of TPR threads per row of at most TPR * NE values, read once.
+// VEC: whole 16-byte vectors at aligned places.
+template <typename T, typename WT, int TPR, int NE, bool VEC>
+__global__ void __launch_bounds__(TPR)
+layernorm_dx_tile_kernel(const T *dy, long long lddy, const T *x, long long ldx, const T *dsum,
+                         long long lddsum, T *dx, long long lddx, const WT *w,
+                         const float *mean_in, const float *rstd_in, int D) {
     pdl_begin();
-    const int c = blockIdx.x * blockDim.x + threadIdx.x;
-    if (c >= D) return;
-    const long long r0 = blockIdx.y * chunk, r1 = min(rows, r0 + chunk);
-    float sw = 0.0f, sb = 0.0f;
-    for (long long r = r0; r < r1; r++) {
-        const float g = to_float(dy[r * lddy + c]);
-        sw += g * ((to_float(x[r * ldx + c]) - mean[r]) * rstd[r]);
-        sb += g;
+    pdl_trigger();
+    __shared__ float sh[32];
+    const int lane = threadIdx.x;
+    const long long row = blockIdx.x;
+    const float rstd = rstd_in[row], inv_d = 1.0f / (float)D;
+    // x r - mean r: off by the rounding of mean r, u |mean| r
+    const float mr = -mean_in[row] * rstd;
+    if constexpr (VEC) {
+        using Tile = PairTile<T, TPR, NE>;
+        constexpr int kHalf = Tile::kVec / 2;
+        typename Tile::Raw rx, rd;
+        Tile::load(rx, x + row * ldx, D, lane);
+        Tile::load(rd, dy + row * lddy, D, lane);
+        const bool wide = sizeof(WT) * Tile::kVec >= 16 && ((uintptr_t)w & 15) == 0;
+        float2 g[NE / 2], t0 = both(0.0f), t1 = both(0.0f);
+#pragma unroll
+        for (int i = 0; i < Tile::kVecs; i++) {
+            float2 p[kHalf];
+            Tile::vector_params(p, w, 1.0f, i, D, lane, wide);
+#pragma unroll
+            for (int k = 0; k < kHalf; k++) {
+                const int j = i * kHalf + k;
+                g[j] = mul2(Tile::pair(rd, j), p[k]);
+                t0 = add2(t0, g[j]);
+                t1 = fma2(g[j], fma2(Tile::pair(rx, j), both(rstd), both(mr)), t1);
+            }
+        }
+        const float s0 = block_sum(t0.x + t0.y, sh), s1 = block_sum(t1.x + t1.y, sh);
+        const float2 m1 = both(-s0 * inv_d * rstd), m2 = both(-s1 * inv_d * rstd);
+        if (dsum) Tile::load(rd, dsum + row * lddsum, D, lane);
+#pragma unroll
+        for (int j = 0; j < NE / 2; j++) {
+            const float2 xh = fma2(Tile::pair(rx, j), both(rstd), both(mr));
+            float2 v = fma2(g[j], both(rstd), fma2(xh, m2, m1));
+            if (dsum) v = add2(v, Tile::pair(rd, j));
+            Tile::set_pair(rx, j, v);
+        }
+        Tile::store(dx + row * lddx, rx, D, lane);
+    } else {
+        using Tile = RowTile<T, TPR, NE>;
+        typename Tile::Raw rx, rd;
+        Tile::load(rx, x + row * ldx, D, lane);
+        Tile::load(rd, dy + row * lddy, D, lane);
+        float g[NE], t0 = 0.0f, t1 = 0.0f;
+        Tile::load_params(g, w, 1.0f, D, lane);
+#pragma unroll
+        for (int j = 0; j < NE; j++) {
+            g[j] *= to_float(rd.v[j]);
+            t0 += g[j];
+            t1 += g[j] * (to_float(rx.v[j]) * rstd + mr);
+        }
+        const float m1 = block_sum(t0, sh) * inv_d, m2 = block_sum(t1, sh) * inv_d;
+        if (dsum) Tile::load(rd, dsum + row * lddsum, D, lane);
+#pragma unroll
+        for (int j = 0; j < NE; j++) {
+            float v = (g[j] - m1 - (to_float(rx.v[j]) * rstd + mr) * m2) * rstd;
+            if (dsum) v += to_float(rd.v[j]);
+            rx.v[j] = from_float<T>(v);
+        }
+        Tile::store(dx + row * lddx, rx, D, lane);
     }
-    part[((long long)blockIdx.y * 2) * D + c] = sw;
-    part[((long long)blockIdx.y * 2 + 1) * D + c] = sb;
+}
+
+// Column sums of dy xh and dy over the row chunk blockIdx.y and the 32 * NE
+// columns of blockIdx.x, into part[chunk][2][D]: 8 warps take the chunk's rows
+// in turn, NE columns a lane.
+template <typename T, int NE, bool VEC>
+__global__ void __launch_bounds__(256)
+layernorm_dw_column_kernel(const T *dy, long long lddy, const T *x, long long ldx,
+                           const float *mean, const float *rstd, long long rows, int D,
+                           long long chunk, float *part) {
+    pdl_begin();
+    pdl_trigger();
+    __shared__ float red[2][8][32 * NE];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c0 = blockIdx.x * 32 * NE;
+    const int left = D - c0;  // the warps' rows are the columns from c0 on
+    const long long r0 = blockIdx.y * chunk, r1 = min(rows, r0 + chunk);
+    using Tile = std::conditional_t<VEC, PairTile<T, 32, NE>, RowTile<T, 32, NE>>;
+    float sw[NE], sb[NE];
+#pragma unroll
+    for (int j = 0; j < NE; j++) sw[j] = sb[j] = 0.0f;
+    dy += c0;
+    x += c0;
+#pragma unroll 2
+    for (long long r = r0 + warp; r < r1; r += 8) {
+        typename Tile::Raw rx, rd;
+        Tile::load(rx, x + r * ldx, left, lane);
+        Tile::load(rd, dy + r * lddy, left, lane);
+        const float s = rstd[r], mr = -mean[r] * s;
+#pragma unroll
+        for (int j = 0; j < NE; j++) {
+            float g, v;
+            if constexpr (VEC) {
+                g = j % 2 ? Tile::pair(rd, j / 2).y : Tile::pair(rd, j / 2).x;
+                v = j % 2 ? Tile::pair(rx, j / 2).y : Tile::pair(rx, j / 2).x;
+            } else {
+                g = to_float(rd.v[j]);
+                v = to_float(rx.v[j]);
+            }
+            sw[j] += g * (v * s + mr);
+            sb[j] += g;
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < NE; j++) {
+        int c;
+        if constexpr (VEC) c = Tile::pair_column(j / 2, lane) + j % 2;
+        else c = Tile::column(j, lane);
+        red[0][warp][c] = sw[j];
+        red[1][warp][c] = sb[j];
+    }
+    __syncthreads();
+    part += (long long)blockIdx.y * 2 * D + c0;
+    for (int t = threadIdx.x; t < 2 * 32 * NE; t += 256) {
+        const int which = t / (32 * NE), c = t % (32 * NE);
+        if (c >= left) continue;
+        float sum = 0.0f;
+        for (int q = 0; q < 8; q++) sum += red[which][q][c];
+        part[(long long)which * D + c] = sum;
+    }
 }
 
 // The whole backward pass in one reading of dy and x: TPR threads hold a row
@@ -778,6 +889,7 @@ __global__ void __launch_bounds__(256) layernorm_dw_sum_kernel(const float *part
 
 // blocks that keep column sums, at most: two on each of 148 SMs
 constexpr int kMaxParts = 296;
+constexpr int kBwdTileMax = 4096;
 int row_parts(long long rows) { return (int)(rows < kMaxParts ? rows : kMaxParts); }
 
 // f(T{}, WT{}) for the element types of rows and weights
@@ -1059,22 +1171,35 @@ Status launch_layernorm_backward(const LayerNormBackwardArgs &a, cudaStream_t st
             tile(Int<128>{}, Int<8>{});
         } else if (a.D <= 2048) {
             tile(Int<256>{}, Int<8>{});
-        } else if (a.D <= 4096) {
+        } else if (a.D <= kBwdTileMax) {
             tile(Int<512>{}, Int<8>{});
-        } else if (a.D <= 8192) {
-            tile(Int<1024>{}, Int<8>{});
         } else {
-            pdl_launch(layernorm_dx_row_kernel<T, WT>, (unsigned)a.rows, 512, 0, st,
-                       (const T *)a.dy.p, a.dy.ld, (const T *)a.x.p, a.x.ld,
-                       (const T *)a.dsum.p, a.dsum.ld, ptr<T>(a.dx), a.dx.ld, (const WT *)a.weight,
-                       a.mean, a.rstd, a.D);
-            if (grads) {
-                const long long chunk = (a.rows + row_parts(a.rows) - 1) / row_parts(a.rows);
+            // two readings: dx row by row, the weights' gradients column by
+            // column
+            auto dx = [&](auto kernel, int threads) {
+                pdl_launch(kernel, (unsigned)a.rows, threads, 0, st, (const T *)a.dy.p, a.dy.ld,
+                           (const T *)a.x.p, a.x.ld, (const T *)a.dsum.p, a.dsum.ld, ptr<T>(a.dx),
+                           a.dx.ld, (const WT *)a.weight, a.mean, a.rstd, a.D);
+            };
+            auto column = [&](auto kernel, int ne) {
+                // some 8 blocks of 8 warps an SM, at least 16 chunks of rows
+                const long long across = (a.D + 32 * ne - 1) / (32 * ne);
+                const long long want = (8 * kSms + across - 1) / across;
+                const long long most = row_parts(a.rows);
+                const long long n = want < 16 ? 16 : want, cut = n < most ? n : most;
+                const long long chunk = (a.rows + cut - 1) / cut;
                 parts = (int)((a.rows + chunk - 1) / chunk);
-                pdl_launch(layernorm_dw_column_kernel<T>, dim3(cdiv(a.D, 128), parts), 128, 0, st,
-                           (const T *)a.dy.p, a.dy.ld, (const T *)a.x.p, a.x.ld, a.mean, a.rstd,
-                           a.rows, a.D, chunk, a.work);
-            }
+                pdl_launch(kernel, dim3((unsigned)across, parts), 256, 0, st, (const T *)a.dy.p,
+                           a.dy.ld, (const T *)a.x.p, a.x.ld, a.mean, a.rstd, a.rows, a.D, chunk,
+                           a.work);
+            };
+            if (vec && a.D <= 16384) dx(layernorm_dx_tile_kernel<T, WT, 1024, 16, true>, 1024);
+            else if (!vec && a.D <= 8192) dx(layernorm_dx_tile_kernel<T, WT, 512, 16, false>, 512);
+            else if (!vec && a.D <= 16384) dx(layernorm_dx_tile_kernel<T, WT, 1024, 16, false>, 1024);
+            else dx(layernorm_dx_row_kernel<T, WT>, 512);
+            constexpr int kVec = 16 / (int)sizeof(T);
+            if (grads && vec) column(layernorm_dw_column_kernel<T, kVec, true>, kVec);
+            else if (grads) column(layernorm_dw_column_kernel<T, 4, false>, 4);
         }
         if (grads)
             pdl_launch(layernorm_dw_sum_kernel<WT>, dim3(cdiv(a.D, 32), 2), 256, 0, st, a.work,
