@@ -403,7 +403,7 @@ __global__ void layernorm_dx_row_kernel(const T *dy, long long lddy, const T *x,
 // dx, one block of TPR threads per row of at most TPR * NE values, read once.
 // VEC: whole 16-byte vectors at aligned places.
 template <typename T, typename WT, int TPR, int NE, bool VEC>
-__global__ void __launch_bounds__(TPR)
+__global__ void __launch_bounds__(TPR, 1024 / TPR)
 layernorm_dx_tile_kernel(const T *dy, long long lddy, const T *x, long long ldx, const T *dsum,
                          long long lddsum, T *dx, long long lddx, const WT *w,
                          const float *mean_in, const float *rstd_in, int D) {
@@ -889,7 +889,6 @@ __global__ void __launch_bounds__(256) layernorm_dw_sum_kernel(const float *part
 
 // blocks that keep column sums, at most: two on each of 148 SMs
 constexpr int kMaxParts = 296;
-constexpr int kBwdTileMax = 4096;
 int row_parts(long long rows) { return (int)(rows < kMaxParts ? rows : kMaxParts); }
 
 // f(T{}, WT{}) for the element types of rows and weights
@@ -1171,11 +1170,12 @@ Status launch_layernorm_backward(const LayerNormBackwardArgs &a, cudaStream_t st
             tile(Int<128>{}, Int<8>{});
         } else if (a.D <= 2048) {
             tile(Int<256>{}, Int<8>{});
-        } else if (a.D <= kBwdTileMax) {
+        } else if (a.D <= 4096) {
             tile(Int<512>{}, Int<8>{});
         } else {
             // two readings: dx row by row, the weights' gradients column by
-            // column
+            // column (14000 x 4097 BF16 228 us, in one reading with 1024
+            // threads a row and one block an SM 397; 100 x 5001 FP32 8.4 / 12)
             auto dx = [&](auto kernel, int threads) {
                 pdl_launch(kernel, (unsigned)a.rows, threads, 0, st, (const T *)a.dy.p, a.dy.ld,
                            (const T *)a.x.p, a.x.ld, (const T *)a.dsum.p, a.dsum.ld, ptr<T>(a.dx),
