@@ -12,12 +12,22 @@
 // so that the backward pass (which reads the stored sum) differentiates the
 // function that ran.  The variance is the sum of squared deviations from the
 // mean, not a difference of moments, so a large common offset costs nothing.
+//
+// Memory bounds all of it: a few operations a value, and every value is read
+// and written once.  Measured (copy rate 6.54 TB/s): forward 52500 x 256 FP32
+// with residual, stored sum and statistics 33.6 us (98 % of it), 8192 x 4096
+// BF16 30.1 (68 %), backward 16384 x 4096 BF16 84.4 (73 %), 52500 x 256 FP32
+// 33 (75 %); one row of 4096 3.1 us, 2400 x 256 backward 8 us in two kernels,
+// which is latency.  Rows in registers for what has few rows or is narrow;
+// rings of bulk copies where more bytes have to be in flight than registers
+// hold; groups of rows through shared memory where rows are no whole vectors;
+// one value at a time for the rest.
+#include <initializer_list>
+#include <type_traits>
+
 #include "block.cuh"
 #include "block.h"
 #include "rows.cuh"
-
-#include <initializer_list>
-#include <type_traits>
 #include "tc_ptx.cuh"
 
 namespace ppdl {
@@ -289,8 +299,10 @@ layernorm_ring_kernel(const T *x, long long ldx, const T *res, long long ldres, 
 }
 
 // Dense rows that are no whole 16-byte vectors, groups of them through shared
-// memory (GroupRing): one block of 512 threads on each SM, TPR threads a row,
-// weights and biases in registers.
+// memory (GroupRing), TPR threads a row, weights and biases in registers.
+// Row by row, a warp's 16-bit loads are 64 bytes each and at any alignment
+// two transactions, and a thread has 32 of them (50000 x 1153 FP16 195 us,
+// so 63, 56 % of the copy rate: the barriers' latency bounds it now).
 constexpr int kGroupThreads = 512, kGroupMaxRows = 128;
 template <typename T, typename WT, int TPR, int NP>
 __global__ void __launch_bounds__(kGroupThreads, 1)
@@ -917,13 +929,16 @@ bool ring_dispatch(int D, F f) {
     return false;
 }
 
-// Rows of a group for TPR threads a row: whole 16-byte vectors together, one
-// for every team, and 8 KB (a shorter copy is not worth its barrier); 0 when
-// the matrices (null, or dense and 16-byte aligned) or the shared memory do
-// not allow it.  `read` of them go through the ring; `stages` gets what fits,
-// at least 3: one in work, one leaving, one coming.
+// How groups of rows are taken by teams of tpr threads: whole 16-byte vectors
+// together, a row for every team, and 8 KB (a shorter copy is not worth its
+// barrier).  `read` matrices go through the ring, of at least 3 stages: one in
+// work, one leaving, one coming.  `most` blocks of 256 threads on an SM, when
+// their rings fit, or two, or one of 512: a block that waits at its barriers
+// leaves the SM to the others (50000 x 1153 FP16 forward 63 us with three,
+// with one 90; backward 200000 x 257 BF16 108 with two, with one 142).  False when a matrix is neither
+// null nor dense and 16-byte aligned, or nothing fits.
 struct Groups {
-    int rows_at, stages, threads, blocks;
+    int rows_at, stages, threads;
     unsigned grid;
     size_t smem;
 };

@@ -1,5 +1,9 @@
 // quantize.cu — 8-bit rows with a scale each: scale = max |x| / 127,
 // q = x / scale rounded half to even on the exact quotient.
+//
+// Memory bounds it (a row stays in registers between its maximum and its
+// quotients): 8192 x 8192 BF16 46 us, 4.4 TB/s; 52500 x 256 FP32 10.5 us, its
+// input partly in L2.
 #include "block.cuh"
 #include "block.h"
 #include "quantize.cuh"

@@ -11,6 +11,11 @@
 // frequency is taken in turns (revolutions) in 64 bits, whole turns are
 // dropped, and only the fraction in [-1/2, 1/2] goes through the FP32 sine
 // and cosine.
+//
+// Memory bounds it, once the turns are made once a token and not once a
+// head: 8 x 2500 tokens of 16 + 16 heads x 64 FP32 50.7 us (99 % of the copy
+// rate), 4 x 4096 tokens of 32 + 8 heads x 128 BF16 62.6 (82 %); 64 new
+// tokens of 32 + 8 heads 2.4 us, which is latency.
 #include "block.cuh"
 #include "block.h"
 
@@ -232,7 +237,8 @@ Status launch_rotary(const RotaryArgs &a, cudaStream_t st) {
         const long long per_token = (long long)heads * g.all;
         if (vector_heads(a, (int)sizeof(T)) && per_token < (1 << 20)) {
             // about four units a thread, as long as all SMs have blocks
-            // (20000 tokens of 256 units: 4 tokens a block 60 us, 1 token 70)
+            // (4 x 4096 tokens of 40 heads x 128 BF16 62.6 us, with one token
+            // a block 82.6; of 5 heads x 32 15.3 / 131)
             long long per = 1024 / per_token;
             if (per > tokens / (8 * 148)) per = tokens / (8 * 148);
             if (per > 4096 / pairs) per = 4096 / pairs;  // 32 KB of table

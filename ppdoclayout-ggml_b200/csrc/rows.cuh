@@ -209,9 +209,8 @@ struct PairTile {
 // behind a barrier of the team, by one of its warps in turn, so that the
 // copies' issue is neither on one warp's path nor repeated by all (with a
 // slice of the row for every warp the backward pass of 16384 x 4096 BF16 took
-// 95 us, so 84.4).  Every wait is bounded; a
-// thread that gave up goes on through its rows (barriers stay matched) and
-// stores nothing.
+// 95 us, so 84.4).  Every wait is bounded; a thread that gave up goes on
+// through its rows (barriers stay matched) and stores nothing.
 constexpr int kRingStages = 8;  // at most
 
 template <typename T, int TPR, int NE, int THREADS, int N>
