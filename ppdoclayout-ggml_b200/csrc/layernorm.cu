@@ -296,6 +296,7 @@ layernorm_ring_kernel(const T *x, long long ldx, const T *res, long long ldres, 
         if (mean_out) mean_out += ring.step;
         if (rstd_out) rstd_out += ring.step;
     }
+    ring.finish();
 }
 
 // Dense rows that are no whole 16-byte vectors, groups of them through shared
@@ -739,6 +740,7 @@ layernorm_bwd_ring_kernel(const T *dy, long long lddy, const T *x, long long ldx
             Tile::store(dx, out, D, lane);
         }
     }
+    ring.finish();
     if (!part) return;
     part += (long long)blockIdx.x * 2 * D;
     if constexpr (kRows == 1) {

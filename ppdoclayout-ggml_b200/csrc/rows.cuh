@@ -199,6 +199,15 @@ struct PairTile {
     }
 };
 
+// After a wait that gave up: what is still on its way into a ring (`fills`
+// stages in turn, all of them issued) lands before the block may exit.
+__device__ __forceinline__ void ring_drain(uint32_t full, int stages, int fills, int *error) {
+    for (int s = 0; s < stages && s < fills; s++) {
+        int none = 0;
+        mbar_wait_bounded(full + 8 * s, (uint32_t)((fills - 1 - s) / stages & 1), &none, error);
+    }
+}
+
 // Rows (of whole 16-byte vectors) through rings of buffers in shared memory,
 // several rows ahead, by bulk copies.  With one row ahead in registers an
 // iteration takes a memory latency, and the rows that two or three blocks
@@ -210,7 +219,8 @@ struct PairTile {
 // copies' issue is neither on one warp's path nor repeated by all (with a
 // slice of the row for every warp the backward pass of 16384 x 4096 BF16 took
 // 95 us, so 84.4).  Every wait is bounded; a thread that gave up goes on
-// through its rows (barriers stay matched) and stores nothing.
+// through its rows (barriers stay matched), stores nothing and drains the
+// ring.
 constexpr int kRingStages = 8;  // at most
 
 template <typename T, int TPR, int NE, int THREADS, int N>
@@ -314,6 +324,10 @@ struct RowRing {
     __device__ __forceinline__ void refill() {
         if (TPR <= 32) __syncwarp();
         fill(at.i);
+    }
+    // behind the last row
+    __device__ __forceinline__ void finish() {
+        if (!good) ring_drain(full, stages, iters, error);
     }
 };
 
@@ -536,6 +550,7 @@ struct GroupRing {
     }
     // thread 0 leaves last: its stores have been written
     __device__ __forceinline__ void finish() {
+        if (!good) ring_drain(full, stages, iters, error);
         if (threadIdx.x == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     }
 };
