@@ -622,7 +622,7 @@ layernorm_bwd_tile_kernel(const T *dy, long long lddy, const T *x, long long ldx
     if constexpr (kRows == 1) {
 #pragma unroll
         for (int j = 0; j < NE; j++) {
-            const int c = Tile::column(j / Tile::kVec, lane) + j % Tile::kVec;
+            const int c = Tile::column(j, lane);
             if (c < D) {
                 part[c] = dw[j];
                 part[D + c] = db[j];
@@ -637,7 +637,7 @@ layernorm_bwd_tile_kernel(const T *dy, long long lddy, const T *x, long long ldx
             __syncthreads();
             for (int t = threadIdx.x; t < TPR * NE; t += kThreads) {
                 const int j = t / TPR, l = t % TPR;
-                const int c = Tile::column(j / Tile::kVec, l) + j % Tile::kVec;
+                const int c = Tile::column(j, l);
                 if (c < D) {
                     float sum = 0.0f;
                     for (int q = 0; q < kRows; q++) sum += red[q * NE * TPR + t];

@@ -15,36 +15,29 @@ template <int V>
 using Int = std::integral_constant<int, V>;
 
 // TPR threads hold one row of at most TPR * NE values, NE each, value by
-// value (any alignment): neighbours in groups of GROUP (1: consecutive lanes
-// hold consecutive values).
-template <typename T, int TPR, int NE, int GROUP = 1>
+// value (any alignment): consecutive lanes hold consecutive values.
+template <typename T, int TPR, int NE>
 struct RowTile {
-    static constexpr int kVec = GROUP, kVecs = NE / GROUP;
-    static_assert(NE % GROUP == 0, "whole groups");
-
     struct Raw {
         T v[NE];
     };
 
-    // column of the first value of group i
-    static __device__ __forceinline__ int column(int i, int lane) {
-        return (i * TPR + lane) * GROUP;
-    }
+    static __device__ __forceinline__ int column(int j, int lane) { return j * TPR + lane; }
     static __device__ __forceinline__ void load(Raw &r, const T *row, int D, int lane) {
 #pragma unroll
         for (int j = 0; j < NE; j++) {
             r.v[j] = from_float<T>(0.0f);
-            if (inside(j, D, lane)) r.v[j] = row[column(j / GROUP, lane) + j % GROUP];
+            if (inside(j, D, lane)) r.v[j] = row[column(j, lane)];
         }
     }
     static __device__ __forceinline__ void store(T *row, const Raw &r, int D, int lane) {
 #pragma unroll
         for (int j = 0; j < NE; j++)
-            if (inside(j, D, lane)) row[column(j / GROUP, lane) + j % GROUP] = r.v[j];
+            if (inside(j, D, lane)) row[column(j, lane)] = r.v[j];
     }
     // true for value j of the tile inside the row
     static __device__ __forceinline__ bool inside(int j, int D, int lane) {
-        return column(j / GROUP, lane) + j % GROUP < D;
+        return column(j, lane) < D;
     }
     // parameters (weights) at the tile's columns, `none` where w is null
     template <typename WT>
@@ -53,7 +46,7 @@ struct RowTile {
 #pragma unroll
         for (int j = 0; j < NE; j++) {
             p[j] = none;
-            if (w && inside(j, D, lane)) p[j] = to_float(w[column(j / GROUP, lane) + j % GROUP]);
+            if (w && inside(j, D, lane)) p[j] = to_float(w[column(j, lane)]);
         }
     }
 };

@@ -325,6 +325,30 @@ def test_quantize_rows(cuda, rows, K, t):
         assert torch.equal(s, ws) and torch.equal(q, wq)
 
 
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("rows,K", [(16001, 67), (12001, 99), (8201, 131), (4099, 257), (3301, 322),
+                                    (2101, 513), (1003, 1153), (901, 1281), (521, 2049), (271, 4095),
+                                    (301, 4097)])
+def test_quantize_dense_odd_rows(cuda, rows, K, t):
+    """Dense rows that are no whole vectors, among them zeros, an infinity and
+    a NaN; nothing is written past a row's K values."""
+    g = gen(rows + K)
+    x = normal(g, rows, K, t=TYPES[t], scale=3.0)
+    x[1], x[rows - 2, K - 1], x[rows // 2, 0] = 0, float("inf"), float("nan")
+    ldq = (K + 31) // 16 * 16
+    q = torch.full((rows, ldq), 55, device="cuda", dtype=torch.int8)
+    scale = torch.empty(rows, device="cuda")
+    ppdl.check(ppdl.lib().ppdl_quantize_rows_i8(
+        x.data_ptr(), K, {"f32": 0, "bf16": 1, "f16": 2}[t], rows, K, q.data_ptr(), ldq,
+        scale.data_ptr(), torch.cuda.current_stream().cuda_stream))
+    bad = torch.zeros(rows, dtype=torch.bool)
+    bad[[rows - 2, rows // 2]] = True
+    want, ws = q_want(x[~bad])
+    assert torch.equal(q[~bad][:, :K], want) and torch.equal(scale[~bad], ws)
+    assert (q[bad][:, :K] == 0).all() and not scale[bad].isfinite().any()
+    assert (q[:, K:] == 55).all()
+
+
 def test_quantize_ties_and_extremes(cuda):
     """Ties on exact halves go to the even neighbour; quotients next to a half
     fall on their own side; tiny, zero, infinite and NaN rows."""
