@@ -301,9 +301,9 @@ layernorm_ring_kernel(const T *x, long long ldx, const T *res, long long ldres, 
 
 // Dense rows that are no whole 16-byte vectors, groups of them through shared
 // memory (GroupRing), TPR threads a row, weights and biases in registers.
-// Row by row, a warp's 16-bit loads are 64 bytes each and at any alignment
-// two transactions, and a thread has 32 of them (50000 x 1153 FP16 195 us,
-// so 63, 56 % of the copy rate: the barriers' latency bounds it now).
+// Row by row, a warp's loads are of one value a lane, 16-bit ones 64 bytes for
+// a whole instruction (16771 x 2001 BF16 48.7 us, so 38.8, 53 % of the copy
+// rate: the barriers' latency bounds it now).
 constexpr int kGroupThreads = 512, kGroupMaxRows = 128;
 template <typename T, typename WT, int TPR, int NP>
 __global__ void __launch_bounds__(kGroupThreads, 1)
@@ -1065,33 +1065,51 @@ Status launch_layernorm(const LayerNormArgs &a, cudaStream_t st) {
                        (const WT *)a.bias, a.mean, a.rstd, a.rows, a.D, a.eps, g.rows_at, g.stages);
             return true;
         };
-        // other dense rows through groups (50000 x 1153 FP16 63 us, 195 by the
-        // tile; FP32 81 / 110; 200000 x 257 BF16 70 / 129), unless they are
-        // narrow (200000 x 100 BF16 33.0 / 31.4) or few (300 x 1153 FP32 2.8 /
-        // 2.3, 2400 x 641 4.7 / 5.1; the tile's 16-bit loads cost it more: 300
-        // x 1153 BF16 5.0 / 8.3)
-        if (!vec && a.D > 256 && (sizeof(T) == 2 ? a.rows >= kSms : a.rows * a.D >= 3 << 19) &&
+        // other dense rows through groups (16771 x 2001 BF16 38.8 us, by the
+        // tile 48.7; 29104 x 1153 40.2 / 49.9; 52350 x 641 FP32 56.6 / 85.5),
+        // unless they are narrow (200000 x 100 BF16 33.0 / 31.4) or few (3640 x
+        // 1153 8.9 / 7.5, 2043 x 257 3.6 / 2.5), or FP32 with a residual (29101
+        // x 1153 96 / 80: three stages of two matrices leave one block an SM)
+        if (!vec && a.D > 256 && a.rows * a.D >= 1 << 22 && !(sizeof(T) == 4 && a.res.p) &&
             group_dispatch<false>(a.D, group))
             return cuda_status();
-        // the smallest tile that holds the row, 64 bytes a thread (rows up to
-        // 256 values half of that)
+        // the smallest tile that holds the row, in vectors 64 bytes a thread
+        // (rows up to 256 values half of that)
         constexpr int NE = sizeof(T) == 2 ? 32 : 16, F = sizeof(T) == 2 ? 1 : 2;
-        auto any = [&](auto v) {
-            bool some = true;
-            if (a.D <= 64) tile(Int<4>{}, Int<16>{}, v);
-            else if (a.D <= 128) tile(Int<8>{}, Int<16>{}, v);
-            else if (a.D <= 256) tile(Int<16>{}, Int<16>{}, v);
-            else if (a.D <= 512) tile(Int<16 * F>{}, Int<NE>{}, v);
-            else if (a.D <= 1024) tile(Int<32 * F>{}, Int<NE>{}, v);
-            else if (a.D <= 2048) tile(Int<64 * F>{}, Int<NE>{}, v);
-            else if (a.D <= 4096) tile(Int<128 * F>{}, Int<NE>{}, v);
-            else if (a.D <= 8192) tile(Int<256 * F>{}, Int<NE>{}, v);
-            else if (a.D <= 16384) tile(Int<512 * F>{}, Int<NE>{}, v);
-            else if (a.D <= 1024 * NE && sizeof(T) == 2) tile(Int<1024>{}, Int<NE>{}, v);
+        constexpr Int<1> vector;
+        constexpr Int<0> single;
+        bool some = true;
+        if (vec) {
+            if (a.D <= 64) tile(Int<4>{}, Int<16>{}, vector);
+            else if (a.D <= 128) tile(Int<8>{}, Int<16>{}, vector);
+            else if (a.D <= 256) tile(Int<16>{}, Int<16>{}, vector);
+            else if (a.D <= 512) tile(Int<16 * F>{}, Int<NE>{}, vector);
+            else if (a.D <= 1024) tile(Int<32 * F>{}, Int<NE>{}, vector);
+            else if (a.D <= 2048) tile(Int<64 * F>{}, Int<NE>{}, vector);
+            else if (a.D <= 4096) tile(Int<128 * F>{}, Int<NE>{}, vector);
+            else if (a.D <= 8192) tile(Int<256 * F>{}, Int<NE>{}, vector);
+            else if (a.D <= 16384) tile(Int<512 * F>{}, Int<NE>{}, vector);
+            else if (a.D <= 1024 * NE && sizeof(T) == 2) tile(Int<1024>{}, Int<NE>{}, vector);
             else some = false;
-            return some;
-        };
-        if (vec ? any(Int<1>{}) : any(Int<0>{})) return cuda_status();
+        } else {
+            if (a.D <= 64) tile(Int<4>{}, Int<16>{}, single);
+            else if (a.D <= 128) tile(Int<8>{}, Int<16>{}, single);
+            else if (a.D <= 256) tile(Int<16>{}, Int<16>{}, single);
+            else if (a.D <= 320) tile(Int<32>{}, Int<10>{}, single);
+            else if (a.D <= 512) tile(Int<32>{}, Int<16>{}, single);
+            else if (a.D <= 640) tile(Int<64>{}, Int<10>{}, single);
+            else if (a.D <= 1024) tile(Int<64>{}, Int<16>{}, single);
+            else if (a.D <= 1280) tile(Int<128>{}, Int<10>{}, single);
+            else if (a.D <= 2048) tile(Int<128>{}, Int<16>{}, single);
+            else if (a.D <= 2560) tile(Int<256>{}, Int<10>{}, single);
+            else if (a.D <= 4096) tile(Int<256>{}, Int<16>{}, single);
+            else if (a.D <= 5120) tile(Int<512>{}, Int<10>{}, single);
+            else if (a.D <= 8192) tile(Int<512>{}, Int<16>{}, single);
+            else if (a.D <= 10240) tile(Int<1024>{}, Int<10>{}, single);
+            else if (a.D <= 16384) tile(Int<1024>{}, Int<16>{}, single);
+            else some = false;
+        }
+        if (some) return cuda_status();
         pdl_launch(layernorm_row_kernel<T, WT>, (unsigned)a.rows, 512, 0, st,
                    (const T *)a.x.p, a.x.ld, (const T *)a.res.p, a.res.ld, ptr<T>(a.y), a.y.ld,
                    ptr<T>(a.sum), a.sum.ld, (const WT *)a.weight, (const WT *)a.bias, a.mean,
@@ -1191,8 +1209,8 @@ Status launch_layernorm_backward(const LayerNormBackwardArgs &a, cudaStream_t st
             tile(Int<512>{}, Int<8>{});
         } else {
             // two readings: dx row by row, the weights' gradients column by
-            // column (14000 x 4097 BF16 228 us, in one reading with 1024
-            // threads a row and one block an SM 397; 100 x 5001 FP32 8.4 / 12)
+            // column (14000 x 4097 BF16 211 us, in one reading with 1024
+            // threads a row and one block an SM 397; 100 x 5001 FP32 7.8 / 12)
             auto dx = [&](auto kernel, int threads) {
                 pdl_launch(kernel, (unsigned)a.rows, threads, 0, st, (const T *)a.dy.p, a.dy.ld,
                            (const T *)a.x.p, a.x.ld, (const T *)a.dsum.p, a.dsum.ld, ptr<T>(a.dx),
@@ -1211,7 +1229,9 @@ Status launch_layernorm_backward(const LayerNormBackwardArgs &a, cudaStream_t st
                            a.work);
             };
             if (vec && a.D <= 16384) dx(layernorm_dx_tile_kernel<T, WT, 1024, 16, true>, 1024);
+            else if (!vec && a.D <= 5120) dx(layernorm_dx_tile_kernel<T, WT, 512, 10, false>, 512);
             else if (!vec && a.D <= 8192) dx(layernorm_dx_tile_kernel<T, WT, 512, 16, false>, 512);
+            else if (!vec && a.D <= 10240) dx(layernorm_dx_tile_kernel<T, WT, 1024, 10, false>, 1024);
             else if (!vec && a.D <= 16384) dx(layernorm_dx_tile_kernel<T, WT, 1024, 16, false>, 1024);
             else dx(layernorm_dx_row_kernel<T, WT>, 512);
             constexpr int kVec = 16 / (int)sizeof(T);

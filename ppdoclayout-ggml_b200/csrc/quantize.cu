@@ -220,24 +220,24 @@ Status launch_quantize_rows(const Rows &x, int type, long long rows, int K, int8
         constexpr Int<1> vector;
         constexpr Int<0> single;
         if (vec) {
-            constexpr int kNE = 64 / (int)sizeof(T);
-            constexpr Int<kNE> NE;
-            constexpr Int<kNE / 4 * 3> LESS;
-            if (K <= 4 * kNE) return tile(Int<4>{}, NE, vector);
-            if (K <= 8 * kNE) return tile(Int<8>{}, NE, vector);
-            if (K <= 16 * kNE / 4 * 3) return tile(Int<16>{}, LESS, vector);
-            if (K <= 16 * kNE) return tile(Int<16>{}, NE, vector);
-            if (K <= 32 * kNE / 4 * 3) return tile(Int<32>{}, LESS, vector);
-            if (K <= 32 * kNE) return tile(Int<32>{}, NE, vector);
-            if (K <= 64 * kNE / 4 * 3) return tile(Int<64>{}, LESS, vector);
-            if (K <= 64 * kNE) return tile(Int<64>{}, NE, vector);
-            if (K <= 128 * kNE / 4 * 3) return tile(Int<128>{}, LESS, vector);
-            if (K <= 128 * kNE) return tile(Int<128>{}, NE, vector);
-            if (K <= 256 * kNE / 4 * 3) return tile(Int<256>{}, LESS, vector);
-            if (K <= 256 * kNE) return tile(Int<256>{}, NE, vector);
-            if (K <= 512 * kNE / 4 * 3) return tile(Int<512>{}, LESS, vector);
-            if (K <= 512 * kNE) return tile(Int<512>{}, NE, vector);
-            if (K <= 1024 * kNE) return tile(Int<1024>{}, NE, vector);
+            constexpr int kNE = 64 / (int)sizeof(T), kLess = kNE / 4 * 3, kMore = kNE / 4 * 5;
+            auto by = [&](auto tpr) {
+                constexpr int TPR = decltype(tpr)::value;
+                if constexpr (TPR >= 16 && TPR < 1024 && TPR * kNE != 4096) {
+                    if (K <= TPR * kLess) return tile(tpr, Int<kLess>{}, vector);
+                }
+                return tile(tpr, Int<kNE>{}, vector);
+            };
+            if (K <= 4 * kNE) return by(Int<4>{});
+            if (K <= 8 * kNE) return by(Int<8>{});
+            if (K <= 16 * kNE) return by(Int<16>{});
+            if (K <= 32 * kNE) return by(Int<32>{});
+            if (K <= 64 * kNE) return by(Int<64>{});
+            if (K > 2048 && K <= 2560) return tile(Int<2560 / kMore>{}, Int<kMore>{}, vector);
+            if (K <= 128 * kNE) return by(Int<128>{});
+            if (K <= 256 * kNE) return by(Int<256>{});
+            if (K <= 512 * kNE) return by(Int<512>{});
+            if (K <= 1024 * kNE) return by(Int<1024>{});
         }
         if (K <= 64) return tile(Int<8>{}, Int<8>{}, single);
         if (K <= 128) return tile(Int<8>{}, Int<16>{}, single);
@@ -248,8 +248,11 @@ Status launch_quantize_rows(const Rows &x, int type, long long rows, int K, int8
         if (K <= 1024) return tile(Int<32>{}, Int<32>{}, single);
         if (K <= 1280) return tile(Int<64>{}, Int<20>{}, single);
         if (K <= 2048) return tile(Int<128>{}, Int<16>{}, single);
+        if (K <= 2560) return tile(Int<128>{}, Int<20>{}, single);
         if (K <= 4096) return tile(Int<256>{}, Int<16>{}, single);
+        if (K <= 5120) return tile(Int<256>{}, Int<20>{}, single);
         if (K <= 8192) return tile(Int<512>{}, Int<16>{}, single);
+        if (K <= 10240) return tile(Int<512>{}, Int<20>{}, single);
         if (K <= 16384) return tile(Int<1024>{}, Int<16>{}, single);
         pdl_launch(quantize_row_kernel<T>, (unsigned)rows, 512, 0, st, (const T *)x.p, x.ld, K, q,
                    ldq, scale);
