@@ -1199,12 +1199,20 @@ Status launch_layernorm_backward(const LayerNormBackwardArgs &a, cudaStream_t st
             tile(Int<8>{}, Int<8>{});
         } else if (a.D <= 256) {
             tile(Int<32>{}, Int<8>{});
+        } else if (a.D <= 320) {
+            tile(Int<64>{}, Int<5>{});
         } else if (a.D <= 512) {
             tile(Int<64>{}, Int<8>{});
+        } else if (a.D <= 640) {
+            tile(Int<128>{}, Int<5>{});
         } else if (a.D <= 1024) {
             tile(Int<128>{}, Int<8>{});
+        } else if (a.D <= 1280) {
+            tile(Int<256>{}, Int<5>{});
         } else if (a.D <= 2048) {
             tile(Int<256>{}, Int<8>{});
+        } else if (a.D <= 2560) {
+            tile(Int<512>{}, Int<5>{});
         } else if (a.D <= 4096) {
             tile(Int<512>{}, Int<8>{});
         } else {
