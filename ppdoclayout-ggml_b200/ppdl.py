@@ -551,7 +551,7 @@ def layernorm_backward(dy, x, weight, mean, rstd, *, dsum=None, param_grads: boo
     if param_grads:
         dw, db = (x.new_empty(D), x.new_empty(D)) if weight is None else \
             (_tt["empty_like"](weight), _tt["empty_like"](weight))
-        work = mean.new_empty(_lib.ppdl_layernorm_backward_workspace(rows, D))
+        work = mean.new_empty(_backward_work(rows, D))
         dwp, dbp, wsp = dw.data_ptr(), db.data_ptr(), work.data_ptr()
     fn = _lib.ppdl_layernorm_backward
     status = fn(dy.data_ptr(), lddy, x.data_ptr(), ldx, wp, mean.data_ptr(), rstd.data_ptr(), dsp,
@@ -559,6 +559,11 @@ def layernorm_backward(dy, x, weight, mean, rstd, *, dsum=None, param_grads: boo
     if status:
         _failed(fn, status)
     return dx, dw, db
+
+
+@functools.lru_cache(maxsize=256)
+def _backward_work(rows: int, D: int) -> int:
+    return _lib.ppdl_layernorm_backward_workspace(rows, D)
 
 
 def quantize_rows(x):
