@@ -263,6 +263,38 @@ def test_layernorm_dense_odd_rows(cuda, rows, D, t):
     assert (xr[rows * D:] == 7).all() and (rr[rows * D:] == 7).all()
 
 
+@pytest.mark.parametrize("rows,D", [(8195, 513), (3651, 1153), (16384, 1024), (1200, 8192)])
+def test_layernorm_chain(cuda, rows, D):
+    """Kernels that start before the ones they follow have ended wait for all
+    that those store, by bulk copies too: a chain gives what it gives with a
+    pause after every call, eagerly and in a graph."""
+    g = gen(rows + D)
+    T = torch.bfloat16
+    x, dy, w = normal(g, rows, D, t=T), normal(g, rows, D, t=T), normal(g, D, t=T, shift=1.0, scale=0.2)
+
+    def chain(pause):
+        out = [x]
+        for _ in range(3):
+            y, s, mean, rstd = ppdl.layernorm(out[-1], w, None, residual=dy, return_sum=True, return_stats=True)
+            pause()
+            dx, dw, db = ppdl.layernorm_backward(dy, s, w, mean, rstd, dsum=y)
+            pause()
+            q, scale = ppdl.quantize_rows(dx)
+            pause()
+            out += [y, s, dw, db, scale, q.contiguous(), dx]
+        return out
+
+    want = chain(torch.cuda.synchronize)
+    for _ in range(3):
+        assert all(torch.equal(a, b) for a, b in zip(chain(lambda: None), want))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = chain(lambda: None)
+    for _ in range(3):
+        graph.replay()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 def test_layernorm_backward_no_rows(cuda):
     """No rows: the weights' gradients are zeros, not what the memory held."""
     x, s = torch.empty((0, 300), device="cuda"), torch.empty(0, device="cuda")
