@@ -956,7 +956,7 @@ bool group_shape(Groups &g, std::initializer_list<const Rows *> all, int read, l
                ((long long)at * D * size % 16 || (long long)at * D * size < 8192))
             at *= 2;
         const long long stage = (long long)read * at * D * size;
-        const long long fit = (blocks == 1 ? kGroupSmem : blocks == 2 ? 108 * 1024 : 71 * 1024) / stage;
+        const long long fit = (blocks == 1 ? kGroupSmem : blocks == 2 ? 110 * 1024 : 72 * 1024) / stage;
         if (at > kGroupMaxRows || fit < 3) continue;
         g.rows_at = at;
         g.stages = fit > kRingStages ? kRingStages : (int)fit;
@@ -1186,9 +1186,9 @@ Status launch_layernorm_backward(const LayerNormBackwardArgs &a, cudaStream_t st
         // rows spill; wider than 4096 they have to)
         constexpr int kNE = 32 / (int)sizeof(T);
         // dense rows that are no vectors go through groups (50000 x 1153 FP16
-        // 112 us, 161 by the tile; FP32 123 / 186; 200000 x 79 BF16 34 / 75),
-        // unless they are narrow (200000 x 51 BF16 36 / 26) or few (4800 x 641
-        // BF16 17.3 / 14.3, 4800 x 1153 19.1 / 24.4)
+        // 95.5 us, 142 by the tile; FP32 122 / 171; 200000 x 79 BF16 34 / 73),
+        // unless they are narrow (200000 x 51 BF16 36 / 26) or few (4191 x 1001
+        // BF16 17.7 / 14.9, 16761 x 1001 33.2 / 36.4)
         const bool done =
             a.rows == 0 ||
             (vec ? ring_dispatch<kNE>(a.D, [&](auto tpr) { return ring(tpr, Int<kNE>{}); }) ||
