@@ -509,6 +509,16 @@ linear_i8_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
                     wait_for(bar_full + 8 * (int)(j % S), (uint32_t)((j / S) & 1),
                              (volatile int *)&dummy);
                 }
+            // so must the leader's arrivals at this CTA's barriers (a later
+            // grid's CTA may already have this shared memory by then): the
+            // stages' last releases, then the end of all MMAs.  What the
+            // epilogue's barriers get, the epilogue has waited for.
+            if constexpr (FORM == PAIR) {
+                for (long long j = it > S ? it - S : 0; j < it && ok; j++)
+                    ok = wait_for(bar_empty + 8 * (int)(j % S), (uint32_t)((j / S) & 1), abort_flag);
+                int dummy = 0;
+                if (rank != 0) wait_for(bar_done, 0, (volatile int *)&dummy);
+            }
         }
     } else if (warp == kWarpMma) {
         if (lane == 0 && (FORM != PAIR || rank == 0)) {
