@@ -40,7 +40,8 @@ __device__ __forceinline__ float weight_at(const WT *w, long long i, float none)
 }
 
 // One block per row, any width (rows too wide for registers): read once for the
-// mean, and again, from L2, for the variance and for the output.
+// mean, and again, from L2, for the variance and for the output.  (The column
+// is unsigned: its last step passes 2^31 - 1 where D is next to it.)
 template <typename T, typename WT>
 __global__ void layernorm_row_kernel(const T *x, long long ldx, const T *res, long long ldres, T *y,
                                      long long ldy, T *sum, long long ldsum, const WT *w,
@@ -53,20 +54,20 @@ __global__ void layernorm_row_kernel(const T *x, long long ldx, const T *res, lo
     y += row * ldy;
     if (res) res += row * ldres;
     if (sum) sum += row * ldsum;
-    auto value = [&](int i) {
+    auto value = [&](unsigned i) {
         const float v = to_float(x[i]);
         return res ? to_float(from_float<T>(v + to_float(res[i]))) : v;
     };
     float s = 0.0f;
-    for (int i = threadIdx.x; i < D; i += blockDim.x) s += value(i);
+    for (unsigned i = threadIdx.x; i < (unsigned)D; i += blockDim.x) s += value(i);
     const float mean = block_sum(s, sh) / (float)D;
     s = 0.0f;
-    for (int i = threadIdx.x; i < D; i += blockDim.x) {
+    for (unsigned i = threadIdx.x; i < (unsigned)D; i += blockDim.x) {
         const float d = value(i) - mean;
         s += d * d;
     }
     const float rstd = rsqrtf(block_sum(s, sh) / (float)D + eps);
-    for (int i = threadIdx.x; i < D; i += blockDim.x) {
+    for (unsigned i = threadIdx.x; i < (unsigned)D; i += blockDim.x) {
         const float v = value(i);
         if (sum) sum[i] = from_float<T>(v);
         y[i] = from_float<T>((v - mean) * rstd * weight_at(w, i, 1.0f) + weight_at(b, i, 0.0f));
@@ -383,7 +384,7 @@ layernorm_group_kernel(const T *x, const T *res, T *y, T *sum, const WT *w, cons
     ring.finish();
 }
 
-// dx, one block per row, any width.
+// dx, one block per row, any width (unsigned columns as above).
 template <typename T, typename WT>
 __global__ void layernorm_dx_row_kernel(const T *dy, long long lddy, const T *x, long long ldx,
                                         const T *dsum, long long lddsum, T *dx, long long lddx,
@@ -398,13 +399,13 @@ __global__ void layernorm_dx_row_kernel(const T *dy, long long lddy, const T *x,
     if (dsum) dsum += row * lddsum;
     const float mean = mean_in[row], rstd = rstd_in[row];
     float s1 = 0.0f, s2 = 0.0f;
-    for (int i = threadIdx.x; i < D; i += blockDim.x) {
+    for (unsigned i = threadIdx.x; i < (unsigned)D; i += blockDim.x) {
         const float g = to_float(dy[i]) * weight_at(w, i, 1.0f);
         s1 += g;
         s2 += g * ((to_float(x[i]) - mean) * rstd);
     }
     const float m1 = block_sum(s1, sh) / (float)D, m2 = block_sum(s2, sh) / (float)D;
-    for (int i = threadIdx.x; i < D; i += blockDim.x) {
+    for (unsigned i = threadIdx.x; i < (unsigned)D; i += blockDim.x) {
         const float g = to_float(dy[i]) * weight_at(w, i, 1.0f);
         const float xh = (to_float(x[i]) - mean) * rstd;
         float v = (g - m1 - xh * m2) * rstd;

@@ -179,7 +179,8 @@ quantize_kernel(const T *x, long long ldx, long long rows, int K, int8_t *q, lon
 }
 
 // One block per row, any width (rows too wide for registers): read once for
-// the scale and again, from L2, for the quotients.
+// the scale and again, from L2, for the quotients.  (The column is unsigned:
+// its last step passes 2^31 - 1 where K is next to it.)
 template <typename T>
 __global__ void quantize_row_kernel(const T *x, long long ldx, int K, int8_t *q, long long ldq,
                                     float *scale) {
@@ -190,11 +191,11 @@ __global__ void quantize_row_kernel(const T *x, long long ldx, int K, int8_t *q,
     x += row * ldx;
     q += row * ldq;
     unsigned m = 0;
-    for (int i = threadIdx.x; i < K; i += blockDim.x)
+    for (unsigned i = threadIdx.x; i < (unsigned)K; i += blockDim.x)
         m = max(m, __float_as_uint(fabsf(to_float(x[i]))));
     const Divisor d(row_max<512>(m, sh));
     if (threadIdx.x == 0) scale[row] = d.s;
-    for (int i = threadIdx.x; i < K; i += blockDim.x) q[i] = (int8_t)d(to_float(x[i]));
+    for (unsigned i = threadIdx.x; i < (unsigned)K; i += blockDim.x) q[i] = (int8_t)d(to_float(x[i]));
 }
 
 }  // namespace
