@@ -327,7 +327,8 @@ PPDL_OPS_API int ppdl_quantize_rows_i8(const void * x, long long ldx, int type, 
    exact.  ldq and ldw are multiples of 16 bytes, q and w 16-byte aligned;
    bytes past K are ignored.  bias [N] FP32 and res may be NULL; res and y
    are of `type`; y may be res (same pointer and ld).  act 0/1/2/3 =
-   none/ReLU/SiLU/GELU.  1 <= K <= 131071 (the sums fit 32 bits).
+   none/ReLU/SiLU/GELU, a NaN staying one through each.  1 <= K <= 131071
+   (the sums fit 32 bits).
    Returns PPDL_OK / PPDL_ERR_SHAPE / PPDL_ERR_CUDA. */
 PPDL_OPS_API int ppdl_linear_i8(const int8_t * q, long long ldq, const float * q_scale,
                                 const int8_t * w, long long ldw, const float * w_scale,

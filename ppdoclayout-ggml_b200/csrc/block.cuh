@@ -90,6 +90,15 @@ __device__ __forceinline__ float2 sub2(float2 a, float2 b) {
 }
 __device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 
+// act_apply with a ReLU that keeps a NaN: a token that is not finite has to
+// stay visible in its output row (fmaxf would return the zero).
+__device__ __forceinline__ float act_keep_nan(float v, int act) {
+    if (act != ACT_RELU) return act_apply(v, act);
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(v), "f"(0.0f));
+    return r;
+}
+
 // n / d for 0 <= n < 2^31 by a multiplication (Granlund and Montgomery,
 // "Division by invariant integers using multiplication", PLDI 1994)
 struct FastDiv {

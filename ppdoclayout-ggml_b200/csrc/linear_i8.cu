@@ -225,10 +225,10 @@ __device__ __forceinline__ void finish_all(float (&v)[C], const uint32_t (&acc)[
         const float2 a01 = make_float2((float)(int)acc[j], (float)(int)acc[j + 1]);
         const float2 a23 = make_float2((float)(int)acc[j + 2], (float)(int)acc[j + 3]);
         const float2 v01 = fma2(a01, s01, bias2), v23 = fma2(a23, s23, bias2);
-        v[j] = act_apply(v01.x, ACT);
-        v[j + 1] = act_apply(v01.y, ACT);
-        v[j + 2] = act_apply(v23.x, ACT);
-        v[j + 3] = act_apply(v23.y, ACT);
+        v[j] = act_keep_nan(v01.x, ACT);
+        v[j + 1] = act_keep_nan(v01.y, ACT);
+        v[j + 2] = act_keep_nan(v23.x, ACT);
+        v[j + 3] = act_keep_nan(v23.y, ACT);
     }
 }
 
@@ -687,7 +687,7 @@ linear_i8_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
                 if (n + i >= a.N) break;
                 float v = __fmaf_rn((float)sums[i], sx * __ldg(a.w_scale + n + i),
                                     a.bias ? __ldg(a.bias + n + i) : 0.0f);
-                v = act_apply(v, a.act);
+                v = act_keep_nan(v, a.act);
                 if (a.res)
                     v = __fadd_rn(v, to_float(((const T *)a.res)[(long long)t * a.ldres + n + i]));
                 ((T *)a.y)[(long long)t * a.ldy + n + i] = from_float<T>(v);

@@ -5,8 +5,11 @@ import pytest
 import torch
 
 import ppdl
+from test_block_ops_gpu import TYPES, gen, normal
 
 pytestmark = pytest.mark.gpu
+INF, NAN = float("inf"), float("nan")
+
 
 WIDEST = 2 ** 31 - 1
 
@@ -62,3 +65,28 @@ def test_widest_row_backward(cuda):
     assert torch.equal(dx, dy)
     assert (room[:4096] == 7).all() and (room[4096 + WIDEST:] == 7).all()
 
+
+@pytest.mark.parametrize("act", ppdl.ACTS)
+@pytest.mark.parametrize("M,K,N", [(1, 512, 200), (2, 300, 200), (16, 512, 1000), (5, 2047, 260), (40, 256, 96),
+                                   (300, 256, 1024), (2400, 256, 256), (5003, 200, 2100), (20, 4096, 4097),
+                                   (100, 4096, 641), (2049, 513, 1025), (2570, 1024, 1537)])
+def test_bad_tokens_stay_bad(cuda, M, K, N, act):
+    """A token with a NaN or an infinity is a row of NaNs behind every
+    activation, in every form of the product; so is a channel whose scale or
+    bias is a NaN.  Nothing else changes."""
+    g = gen(M + K + N)
+    for T in TYPES.values():
+        x, res = normal(g, M, K, t=T), normal(g, M, N, t=T)
+        wq, ws = ppdl.quantize_rows(normal(g, N, K, scale=K ** -0.5))
+        bias = normal(g, N)
+        for r in (None, res):
+            clean = ppdl.linear_i8(x, wq, ws, bias=bias, act=act, residual=r)
+            bad, bs, bb = x.clone(), ws.clone(), bias.clone()
+            rows, cols = {M - 1, M // 2}, {N - 1, N // 3}
+            bad[M - 1, K - 1], bad[M // 2, 0] = NAN, -INF
+            bs[N - 1], bb[N // 3] = NAN, NAN
+            y = ppdl.linear_i8(bad, wq, bs, bias=bb, act=act, residual=r)
+            keep_r = [i for i in range(M) if i not in rows]
+            keep_c = [i for i in range(N) if i not in cols]
+            assert y[list(rows)].isnan().all() and y[:, list(cols)].isnan().all()
+            assert torch.equal(y[keep_r][:, keep_c], clean[keep_r][:, keep_c])
