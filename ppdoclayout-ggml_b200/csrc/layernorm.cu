@@ -571,13 +571,16 @@ layernorm_bwd_tile_kernel(const T *dy, long long lddy, const T *x, long long ldx
 
     typename Tile::Raw rx, rdy;
     float mean = 0.0f, rstd = 0.0f;
-    // rows past the end repeat the last one with a zero gradient
+    // rows past the end are zeros with no spread: they add nothing, where a
+    // repeated row with a zero factor would add NaNs for its infinities
     auto load = [&](long long row) {
-        const long long at = min(row, rows - 1);
-        Tile::load(rx, x + at * ldx, D, lane);
-        Tile::load(rdy, dy + at * lddy, D, lane);
-        mean = mean_in[at];
-        rstd = rstd_in[at];
+        const bool real = kRows == 1 || row < rows;  // a block of one row stops before
+        const long long at = real ? row : rows - 1;
+        const int width = real ? D : 0;
+        Tile::load(rx, x + at * ldx, width, lane);
+        Tile::load(rdy, dy + at * lddy, width, lane);
+        mean = real ? mean_in[at] : 0.0f;
+        rstd = real ? rstd_in[at] : 0.0f;
     };
     const long long step = (long long)gridDim.x * kRows;
     long long row = (long long)blockIdx.x * kRows + group;
@@ -585,13 +588,13 @@ layernorm_bwd_tile_kernel(const T *dy, long long lddy, const T *x, long long ldx
     load(row);
     for (long long base = (long long)blockIdx.x * kRows; base < rows;
          base += step, row += step, parity ^= 1) {
-        const bool real = row < rows;
-        const float m = mean, r = rstd, gate = real ? 1.0f : 0.0f;
+        const bool real = kRows == 1 || row < rows;
+        const float m = mean, r = rstd;
         float xh[NE], g[NE];
 #pragma unroll
         for (int j = 0; j < NE; j++) {
             xh[j] = (to_float(rx.v[j]) - m) * r;
-            g[j] = to_float(rdy.v[j]) * gate;
+            g[j] = to_float(rdy.v[j]);
         }
         if (base + step < rows) load(row + step);
         float s[2] = {0.0f, 0.0f};

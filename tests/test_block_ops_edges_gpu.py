@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import ppdl
-from test_block_ops_gpu import TYPES, gen, normal
+from test_block_ops_gpu import TYPES, bwd_want, close, gen, normal
 
 pytestmark = pytest.mark.gpu
 INF, NAN = float("inf"), float("nan")
@@ -90,3 +90,31 @@ def test_bad_tokens_stay_bad(cuda, M, K, N, act):
             keep_c = [i for i in range(N) if i not in cols]
             assert y[list(rows)].isnan().all() and y[:, list(cols)].isnan().all()
             assert torch.equal(y[keep_r][:, keep_c], clean[keep_r][:, keep_c])
+
+
+# rows that fill no block of any form; by value, groups, rings and two readings
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("rows,D", [(1, 3), (5, 31), (33, 51), (3, 101), (13, 257), (7, 333), (5, 641), (9, 1001),
+                                    (5, 1153), (3, 2501), (3, 4097), (2, 16383), (2, 20001), (64001, 79), (17001, 257),
+                                    (3651, 1153), (5, 8), (5, 64), (33, 256), (13, 1000), (5, 4096), (3, 8192),
+                                    (3, 16384), (2, 32768)])
+def test_backward_infinite_gradient_of_the_last_row(cuda, rows, D, t):
+    """An infinity in the last row's gradient spoils its own row of dx and its
+    own columns of dweight and dbias: their sums are infinite, not NaN."""
+    T = TYPES[t]
+    g = gen(rows + D)
+    x, dy, w = normal(g, rows, D, t=T), normal(g, rows, D, t=T), normal(g, D, t=T, shift=1.0, scale=0.2)
+    _, mean, rstd = ppdl.layernorm(x, w, None, return_stats=True)
+    up, down = D - 1, D // 2
+    xh = (x[-1].double() - mean[-1].double()) * rstd[-1].double()
+    dy[-1, up], dy[-1, down] = INF, -INF
+    dx, dw, db = ppdl.layernorm_backward(dy, x, w, mean, rstd)
+    assert db[up] == INF and db[down] == -INF
+    assert dw[up] == INF * float(xh[up].sign()) and dw[down] == -INF * float(xh[down].sign())
+    finite = dy.clone()
+    finite[-1, up] = finite[-1, down] = 0
+    want, tol = bwd_want(finite, x, w, mean, rstd)
+    keep = [c for c in range(D) if c not in (up, down)]
+    close(dw[keep], want[1][keep], tol[1][keep])
+    close(db[keep], want[2][keep], tol[2][keep])
+    close(dx[:-1], want[0][:-1], tol[0][:-1])
