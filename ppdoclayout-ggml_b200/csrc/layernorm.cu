@@ -384,6 +384,27 @@ layernorm_group_kernel(const T *x, const T *res, T *y, T *sum, const WT *w, cons
     ring.finish();
 }
 
+// xh = (x - mean) rstd, the difference first: x rstd - mean rstd costs an
+// instruction less, but the rounding of mean rstd is u |mean| rstd whatever
+// the difference, and the product can pass FP32's range.
+__device__ __forceinline__ float2 normalised(float2 x, float mean, float rstd) {
+    return mul2(add2(x, both(-mean)), both(rstd));
+}
+
+// dx = rstd (g - mean(g) - xh mean(g xh)), xh as (x - mean) rstd with rstd
+// taken to its factor: m1 = -mean(g) rstd, m2 = -mean(g xh) rstd.
+__device__ __forceinline__ float2 dx_of(float2 x, float mean, float rstd, float2 g, float2 m1,
+                                        float2 m2) {
+    return fma2(fma2(add2(x, both(-mean)), m2, g), both(rstd), m1);
+}
+
+// A row's places past D hold x = 0 and g = 0, which add nothing to the row's
+// sums as long as xh = -mean rstd is finite there; where it is not, the sum of
+// g xh is taken again without them.
+__device__ __forceinline__ bool zero_overflows(float mean, float rstd) {
+    return !(fabsf(mean * rstd) < INFINITY);
+}
+
 // dx, one block per row, any width (unsigned columns as above).
 template <typename T, typename WT>
 __global__ void layernorm_dx_row_kernel(const T *dy, long long lddy, const T *x, long long ldx,
@@ -426,9 +447,7 @@ layernorm_dx_tile_kernel(const T *dy, long long lddy, const T *x, long long ldx,
     __shared__ float sh[32];
     const int lane = threadIdx.x;
     const long long row = blockIdx.x;
-    const float rstd = rstd_in[row], inv_d = 1.0f / (float)D;
-    // x r - mean r: off by the rounding of mean r, u |mean| r
-    const float mr = -mean_in[row] * rstd;
+    const float mean = mean_in[row], rstd = rstd_in[row], inv_d = 1.0f / (float)D;
     if constexpr (VEC) {
         using Tile = PairTile<T, TPR, NE>;
         constexpr int kHalf = Tile::kVec / 2;
@@ -446,16 +465,22 @@ layernorm_dx_tile_kernel(const T *dy, long long lddy, const T *x, long long ldx,
                 const int j = i * kHalf + k;
                 g[j] = mul2(Tile::pair(rd, j), p[k]);
                 t0 = add2(t0, g[j]);
-                t1 = fma2(g[j], fma2(Tile::pair(rx, j), both(rstd), both(mr)), t1);
+                t1 = fma2(g[j], normalised(Tile::pair(rx, j), mean, rstd), t1);
             }
+        }
+        if (zero_overflows(mean, rstd)) {
+            t1 = both(0.0f);
+#pragma unroll
+            for (int j = 0; j < NE / 2; j++)
+                if (Tile::pair_column(j, lane) < D)
+                    t1 = fma2(g[j], normalised(Tile::pair(rx, j), mean, rstd), t1);
         }
         const float s0 = block_sum(t0.x + t0.y, sh), s1 = block_sum(t1.x + t1.y, sh);
         const float2 m1 = both(-s0 * inv_d * rstd), m2 = both(-s1 * inv_d * rstd);
         if (dsum) Tile::load(rd, dsum + row * lddsum, D, lane);
 #pragma unroll
         for (int j = 0; j < NE / 2; j++) {
-            const float2 xh = fma2(Tile::pair(rx, j), both(rstd), both(mr));
-            float2 v = fma2(g[j], both(rstd), fma2(xh, m2, m1));
+            float2 v = dx_of(Tile::pair(rx, j), mean, rstd, g[j], m1, m2);
             if (dsum) v = add2(v, Tile::pair(rd, j));
             Tile::set_pair(rx, j, v);
         }
@@ -471,13 +496,19 @@ layernorm_dx_tile_kernel(const T *dy, long long lddy, const T *x, long long ldx,
         for (int j = 0; j < NE; j++) {
             g[j] *= to_float(rd.v[j]);
             t0 += g[j];
-            t1 += g[j] * (to_float(rx.v[j]) * rstd + mr);
+            t1 += g[j] * ((to_float(rx.v[j]) - mean) * rstd);
+        }
+        if (zero_overflows(mean, rstd)) {
+            t1 = 0.0f;
+#pragma unroll
+            for (int j = 0; j < NE; j++)
+                if (Tile::inside(j, D, lane)) t1 += g[j] * ((to_float(rx.v[j]) - mean) * rstd);
         }
         const float m1 = block_sum(t0, sh) * inv_d, m2 = block_sum(t1, sh) * inv_d;
         if (dsum) Tile::load(rd, dsum + row * lddsum, D, lane);
 #pragma unroll
         for (int j = 0; j < NE; j++) {
-            float v = (g[j] - m1 - (to_float(rx.v[j]) * rstd + mr) * m2) * rstd;
+            float v = (g[j] - m1 - (to_float(rx.v[j]) - mean) * rstd * m2) * rstd;
             if (dsum) v += to_float(rd.v[j]);
             rx.v[j] = from_float<T>(v);
         }
@@ -510,7 +541,7 @@ layernorm_dw_column_kernel(const T *dy, long long lddy, const T *x, long long ld
         typename Tile::Raw rx, rd;
         Tile::load(rx, x + r * ldx, left, lane);
         Tile::load(rd, dy + r * lddy, left, lane);
-        const float s = rstd[r], mr = -mean[r] * s;
+        const float m = mean[r], s = rstd[r];
 #pragma unroll
         for (int j = 0; j < NE; j++) {
             float g, v;
@@ -521,7 +552,7 @@ layernorm_dw_column_kernel(const T *dy, long long lddy, const T *x, long long ld
                 g = to_float(rd.v[j]);
                 v = to_float(rx.v[j]);
             }
-            sw[j] += g * (v * s + mr);
+            sw[j] += g * ((v - m) * s);
             sb[j] += g;
         }
     }
@@ -596,11 +627,15 @@ layernorm_bwd_tile_kernel(const T *dy, long long lddy, const T *x, long long ldx
             xh[j] = (to_float(rx.v[j]) - m) * r;
             g[j] = to_float(rdy.v[j]);
         }
+        if (zero_overflows(m, r)) {
+#pragma unroll
+            for (int j = 0; j < NE; j++)
+                if (!Tile::inside(j, D, lane)) xh[j] = 0.0f;
+        }
         if (base + step < rows) load(row + step);
         float s[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int j = 0; j < NE; j++) {
-            // past D every g is zero (loaded as zero), and xh counts only with it
             dw[j] += g[j] * xh[j];
             db[j] += g[j];
             g[j] *= p[j];
@@ -698,9 +733,7 @@ layernorm_bwd_ring_kernel(const T *dy, long long lddy, const T *x, long long ldx
     const long long dxstep = ring.step * lddx;
     for (int it = 0; it < ring.iters; it++, ring.at.next(), dx += dxstep) {
         ring.wait();
-        const float r = rstd[0];
-        // x r - mean r: off by the rounding of mean r, u |mean| r
-        const float mr = -mean[0] * r;
+        const float r = rstd[0], m = mean[0];
         mean[0] = mean[1];
         rstd[0] = rstd[1];
         if (it + 2 < ring.mine) {
@@ -711,20 +744,32 @@ layernorm_bwd_ring_kernel(const T *dy, long long lddy, const T *x, long long ldx
         rstd_in += ring.step;
         const bool real = it < ring.mine;
         typename Tile::Raw rx, rdy, out;
-        float2 g[NE / 2], t0 = both(0.0f), t1 = both(0.0f);
+        // xh and g rstd + dsum are kept in place of x, g and dsum, which nothing
+        // is spilled for (4096 x 8192 FP32 89.4 us, with the three kept 108);
+        // 16-bit rows of 512 threads take x - mean twice (8192 x 8192 BF16
+        // 94.2 us, 96.0 with xh kept)
+        constexpr bool kKeep = sizeof(T) == 4 || TPR < 512;
+        float2 xh[kKeep ? NE / 2 : 1], g[NE / 2], t0 = both(0.0f), t1 = both(0.0f);
         if (real) {
             Tile::load(rx, ring.row(0), D, lane);
             Tile::load(rdy, ring.row(1), D, lane);
             if (dsum) Tile::load(out, ring.row(2), D, lane);
 #pragma unroll
             for (int j = 0; j < NE / 2; j++) {
-                const float2 xh = fma2(Tile::pair(rx, j), both(r), both(mr));
+                // (a vector past D, all zeros, keeps its zeros: xh stays finite)
+                const float off = Tile::column(j / (Tile::kVec / 2), lane) < D ? m : 0.0f;
+                const float2 h = normalised(Tile::pair(rx, j), off, r);
                 const float2 d = Tile::pair(rdy, j);
-                dw[j] = fma2(d, xh, dw[j]);
+                dw[j] = fma2(d, h, dw[j]);
                 db[j] = add2(db[j], d);
                 g[j] = mul2(d, p[j]);
                 t0 = add2(t0, g[j]);
-                t1 = fma2(g[j], xh, t1);
+                t1 = fma2(g[j], h, t1);
+                if constexpr (kKeep) {
+                    xh[j] = h;
+                    g[j] = mul2(g[j], both(r));
+                    if (dsum) g[j] = add2(g[j], Tile::pair(out, j));
+                }
             }
         }
         float s[2] = {t0.x + t0.y, t1.x + t1.y};
@@ -734,11 +779,13 @@ layernorm_bwd_ring_kernel(const T *dy, long long lddy, const T *x, long long ldx
         if (real && ring.good) {
 #pragma unroll
             for (int j = 0; j < NE / 2; j++) {
-                // xh again: kept, it would be spilled, and a load from local
-                // memory queues behind the stores
-                const float2 xh = fma2(Tile::pair(rx, j), both(r), both(mr));
-                float2 v = fma2(g[j], both(r), fma2(xh, m2, m1));
-                if (dsum) v = add2(v, Tile::pair(out, j));
+                float2 v;
+                if constexpr (kKeep) {
+                    v = add2(g[j], fma2(xh[j], m2, m1));
+                } else {
+                    v = dx_of(Tile::pair(rx, j), m, r, g[j], m1, m2);
+                    if (dsum) v = add2(v, Tile::pair(out, j));
+                }
                 Tile::set_pair(out, j, v);
             }
             Tile::store(dx, out, D, lane);
@@ -825,23 +872,24 @@ layernorm_bwd_group_kernel(const T *dy, const T *x, const T *dsum, T *dx, const 
             const bool real = q < count;
             T *row = ring.buffer(0) + q * D;
             typename Tile::Raw rx = {}, rd = {};
-            float2 g[NP], t0 = both(0.0f), t1 = both(0.0f);
-            float r = 0.0f, mr = 0.0f;
+            float2 xh[NP], g[NP], t0 = both(0.0f), t1 = both(0.0f);
+            float r = 0.0f;
             if (real) {
                 tile.load(rx, row);
                 tile.load(rd, ring.buffer(1) + q * D);
-                // x r - mean r: off by the rounding of mean r, u |mean| r
+                const float m = stats[it & 1][q].x;
                 r = stats[it & 1][q].y;
-                mr = -stats[it & 1][q].x * r;
 #pragma unroll
                 for (int j = 0; j < NP; j++) {
-                    const float2 xh = fma2(Tile::pair(rx, j), both(r), both(mr));
+                    // (a place outside the row, a zero, keeps it: xh stays finite)
+                    const float2 c = fma2(tile.ones(j), both(-m), Tile::pair(rx, j));
+                    xh[j] = mul2(c, both(r));
                     const float2 d = Tile::pair(rd, j);
-                    dw[j] = fma2(d, xh, dw[j]);
+                    dw[j] = fma2(d, xh[j], dw[j]);
                     db[j] = add2(db[j], d);
                     g[j] = mul2(d, p[j]);
                     t0 = add2(t0, g[j]);
-                    t1 = fma2(g[j], xh, t1);
+                    t1 = fma2(g[j], xh[j], t1);
                 }
             }
             float s[2] = {t0.x + t0.y, t1.x + t1.y};
@@ -851,8 +899,7 @@ layernorm_bwd_group_kernel(const T *dy, const T *x, const T *dsum, T *dx, const 
             if (dsum) tile.load(rd, ring.buffer(2) + q * D);
 #pragma unroll
             for (int j = 0; j < NP; j++) {
-                const float2 xh = fma2(Tile::pair(rx, j), both(r), both(mr));
-                float2 v = fma2(g[j], both(r), fma2(xh, m2, m1));
+                float2 v = fma2(g[j], both(r), fma2(xh[j], m2, m1));
                 if (dsum) v = add2(v, Tile::pair(rd, j));
                 Tile::set_pair(rx, j, v);
             }

@@ -354,6 +354,10 @@ struct WordTile {
     __device__ __forceinline__ bool inside(int j, int h) const {
         return (j >= 1 && j < NP / 2) || (in[h] >> j & 1);
     }
+    // 1 for the pair's values inside the row, 0 for those outside
+    __device__ __forceinline__ float2 ones(int j) const {
+        return make_float2(inside(j, 0) ? 1.0f : 0.0f, inside(j, 1) ? 1.0f : 0.0f);
+    }
     // what lies outside is zero
     __device__ __forceinline__ void load(Raw &r, const T *row) const {
         if constexpr (kWords) {

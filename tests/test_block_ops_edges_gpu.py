@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import ppdl
-from test_block_ops_gpu import TYPES, bwd_want, close, gen, normal
+from test_block_ops_gpu import TYPES, U, bwd_want, close, gen, half, normal
 
 pytestmark = pytest.mark.gpu
 INF, NAN = float("inf"), float("nan")
@@ -118,3 +118,53 @@ def test_backward_infinite_gradient_of_the_last_row(cuda, rows, D, t):
     close(dw[keep], want[1][keep], tol[1][keep])
     close(db[keep], want[2][keep], tol[2][keep])
     close(dx[:-1], want[0][:-1], tol[0][:-1])
+
+
+FORMS = [(5, 31), (5, 64), (3, 100), (7, 257), (6, 333), (5, 641), (8, 1001), (5, 1153), (3, 2501), (3, 4097),
+         (2, 9999), (2, 16383), (2, 20001), (5, 256), (8, 1000), (5, 4096), (3, 8192), (3, 12000), (2, 16384), (2, 32768)]
+
+
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,D", FORMS)
+def test_backward_common_offset(cuda, rows, D, t):
+    """Rows whose values share a large offset: (x - mean) is taken first, one
+    rounding of a small difference, and its product with rstd another, in
+    every form; a product of the offset and rstd would be rounded to far more."""
+    T = TYPES[t]
+    g = gen(rows * 3 + D)
+    x = normal(g, rows, D, scale=1.0 if t == "f32" else 128.0, shift=2.0 ** 14, t=T)
+    mean = x.double().mean(-1).float()
+    rstd = (x.double().var(-1, unbiased=False) + 1e-5).rsqrt().float()
+    w = normal(g, D, shift=1.0, scale=0.2)
+    mm, r = mean.double()[:, None], rstd.double()[:, None]
+    xh = (x.double() - mm) * r
+    dy = (xh.float() / xh.abs().max().float() + 0.1 * normal(g, rows, D)).to(T)
+    gg = dy.double() * w.double()
+    m1, m2 = gg.mean(-1, keepdim=True), (gg * xh).mean(-1, keepdim=True)
+    want = r * (gg - m1 - xh * m2)
+    k = D / 32 + 24
+    size = gg.abs() + gg.abs().mean(-1, keepdim=True) + xh.abs() * (gg * xh).abs().mean(-1, keepdim=True)
+    # xh: 2 u; with it in two products and the two sums
+    tol = r * ((k + 8) * U * size) + (half(T) + U) * want.abs() + 1e-38
+    dx, dw, db = ppdl.layernorm_backward(dy, x, w, mean, rstd)
+    close(dx, want, tol)
+    # at most 8 rows: 8 additions, the product and xh's 2 u
+    p = dy.double() * xh
+    close(dw, p.sum(0), 12 * U * p.abs().sum(0) + 2 * U * p.sum(0).abs() + 1e-38)
+    close(db, dy.double().sum(0), 10 * U * dy.double().abs().sum(0) + 1e-38)
+
+
+@pytest.mark.parametrize("rows,D", FORMS + [(64001, 79), (17001, 257), (3651, 1153)])
+def test_backward_constant_rows_of_large_values(cuda, rows, D):
+    """x = mean = 2^90 and rstd = 2^50 (a constant row with a small eps): xh is
+    zero, although the product of mean and rstd passes FP32's range, in the
+    places past the row's end as well."""
+    for T in (torch.float32, torch.bfloat16):
+        x = torch.full((rows, D), 2.0 ** 90, device="cuda", dtype=T)
+        mean, rstd = torch.full((rows,), 2.0 ** 90, device="cuda"), torch.full((rows,), 2.0 ** 50, device="cuda")
+        dy = normal(gen(D), rows, D, t=T)
+        dx, dw, db = ppdl.layernorm_backward(dy, x, None, mean, rstd)
+        want, tol = bwd_want(dy, x * 0, None, mean * 0, rstd)
+        close(dx, want[0], tol[0])
+        assert (dw == 0).all()
+        close(db, want[2], tol[2])
