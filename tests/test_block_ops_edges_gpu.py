@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import ppdl
-from test_block_ops_gpu import TYPES, U, bwd_want, close, gen, half, normal
+from test_block_ops_gpu import TYPES, U, bwd_want, close, gen, half, normal, q_want
 
 pytestmark = pytest.mark.gpu
 INF, NAN = float("inf"), float("nan")
@@ -168,3 +168,57 @@ def test_backward_constant_rows_of_large_values(cuda, rows, D):
         close(dx, want[0], tol[0])
         assert (dw == 0).all()
         close(db, want[2], tol[2])
+
+
+LIN = [(1, 512, 200), (2, 300, 200), (16, 512, 1000), (5, 2047, 260), (40, 256, 96), (300, 256, 1024), (2400, 256, 256),
+       (5003, 200, 2100), (20, 4096, 4097), (100, 4096, 641), (2049, 513, 1025), (2570, 1024, 1537)]
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("M,K,N", LIN)
+def test_linear_far_scales(cuda, M, K, N, t):
+    """Scales whose product leaves FP32's normal range, with results inside
+    it: no digits lost, no NaN where a sum is zero; ordinary tokens and
+    channels beside them keep their bits."""
+    T = TYPES[t]
+    g = gen(M + K + N)
+    q = torch.randint(-127, 128, (M, (K + 15) // 16 * 16), generator=g).to(torch.int8).cuda()[:, :K]
+    w = torch.randint(-127, 128, (N, (K + 15) // 16 * 16), generator=g).to(torch.int8).cuda()[:, :K]
+    qs, ws = 1e-3 * (1 + torch.rand(M, generator=g)).cuda(), 1e-3 * (1 + torch.rand(N, generator=g)).cuda()
+    w[N // 2] = 0
+    clean = ppdl.linear_i8(q, w, ws, x_scale=qs, out_dtype=T)
+    acc = q.double() @ w.double().t()
+    for rows, cols in (((0, M - 1, M // 3), ()), ((), (0, N - 1, N // 2, N // 3)), ((M // 2, M - 1), (1, N // 2, N - 2))):
+        far_q, far_w = qs.clone(), ws.clone()
+        for i, r in enumerate(rows):
+            far_q[r] = (1e-37, 1e34, 1e-36)[i] if not cols else (1e-20, 1e24)[i % 2]
+        for i, c in enumerate(cols):
+            far_w[c] = (1e-37, 1e35, 1e37, 1e-36)[i] if not rows else (1e-20, 1e33, 1e-25)[i]
+        for act in ("none", "relu"):
+            y = ppdl.linear_i8(q, w, far_w, x_scale=far_q, act=act, out_dtype=T)
+            want = acc * far_q.double()[:, None] * far_w.double()
+            want = want.clamp_min(0) if act == "relu" else want
+            # a result past the type's range is an infinity of its sign, next to its end either
+            end = torch.finfo(T).max
+            tiny = {torch.float32: 2.0 ** -149, torch.bfloat16: 2.0 ** -133, torch.float16: 2.0 ** -24}[T]
+            inside = want.abs() < 0.99 * end
+            tol = (half(T) + 5 * U) * want.abs() + tiny
+            assert (y.isfinite() | ~inside).all()
+            close(torch.where(inside, y.double(), 0.0), torch.where(inside, want, 0.0), tol)
+            past = want.abs() > 1.01 * end
+            assert torch.equal(y[past].double(), want[past].sign() * INF)
+            if act == "none":
+                kr = [i for i in range(M) if i not in rows]
+                kc = [i for i in range(N) if i not in cols]
+                assert torch.equal(y[kr][:, kc], clean[kr][:, kc])
+
+
+def test_linear_tiny_tokens(cuda):
+    """Tokens of 1e-35 through weights of 1/16: results of 1e-34, normal
+    numbers, to a few roundings."""
+    g = gen(77)
+    for M in (1, 2, 40, 600):
+        x, (wq, ws) = normal(g, M, 256, scale=1e-35), ppdl.quantize_rows(normal(g, 96, 256, scale=1 / 16))
+        xq, xs = q_want(x)
+        want = (xq.double() @ wq.double().t()) * xs.double()[:, None] * ws.double()
+        close(ppdl.linear_i8(x, wq, ws), want, 5 * U * want.abs() + 2.0 ** -149)
