@@ -663,6 +663,14 @@ def _heads(x, out, name: str, lead, dim: int, dtype):
     return _pack_heads(x.data_ptr(), out.data_ptr(), shape[2], *i[:3], *o[:3])
 
 
+def _turned(x):
+    """A new tensor for x turned.  empty_like keeps a dense tensor's strides,
+    whichever their order; what it gives for a view whose elements overlap
+    (windows of a buffer) may not have contiguous heads."""
+    y = _tt["empty_like"](x)
+    return y if y.stride(-1) == 1 else x.new_empty(x.shape)
+
+
 def rotary(q, k, positions, freq, sections, *, interleaved: bool = False, inverse: bool = False,
            inplace: bool = False):
     """Rotary positions with several axes (ppdl_rotary) on q [batch, length,
@@ -684,11 +692,10 @@ def rotary(q, k, positions, freq, sections, *, interleaved: bool = False, invers
     if dev != _tt["current"]():
         return _elsewhere(dev, rotary, q, k, positions, freq, sections, interleaved=interleaved,
                           inverse=inverse, inplace=inplace)
-    # (empty_like keeps a dense tensor's strides, whichever their order)
-    qo, ko, hk = q if inplace else _tt["empty_like"](q), None, None
+    qo, ko, hk = q if inplace else _turned(q), None, None
     hq = _heads(q, qo, "q", lead, dim, q.dtype)
     if k is not None:
-        ko = k if inplace else _tt["empty_like"](k)
+        ko = k if inplace else _turned(k)
         hk = _heads(k, ko, "k", lead, dim, q.dtype)
     if lead[0] > 0x7fffffff or lead[1] > 0x7fffffff:
         raise ValueError("batch and length must fit 31 bits")

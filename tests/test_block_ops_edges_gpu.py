@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import ppdl
-from test_block_ops_gpu import TYPES, U, bwd_want, close, gen, half, normal, q_want
+from test_block_ops_gpu import TYPES, U, bwd_want, close, gen, half, normal, q_want, rot_want
 
 pytestmark = pytest.mark.gpu
 INF, NAN = float("inf"), float("nan")
@@ -222,3 +222,20 @@ def test_linear_tiny_tokens(cuda):
         xq, xs = q_want(x)
         want = (xq.double() @ wq.double().t()) * xs.double()[:, None] * ws.double()
         close(ppdl.linear_i8(x, wq, ws), want, 5 * U * want.abs() + 2.0 ** -149)
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_rotary_overlapping_inputs(cuda, interleaved, t):
+    """Windows of one buffer and expanded views as queries and keys: the
+    results are tensors of their own."""
+    g = gen(31)
+    T, B, L, H, D = TYPES[t], 2, 5, 3, 8
+    base = normal(g, 400, t=T)
+    pos, freq = torch.arange(B * L, device="cuda").view(1, B, L), torch.rand(D // 2, generator=g).double().cuda()
+    for strides in ((100, 30, 1, 1), (100, 1, 8, 1), (1, 50, 8, 1), (24, 1, 8, 1), (0, 8, 16, 1), (100, 0, 8, 1),
+                    (100, 24, 0, 1), (0, 0, 0, 1), (120, 24, 8, 1), (100, 3, 12, 1)):
+        x = base.as_strided((B, L, H, D), strides)
+        want, tol = rot_want(x, pos, freq, (D // 2,), interleaved, False)
+        for y in ppdl.rotary(x, x, pos, freq, (D // 2,), interleaved=interleaved):
+            close(y, want, tol)
