@@ -351,7 +351,8 @@ PPDL_OPS_API long long ppdl_linear_i8_dynamic_workspace(int M, int K);
    b*batch + t*token + h*head + d (elements). */
 typedef struct {
     const void * in;
-    void *       out;    /* may be in, with the same strides */
+    void *       out;    /* may be in, with the same strides; no two of its heads
+                            may overlap */
     int32_t      heads;  /* at most 65535; 0: none */
     int64_t      in_batch, in_token, in_head;
     int64_t      out_batch, out_token, out_head;

@@ -86,6 +86,27 @@ int linear_i8(const int8_t *q, long long ldq, const float *q_scale, const int8_t
     return status_of(ppdl::launch_linear_i8(a, (cudaStream_t)stream), "linear_i8: sizes too large");
 }
 
+// True when the results of some heads certainly share memory: heads of dim
+// values nearer to one another than that, or equal steps of two dimensions.
+bool results_overlap(const ppdl_rotary_heads &h, int batch, int length, int dim) {
+    const long long n[3] = {batch, length, h.heads};
+    const long long step[3] = {h.out_batch, h.out_token, h.out_head};
+    for (int i = 0; i < 3; i++) {
+        if (n[i] < 2) continue;
+        if (step[i] < dim && step[i] > -dim) return true;
+        for (int j = 0; j < i; j++)
+            if (n[j] > 1 && (step[i] == step[j] || step[i] + step[j] == 0)) return true;
+    }
+    return false;
+}
+
+// True when heads turned in place would be written where others are read.
+bool moved_in_place(const ppdl_rotary_heads &h, int batch, int length) {
+    return h.in == h.out &&
+           ((batch > 1 && h.in_batch != h.out_batch) || (length > 1 && h.in_token != h.out_token) ||
+            (h.heads > 1 && h.in_head != h.out_head));
+}
+
 }  // namespace
 
 extern "C" {
@@ -225,6 +246,10 @@ PPDL_OPS_API int ppdl_rotary(const ppdl_rotary_heads *q, const ppdl_rotary_heads
         if (h[i]->heads < 0 || h[i]->heads > 65535 || (some && (!h[i]->in || !h[i]->out)) ||
             !aligned(h[i]->in, ppdl::elem_size(type)) || !aligned(h[i]->out, ppdl::elem_size(type)))
             return refuse("rotary: bad number of heads, or null or misaligned heads");
+        if (some && (results_overlap(*h[i], batch, length, dim) || moved_in_place(*h[i], batch, length)))
+            return refuse("rotary: results that overlap, or heads turned in place with other strides");
+        if (some && i == 1 && a.h[0].heads && a.h[0].out == h[1]->out)
+            return refuse("rotary: queries and keys turned into the same place");
         ppdl::RotaryHeads &o = a.h[i];
         o.in = h[i]->in; o.out = h[i]->out; o.heads = h[i]->heads;
         o.in_bs = h[i]->in_batch; o.in_ts = h[i]->in_token; o.in_hs = h[i]->in_head;

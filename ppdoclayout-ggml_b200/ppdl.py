@@ -675,7 +675,8 @@ def rotary(q, k, positions, freq, sections, *, interleaved: bool = False, invers
            inplace: bool = False):
     """Rotary positions with several axes (ppdl_rotary) on q [batch, length,
     heads, dim] and k (its own number of heads, or None): returns both turned
-    (new tensors, or q and k themselves with inplace).  positions int32 or
+    (new tensors, or q and k themselves with inplace, which must not overlap
+    then).  positions int32 or
     int64 [axes, batch, length] (may be expanded views); freq float64
     [rotated / 2] in radians per position turns the first `rotated` values of
     every head; sections says how many consecutive pairs each axis turns.
