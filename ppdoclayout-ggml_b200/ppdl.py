@@ -396,13 +396,14 @@ _types, _tt = {}, {}
 def _bind() -> None:
     import torch
     lib()
-    _types.update({torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16})
     # the current stream's handle without the object around it (2 us)
     raw = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
         (lambda i: torch.cuda.current_stream(i).cuda_stream)
     _tt.update(f32=torch.float32, f64=torch.float64, i8=torch.int8,
                integers=(torch.int32, torch.int64), empty_like=torch.empty_like, stream=raw,
                current=torch.cuda.current_device, device=torch.cuda.device)
+    # last: a thread that finds it filled goes on without binding
+    _types.update({torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16})
 
 
 def _type(t, name: str) -> int:

@@ -1,5 +1,9 @@
 """Refusals and first calls of the transformer-block operators that need no
 GPU.  The pointers are made up and never read."""
+import os
+import subprocess
+import sys
+
 import pytest
 
 import ppdl
@@ -25,3 +29,41 @@ def test_rotary_queries_and_keys_in_the_same_place():
     k = ppdl.RotaryHeads(3 * P, 2 * P, 1, 64, 16, 8, 64, 16, 8)
     assert rotary(q=ppdl.C.byref(q), k=ppdl.C.byref(k)) == ppdl.PPDL_ERR_SHAPE
     assert ppdl.last_error().endswith("the same place")
+
+
+FIRST = """
+import sys, threading
+sys.path.insert(0, sys.argv[1])
+import torch, ppdl
+x, q, s = torch.zeros(4, 16), torch.zeros(4, 16, dtype=torch.int8), torch.ones(4)
+filled, go = threading.Event(), threading.Event()
+class Slow(dict):
+    def update(self, *a, **kw):
+        super().update(*a, **kw)
+        if threading.current_thread() is first:
+            filled.set()
+            assert go.wait(60)
+setattr(ppdl, sys.argv[2], Slow())
+def call(errors):
+    for f in (lambda: ppdl.layernorm(x), lambda: ppdl.linear_i8(x, q, s), lambda: ppdl.quantize_rows(x)):
+        try:
+            f()
+        except Exception as e:
+            errors.append(type(e).__name__)
+ours, theirs = [], []
+first = threading.Thread(target=call, args=(theirs,))
+first.start()
+assert filled.wait(60)
+call(ours)
+go.set()
+first.join()
+assert ours == theirs == ["ValueError"] * 3, (ours, theirs)
+"""
+
+
+@pytest.mark.parametrize("name", ["_types", "_tt"])
+def test_first_calls_of_two_threads(name):
+    """A thread whose first call comes while another's is between filling one
+    of the module's tables and the other: it is told that its tensors are on
+    no GPU, not that a table lacks an entry."""
+    subprocess.run([sys.executable, "-c", FIRST, os.path.dirname(ppdl.__file__), name], check=True, timeout=300)
