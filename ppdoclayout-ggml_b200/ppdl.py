@@ -690,6 +690,10 @@ def rotary(q, k, positions, freq, sections, *, interleaved: bool = False, invers
         raise ValueError("positions must be int32 or int64 [axes, batch, length], one axis a section")
     if freq.dtype != _tt["f64"] or freq.dim() != 1 or not freq.is_contiguous():
         raise ValueError("freq must be contiguous float64 [rotated / 2]")
+    # (what the library takes as 32-bit numbers)
+    if max(q.shape) > 0x7fffffff or freq.numel() > 0x3fffffff or \
+            (k is not None and max(k.shape) > 0x7fffffff):
+        raise ValueError("batch, length, heads, dim and rotated must fit 31 bits each")
     dev = _device(q, k, positions, freq)
     if dev != _tt["current"]():
         return _elsewhere(dev, rotary, q, k, positions, freq, sections, interleaved=interleaved,
@@ -699,8 +703,6 @@ def rotary(q, k, positions, freq, sections, *, interleaved: bool = False, invers
     if k is not None:
         ko = k if inplace else _turned(k)
         hk = _heads(k, ko, "k", lead, dim, q.dtype)
-    if lead[0] > 0x7fffffff or lead[1] > 0x7fffffff:
-        raise ValueError("batch and length must fit 31 bits")
     fn = _lib.ppdl_rotary
     status = fn(hq, hk, t, *lead, dim, 2 * freq.numel(), positions.data_ptr(),
                 positions.element_size(), *positions.stride(), axes, _sections(tuple(sections)),
@@ -712,4 +714,7 @@ def rotary(q, k, positions, freq, sections, *, interleaved: bool = False, invers
 
 @functools.lru_cache(maxsize=64)
 def _sections(sections):
-    return (C.c_int32 * len(sections))(*sections)
+    a = (C.c_int32 * len(sections))(*sections)
+    if tuple(a) != sections:
+        raise ValueError(f"sections {sections} do not fit 31 bits")
+    return a

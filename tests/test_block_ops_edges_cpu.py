@@ -5,6 +5,7 @@ import subprocess
 import sys
 
 import pytest
+import torch
 
 import ppdl
 from test_block_ops_cpu import P, rotary
@@ -29,6 +30,22 @@ def test_rotary_queries_and_keys_in_the_same_place():
     k = ppdl.RotaryHeads(3 * P, 2 * P, 1, 64, 16, 8, 64, 16, 8)
     assert rotary(q=ppdl.C.byref(q), k=ppdl.C.byref(k)) == ppdl.PPDL_ERR_SHAPE
     assert ppdl.last_error().endswith("the same place")
+
+
+def test_rotary_sizes_of_more_than_31_bits():
+    """Sizes that would be cut to 32 bits on their way into the library (a
+    section of 2^32 + 1 pairs to one of one)."""
+    one = torch.zeros(1)
+    q, pos, freq = one.expand(1, 1, 1, 2), torch.zeros(1, 1, 1, dtype=torch.int64), torch.ones(1).double()
+    for shape in ((1, 1, 1, 2 ** 32 + 2), (1, 1, 2 ** 32 + 1, 2), (2 ** 32 + 1, 1, 1, 2)):
+        big = one.expand(shape)
+        with pytest.raises(ValueError, match="31 bits"):
+            ppdl.rotary(big, None, pos.expand(1, *shape[:2]), freq, (1,))
+    with pytest.raises(ValueError, match="31 bits"):
+        ppdl.rotary(q, one.expand(1, 1, 2 ** 31, 2), pos, freq, (1,))
+    with pytest.raises(ValueError, match="31 bits"):
+        ppdl._sections((2 ** 32 + 1,))
+    assert list(ppdl._sections((3, 0, 5))) == [3, 0, 5]
 
 
 FIRST = """
