@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import ppdl
-from test_block_ops_gpu import TYPES, U, bwd_want, close, gen, half, normal, q_want, rot_want
+from test_block_ops_gpu import TYPES, U, bwd_want, close, gen, half, ln_want, normal, q_want, rot_want
 
 pytestmark = pytest.mark.gpu
 INF, NAN = float("inf"), float("nan")
@@ -239,3 +239,68 @@ def test_rotary_overlapping_inputs(cuda, interleaved, t):
         want, tol = rot_want(x, pos, freq, (D // 2,), interleaved, False)
         for y in ppdl.rotary(x, x, pos, freq, (D // 2,), interleaved=interleaved):
             close(y, want, tol)
+
+
+@pytest.mark.parametrize("t,rows,D", [("bf16", 2200000, 1024), ("f16", 1900001, 1153), ("bf16", 560000, 4001),
+                                      ("f32", 140000, 16384)])
+def test_norm_offsets_past_31_bits(cuda, t, rows, D):
+    """More than 2^31 values: the first and last rows against the definition,
+    the weights' gradients by gradients that are zero elsewhere."""
+    T = TYPES[t]
+    assert rows * D > 2 ** 31
+    x = torch.empty((rows, D), device="cuda", dtype=T)
+    x[:] = normal(gen(1), 1, D, t=T)
+    ends = [slice(0, 300), slice(rows - 300, rows)]
+    for i, e in enumerate(ends):
+        x[e] = normal(gen(2 + i), 300, D, t=T)
+    w, b = normal(gen(5), D, shift=1.0, scale=0.3), normal(gen(6), D)
+    y, mean, rstd = ppdl.layernorm(x, w, b, return_stats=True)
+    for e in ends:
+        want = ln_want(x[e], w, b, 1e-5)
+        close(y[e], want[0], want[4])
+    q, scale = ppdl.quantize_rows(x)
+    for e in ends:
+        wq, ws = q_want(x[e])
+        assert torch.equal(q[e], wq) and torch.equal(scale[e], ws)
+    del q, scale
+    y.zero_()
+    for i, e in enumerate(ends):
+        y[e] = normal(gen(7 + i), 300, D, t=T)
+    dx, dw, db = ppdl.layernorm_backward(y, x, w, mean, rstd)
+    both = torch.cat([torch.arange(rows, device="cuda")[e] for e in ends])
+    want, tol = bwd_want(y[both], x[both], w, mean[both], rstd[both])
+    # a column's sum takes in rows / 128 + 320 terms in a row at most, all but 600 zeros
+    for got, a, c in zip((dx[both], dw, db), want, tol):
+        close(got, a, c)
+    assert (dx[300:rows - 300] == 0).all()
+
+
+def test_linear_offsets_past_31_bits(cuda):
+    M, K, N = 1100000, 2000, 2100
+    q = torch.zeros((M, K), device="cuda", dtype=torch.int8)
+    ends = [slice(0, 300), slice(M - 300, M)]
+    g = gen(9)
+    for e in ends:
+        q[e] = torch.randint(-128, 128, (300, K), generator=g).to(torch.int8).cuda()
+    w = torch.randint(-128, 128, (N, K), generator=g).to(torch.int8).cuda()
+    y = ppdl.linear_i8(q, w, torch.ones(N, device="cuda"), x_scale=torch.ones(M, device="cuda"))
+    assert y.numel() > 2 ** 31 and q.numel() > 2 ** 31
+    for e in ends:
+        want = q[e].double() @ w.double().t()
+        assert float(want.abs().max()) < 2 ** 24 and torch.equal(y[e].double(), want)
+    assert (y[300:M - 300] == 0).all()
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("dim", [128, 126])
+def test_rotary_offsets_past_31_bits(cuda, dim, interleaved):
+    B, L, H = 2, 540000, 16
+    qk = torch.empty((B, L, H, dim), device="cuda", dtype=torch.bfloat16)
+    assert qk.numel() > 2 ** 31
+    qk[:] = normal(gen(3), 1, 1, H, dim, t=torch.bfloat16)
+    pos = torch.arange(L, device="cuda").view(1, 1, L).expand(1, B, L)
+    freq = 10000.0 ** (-torch.arange(dim // 2, dtype=torch.float64, device="cuda") / 64)
+    y, _ = ppdl.rotary(qk, None, pos, freq, (dim // 2,), interleaved=interleaved)
+    for e in (slice(0, 200), slice(L - 200, L)):
+        want, tol = rot_want(qk[:, e], pos[:, :, e], freq, (dim // 2,), interleaved, False)
+        close(y[:, e], want, tol)
