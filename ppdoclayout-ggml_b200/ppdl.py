@@ -654,22 +654,26 @@ def linear_i8(x, weight, w_scale, *, x_scale=None, bias=None, act: str = "none",
     return y
 
 
-def _heads(x, out, name: str, lead, dim: int, dtype):
+def _heads(x, inplace: bool, name: str, lead, dim: int, dtype):
+    """ppdl_rotary_heads for x, and the tensor that takes it turned."""
     shape = x.shape
-    if len(shape) != 4 or shape[3] != dim or shape[:2] != lead or x.dtype != dtype:
-        raise ValueError(f"{name} must be [batch, length, heads, {dim}] of one type")
-    i, o = x.stride(), out.stride()
+    if len(shape) != 4 or shape[3] != dim or shape[:2] != lead or x.dtype != dtype or \
+            shape[2] > 0x7fffffff:
+        raise ValueError(f"{name} must be [batch, length, heads, {dim}] of one type, heads of 31 bits")
+    i = x.stride()
     if dim > 1 and i[3] != 1:
         raise ValueError(f"{name}'s heads must be contiguous")
-    return _pack_heads(x.data_ptr(), out.data_ptr(), shape[2], *i[:3], *o[:3])
-
-
-def _turned(x):
-    """A new tensor for x turned.  empty_like keeps a dense tensor's strides,
-    whichever their order; what it gives for a view whose elements overlap
-    (windows of a buffer) may not have contiguous heads."""
-    y = _tt["empty_like"](x)
-    return y if y.stride(-1) == 1 else x.new_empty(x.shape)
+    out, o = x, i
+    if not inplace:
+        # empty_like keeps a dense tensor's strides, whichever their order; what
+        # it gives for a view whose elements overlap (windows of a buffer) may
+        # not have contiguous heads
+        out = _tt["empty_like"](x)
+        o = out.stride()
+        if o[3] != 1:
+            out = x.new_empty(shape)
+            o = out.stride()
+    return _pack_heads(x.data_ptr(), out.data_ptr(), shape[2], *i[:3], *o[:3]), out
 
 
 def rotary(q, k, positions, freq, sections, *, interleaved: bool = False, inverse: bool = False,
@@ -690,21 +694,20 @@ def rotary(q, k, positions, freq, sections, *, interleaved: bool = False, invers
         raise ValueError("positions must be int32 or int64 [axes, batch, length], one axis a section")
     if freq.dtype != _tt["f64"] or freq.dim() != 1 or not freq.is_contiguous():
         raise ValueError("freq must be contiguous float64 [rotated / 2]")
+    pairs = freq.numel()
     # (what the library takes as 32-bit numbers)
-    if max(q.shape) > 0x7fffffff or freq.numel() > 0x3fffffff or \
-            (k is not None and max(k.shape) > 0x7fffffff):
-        raise ValueError("batch, length, heads, dim and rotated must fit 31 bits each")
+    if dim > 0x7fffffff or lead[0] > 0x7fffffff or lead[1] > 0x7fffffff or pairs > 0x3fffffff:
+        raise ValueError("batch, length, dim and rotated must fit 31 bits each")
     dev = _device(q, k, positions, freq)
     if dev != _tt["current"]():
         return _elsewhere(dev, rotary, q, k, positions, freq, sections, interleaved=interleaved,
                           inverse=inverse, inplace=inplace)
-    qo, ko, hk = q if inplace else _turned(q), None, None
-    hq = _heads(q, qo, "q", lead, dim, q.dtype)
+    ko = hk = None
+    hq, qo = _heads(q, inplace, "q", lead, dim, q.dtype)
     if k is not None:
-        ko = k if inplace else _turned(k)
-        hk = _heads(k, ko, "k", lead, dim, q.dtype)
+        hk, ko = _heads(k, inplace, "k", lead, dim, q.dtype)
     fn = _lib.ppdl_rotary
-    status = fn(hq, hk, t, *lead, dim, 2 * freq.numel(), positions.data_ptr(),
+    status = fn(hq, hk, t, *lead, dim, 2 * pairs, positions.data_ptr(),
                 positions.element_size(), *positions.stride(), axes, _sections(tuple(sections)),
                 freq.data_ptr(), interleaved, inverse, _tt["stream"](dev))
     if status:

@@ -35,14 +35,13 @@ def test_rotary_queries_and_keys_in_the_same_place():
 def test_rotary_sizes_of_more_than_31_bits():
     """Sizes that would be cut to 32 bits on their way into the library (a
     section of 2^32 + 1 pairs to one of one)."""
-    one = torch.zeros(1)
-    q, pos, freq = one.expand(1, 1, 1, 2), torch.zeros(1, 1, 1, dtype=torch.int64), torch.ones(1).double()
-    for shape in ((1, 1, 1, 2 ** 32 + 2), (1, 1, 2 ** 32 + 1, 2), (2 ** 32 + 1, 1, 1, 2)):
-        big = one.expand(shape)
+    one, freq = torch.zeros(1), torch.ones(1).double()
+    for shape in ((1, 1, 1, 2 ** 32 + 2), (2 ** 32 + 1, 1, 1, 2), (1, 2 ** 31, 1, 2)):
+        pos = torch.zeros(1, 1, 1, dtype=torch.int64).expand(1, *shape[:2])
         with pytest.raises(ValueError, match="31 bits"):
-            ppdl.rotary(big, None, pos.expand(1, *shape[:2]), freq, (1,))
+            ppdl.rotary(one.expand(shape), None, pos, freq, (1,))
     with pytest.raises(ValueError, match="31 bits"):
-        ppdl.rotary(q, one.expand(1, 1, 2 ** 31, 2), pos, freq, (1,))
+        ppdl._heads(one.expand(1, 1, 2 ** 32 + 1, 2), True, "q", (1, 1), 2, torch.float32)
     with pytest.raises(ValueError, match="31 bits"):
         ppdl._sections((2 ** 32 + 1,))
     assert list(ppdl._sections((3, 0, 5))) == [3, 0, 5]
