@@ -16,8 +16,8 @@
 // Memory bounds all of it: a few operations a value, and every value is read
 // and written once.  Measured (copy rate 6.54 TB/s): forward 52500 x 256 FP32
 // with residual, stored sum and statistics 33.6 us (98 % of it), 8192 x 4096
-// BF16 30.1 (68 %), backward 16384 x 4096 BF16 84.4 (73 %), 52500 x 256 FP32
-// 33 (75 %); one row of 4096 3.1 us, 2400 x 256 backward 8 us in two kernels,
+// BF16 30.1 (68 %), backward 16384 x 4096 BF16 87.2 (71 %), 52500 x 256 FP32
+// 34 (73 %); one row of 4096 3.1 us, 2400 x 256 backward 8 us in two kernels,
 // which is latency.  Rows in registers for what has few rows or is narrow;
 // rings of bulk copies where more bytes have to be in flight than registers
 // hold; groups of rows through shared memory where rows are no whole vectors;
@@ -1118,9 +1118,10 @@ Status launch_layernorm(const LayerNormArgs &a, cudaStream_t st) {
         };
         // other dense rows through groups (16771 x 2001 BF16 38.8 us, by the
         // tile 48.7; 29104 x 1153 40.2 / 49.9; 52350 x 641 FP32 56.6 / 85.5),
-        // unless they are narrow (200000 x 100 BF16 33.0 / 31.4) or few (3640 x
-        // 1153 8.9 / 7.5, 2043 x 257 3.6 / 2.5), or FP32 with a residual (29101
-        // x 1153 96 / 80: three stages of two matrices leave one block an SM)
+        // unless they are narrow (200000 x 100 BF16 33.0 / 31.4) or few (2043 x
+        // 257 3.6 / 2.5; the switch is below the crossover: 3640 x 1153, a
+        // group's, 8.9 / 7.5), or FP32 with a residual (29101 x 1153 96 / 80:
+        // three stages of two matrices leave one block an SM)
         if (!vec && a.D > 256 && a.rows * a.D >= 1 << 22 && !(sizeof(T) == 4 && a.res.p) &&
             group_dispatch<false>(a.D, group))
             return cuda_status();
@@ -1237,9 +1238,10 @@ Status launch_layernorm_backward(const LayerNormBackwardArgs &a, cudaStream_t st
         // rows spill; wider than 4096 they have to)
         constexpr int kNE = 32 / (int)sizeof(T);
         // dense rows that are no vectors go through groups (50000 x 1153 FP16
-        // 95.5 us, 142 by the tile; FP32 122 / 171; 200000 x 79 BF16 34 / 73),
-        // unless they are narrow (200000 x 51 BF16 36 / 26) or few (4191 x 1001
-        // BF16 17.7 / 14.9, 16761 x 1001 33.2 / 36.4)
+        // 95.5 us, 142 by the tile; FP32 122 / 171; 200000 x 79 BF16 36 / 73;
+        // 16761 x 1001 34 / 36.4), unless they are narrow (200000 x 51 BF16 36 /
+        // 26) or few (the switch is below the crossover: 4191 x 1001, a
+        // group's, 17.7 / 14.9)
         const bool done =
             a.rows == 0 ||
             (vec ? ring_dispatch<kNE>(a.D, [&](auto tpr) { return ring(tpr, Int<kNE>{}); }) ||
@@ -1268,7 +1270,7 @@ Status launch_layernorm_backward(const LayerNormBackwardArgs &a, cudaStream_t st
             tile(Int<512>{}, Int<8>{});
         } else {
             // two readings: dx row by row, the weights' gradients column by
-            // column (14000 x 4097 BF16 211 us, in one reading with 1024
+            // column (14000 x 4097 BF16 208 us, in one reading with 1024
             // threads a row and one block an SM 397; 100 x 5001 FP32 7.8 / 12)
             auto dx = [&](auto kernel, int threads) {
                 pdl_launch(kernel, (unsigned)a.rows, threads, 0, st, (const T *)a.dy.p, a.dy.ld,

@@ -34,10 +34,11 @@
 // launch.
 //
 // Measured: 8192 cubed BF16 410-440 us (2.5-2.7 POP/s, the power cap at work),
-// 4096 cubed 53 us (2.6), 52500 x 256 -> 1536 FP32 58.3 us (the result's bytes:
-// 6.5 TB/s), one token of 4096 -> 4096 8.9 us quantised in the call (the weights'
-// 16.8 MB take 2.6; launch, cluster exchange and one trip to memory the rest),
-// 2400 x 256 -> 1024 FP32 5.2 us (latency).
+// 4096 cubed 53 us (2.6), 52500 x 256 -> 1536 FP32 58.6 us (the result's bytes:
+// 6.5 TB/s), one token of 4096 -> 4096 9.8 us quantised in the call (the weights'
+// 16.8 MB take 2.6; launch, two trips to memory, the second behind the
+// quantisation, and the cluster exchange the rest), 2400 x 256 -> 1024 FP32 6.2
+// us (latency).
 //
 // Every mbarrier wait is bounded; on expiry the kernel raises a device error
 // flag, all roles drain out and TMEM is released (ppdl_op_device_error).

@@ -211,7 +211,7 @@ __device__ __forceinline__ void ring_drain(uint32_t full, int stages, int fills,
 // behind a barrier of the team, by one of its warps in turn, so that the
 // copies' issue is neither on one warp's path nor repeated by all (with a
 // slice of the row for every warp the backward pass of 16384 x 4096 BF16 took
-// 95 us, so 84.4).  Every wait is bounded; a thread that gave up goes on
+// 95 us, so 87).  Every wait is bounded; a thread that gave up goes on
 // through its rows (barriers stay matched), stores nothing and drains the
 // ring.
 constexpr int kRingStages = 8;  // at most
