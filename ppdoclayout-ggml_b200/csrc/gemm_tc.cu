@@ -1354,7 +1354,7 @@ typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t
 // The driver's tensor-map encoder, resolved once (a function-local static
 // initialiser runs exactly once even when several host threads make their
 // first call together).
-EncodeTiledFn encode_fn() {
+EncodeTiledFn driver_encode_fn() {
     static const EncodeTiledFn fn = []() -> EncodeTiledFn {
         void *p = nullptr;
         cudaDriverEntryPointQueryResult q;
@@ -1367,6 +1367,28 @@ EncodeTiledFn encode_fn() {
     }();
     return fn;
 }
+
+// The encoder on a host thread that may not have used the GPU yet.  The
+// driver takes the thread's current context; a runtime call would bind the
+// current device's to such a thread, but encoding comes before the first.
+CUresult encode_bound(CUtensorMap *tm, CUtensorMapDataType type, cuuint32_t rank, void *base,
+                      const cuuint64_t *dims, const cuuint64_t *strides, const cuuint32_t *box,
+                      const cuuint32_t *steps, CUtensorMapInterleave interleave,
+                      CUtensorMapSwizzle swizzle, CUtensorMapL2promotion l2,
+                      CUtensorMapFloatOOBfill fill) {
+    auto encode = [&] {
+        return driver_encode_fn()(tm, type, rank, base, dims, strides, box, steps, interleave,
+                                  swizzle, l2, fill);
+    };
+    CUresult rc = encode();
+    int dev = 0;
+    if ((rc == CUDA_ERROR_INVALID_CONTEXT || rc == CUDA_ERROR_NOT_INITIALIZED) &&
+        cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess)
+        rc = encode();
+    return rc;
+}
+
+EncodeTiledFn encode_fn() { return driver_encode_fn() ? encode_bound : nullptr; }
 
 bool encode3d(CUtensorMap *tm, const void *base, uint64_t d0, uint64_t d1, uint64_t d2,
               uint64_t s1_bytes, uint64_t s2_bytes, uint32_t b0, uint32_t b1,

@@ -1,6 +1,9 @@
 """Calls of the transformer-block operators at the edges of what they take:
 infinities, NaNs and far scales in the data, overlapping views, widths next
 to 2^31.  Tolerances count roundings as in test_block_ops_gpu."""
+import ctypes
+import threading
+
 import pytest
 import torch
 
@@ -304,3 +307,47 @@ def test_rotary_offsets_past_31_bits(cuda, dim, interleaved):
     for e in (slice(0, 200), slice(L - 200, L)):
         want, tol = rot_want(qk[:, e], pos[:, :, e], freq, (dim // 2,), interleaved, False)
         close(y[:, e], want, tol)
+
+
+def test_first_call_of_a_new_thread(cuda):
+    """A host thread that has not used the GPU before: its first call may be
+    any of the operators, those that make tensor maps among them."""
+    g = gen(41)
+    x, few = normal(g, 300, 512), normal(g, 2, 512)
+    wq, ws = ppdl.quantize_rows(normal(g, 96, 512))
+    q, s = ppdl.quantize_rows(x)
+    heads, pos = x.view(1, 300, 8, 64), torch.arange(300, device="cuda").view(1, 1, 300)
+    freq = torch.rand(32, generator=g).double().cuda()
+    _, mean, rstd = ppdl.layernorm(x, return_stats=True)
+    a, b = normal(g, 256, 128), normal(g, 64, 128)
+    L = ppdl.lib()
+
+    def gemm():
+        ws_, out = torch.empty(2 * 64 * 128, device="cuda"), torch.empty((256, 64), device="cuda")
+        P, LL = ctypes.c_void_p, ctypes.c_longlong
+        ppdl.check(L.ppdl_gemm_tf32x3(256, 64, 128, 1, P(a.data_ptr()), 0, LL(128), LL(256 * 128), P(b.data_ptr()),
+                                      P(ws_.data_ptr()), P(out.data_ptr()), LL(64), LL(1), LL(256 * 64),
+                                      P(torch.cuda.current_stream().cuda_stream)))
+        return out
+
+    calls = [lambda: ppdl.linear_i8(few, wq, ws), lambda: ppdl.linear_i8(few[:1], wq, ws),
+             lambda: ppdl.linear_i8(q, wq, ws, x_scale=s), lambda: ppdl.linear_i8(x, wq, ws), gemm,
+             lambda: ppdl.quantize_rows(x)[0], lambda: ppdl.layernorm(x),
+             lambda: ppdl.layernorm_backward(x, x, None, mean, rstd)[1], lambda: ppdl.rotary(heads, None, pos, freq, (32,))[0]]
+    want = [f() for f in calls]
+    torch.cuda.synchronize()
+    for f, w in zip(calls, want):
+        got = []
+
+        def run():
+            try:
+                got.append(f())
+            except Exception as e:
+                got.append(e)
+
+        t = threading.Thread(target=run)
+        t.start()
+        t.join()
+        torch.cuda.synchronize()
+        assert torch.is_tensor(got[0]), got[0]
+        assert torch.equal(got[0], w)
