@@ -351,3 +351,30 @@ def test_first_call_of_a_new_thread(cuda):
         torch.cuda.synchronize()
         assert torch.is_tensor(got[0]), got[0]
         assert torch.equal(got[0], w)
+
+
+@pytest.mark.parametrize("t", ["bf16", "f16"])
+@pytest.mark.parametrize("rows,D", [(3000, 2000), (1501, 4096), (1301, 8192), (9001, 513), (2100, 2049)])
+def test_norm_in_place_through_shared_memory(cuda, rows, D, t):
+    """Results over inputs where several rows are on their way at once: y over
+    x and the sum over the residual, and the other way round; x as its own
+    residual."""
+    g = gen(rows)
+    T, code, stream = TYPES[t], {"bf16": 1, "f16": 2}[t], torch.cuda.current_stream().cuda_stream
+    x, r, w = normal(g, rows, D, t=T), normal(g, rows, D, t=T), normal(g, D, t=T)
+    y, s = ppdl.layernorm(x, w, w, residual=r, return_sum=True)
+
+    def run(a, b, out, total):
+        ppdl.check(ppdl.lib().ppdl_layernorm(
+            a.data_ptr(), D, b.data_ptr(), D, w.data_ptr(), w.data_ptr(), code, code, rows, D, 1e-5, out.data_ptr(), D,
+            total.data_ptr() if total is not None else None, D, None, None, stream))
+
+    a, b = x.clone(), r.clone()
+    run(a, b, a, b)
+    assert torch.equal(a, y) and torch.equal(b, s)
+    a, b = x.clone(), r.clone()
+    run(a, b, b, a)
+    assert torch.equal(b, y) and torch.equal(a, s)
+    want = ppdl.layernorm(x, w, w, residual=x)
+    run(x, x, x, None)
+    assert torch.equal(x, want)
