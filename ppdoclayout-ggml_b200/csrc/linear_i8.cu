@@ -565,7 +565,8 @@ linear_i8_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
             // epilogue's barriers get, the epilogue has waited for.
             if constexpr (FORM == PAIR) {
                 for (long long j = it > S ? it - S : 0; j < it && ok; j++)
-                    ok = wait_for(bar_empty + 8 * (int)(j % S), (uint32_t)((j / S) & 1), abort_flag);
+                    ok = wait_for(bar_empty + 8 * (int)(j % S), (uint32_t)((j / S) & 1),
+                                  abort_flag);
                 int dummy = 0;
                 if (rank != 0) wait_for(bar_done, 0, (volatile int *)&dummy);
             }

@@ -246,8 +246,10 @@ PPDL_OPS_API int ppdl_rotary(const ppdl_rotary_heads *q, const ppdl_rotary_heads
         if (h[i]->heads < 0 || h[i]->heads > 65535 || (some && (!h[i]->in || !h[i]->out)) ||
             !aligned(h[i]->in, ppdl::elem_size(type)) || !aligned(h[i]->out, ppdl::elem_size(type)))
             return refuse("rotary: bad number of heads, or null or misaligned heads");
-        if (some && (results_overlap(*h[i], batch, length, dim) || moved_in_place(*h[i], batch, length)))
-            return refuse("rotary: results that overlap, or heads turned in place with other strides");
+        if (some && (results_overlap(*h[i], batch, length, dim) ||
+                     moved_in_place(*h[i], batch, length)))
+            return refuse("rotary: results that overlap, or heads turned in place with other "
+                          "strides");
         if (some && i == 1 && a.h[0].heads && a.h[0].out == h[1]->out)
             return refuse("rotary: queries and keys turned into the same place");
         ppdl::RotaryHeads &o = a.h[i];

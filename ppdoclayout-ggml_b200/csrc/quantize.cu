@@ -196,7 +196,8 @@ __global__ void quantize_row_kernel(const T *x, long long ldx, int K, int8_t *q,
         m = max(m, __float_as_uint(fabsf(to_float(x[i]))));
     const Divisor d(row_max<512>(m, sh));
     if (threadIdx.x == 0) scale[row] = d.s;
-    for (unsigned i = threadIdx.x; i < (unsigned)K; i += blockDim.x) q[i] = (int8_t)d(to_float(x[i]));
+    for (unsigned i = threadIdx.x; i < (unsigned)K; i += blockDim.x)
+        q[i] = (int8_t)d(to_float(x[i]));
 }
 
 }  // namespace

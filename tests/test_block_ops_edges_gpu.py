@@ -333,7 +333,8 @@ def test_first_call_of_a_new_thread(cuda):
     calls = [lambda: ppdl.linear_i8(few, wq, ws), lambda: ppdl.linear_i8(few[:1], wq, ws),
              lambda: ppdl.linear_i8(q, wq, ws, x_scale=s), lambda: ppdl.linear_i8(x, wq, ws), gemm,
              lambda: ppdl.quantize_rows(x)[0], lambda: ppdl.layernorm(x),
-             lambda: ppdl.layernorm_backward(x, x, None, mean, rstd)[1], lambda: ppdl.rotary(heads, None, pos, freq, (32,))[0]]
+             lambda: ppdl.layernorm_backward(x, x, None, mean, rstd)[1],
+             lambda: ppdl.rotary(heads, None, pos, freq, (32,))[0]]
     want = [f() for f in calls]
     torch.cuda.synchronize()
     for f, w in zip(calls, want):
